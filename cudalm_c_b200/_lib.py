@@ -117,6 +117,12 @@ PROTOTYPES = {
     "qlmb_dec_attn": (ci, [vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, vp]),
     "qlmb_dec_greedy": (ci, [vp, vp, vp, ci, ci, vp]),
     "qlmb_dec_sample": (ci, [vp, vp, vp, vp, ci, ci, vp]),
+    "qlmb_dec_rope_kv": (ci, [vp] * 9 + [ci] * 8 + [vp]),
+    "qlmb_dec_attn_prefix_bytes": (sz, [ci] * 6),
+    "qlmb_dec_attn_prefix": (ci, [vp] * 8 + [ci] * 8 + [vp, sz, vp]),
+    "qlmb_dec_verify": (ci, [vp, vp, vp, vp, ci, C.c_longlong, vp, C.c_longlong, vp, vp, vp, vp, ci, ci, ci, vp]),
+    "qlmb_lora_bytes": (sz, [ci] * 4),
+    "qlmb_lora_add": (ci, [vp, vp, vp, ci, vp, vp, vp, ci, vp, vp, ci, ci, ci, ci, vp, sz, vp]),
     "qlmb_attn_fwd": (ci, [vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, vp]),
     "qlmb_attn_bwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, vp]),
     "qlmb_attn_bwd_rope": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, vp]),
@@ -213,6 +219,25 @@ def ptr(t):
     if isinstance(t, np.ndarray):
         return t.ctypes.data
     return t.data_ptr()
+
+
+def need(name, t, dtype, *shape):
+    """Checks an argument of a mirror: a contiguous CUDA tensor of the current device, of `dtype` (one or several) and `shape` (None: any
+    size).  The library takes addresses, so a tensor of another kind, shape or device would be read as something else."""
+    import torch
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: a tensor, got %s" % (name, type(t).__name__))
+    if t.dtype != dtype if isinstance(dtype, torch.dtype) else t.dtype not in dtype:
+        raise TypeError("%s: elements of type %s, got %s" % (name, dtype, t.dtype))
+    if len(t.shape) != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
+        raise ValueError("%s: shape %s, got %s" % (name, shape, tuple(t.shape)))
+    if not t.is_contiguous():
+        raise ValueError("%s: not contiguous" % name)
+    if not t.is_cuda:
+        raise ValueError("%s: on %s, a CUDA tensor is needed" % (name, t.device))
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError("%s: on %s, the current device is cuda:%d" % (name, t.device, torch.cuda.current_device()))
+    return t
 
 
 class _Calls:

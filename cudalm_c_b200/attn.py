@@ -2,7 +2,7 @@
 attention part of gpu_backward, cudalm.cu:5918-5960) over the C ABI."""
 import torch
 
-from ._lib import calls, check, lib, ptr, stream_ptr
+from ._lib import calls, check, lib, need, ptr, stream_ptr
 
 
 def attn_fwd(Q, K, V, B, T, H, KV, win=0):
@@ -24,3 +24,25 @@ def attn_bwd(Q, K, V, O, dA, lse, B, T, H, KV, win=0, rope=None):
         check(lib().qlmb_attn_bwd_rope(ptr(dQ), ptr(dK), ptr(dV), ptr(drow), ptr(Q), ptr(K), ptr(V), ptr(O), ptr(dA), ptr(lse),
                                        ptr(rope[0]), ptr(rope[1]), B, T, H, KV, 64, win, stream_ptr()))
     return dQ, dK, dV, drow
+
+
+def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
+    """Attention of a decode step over a prefix that the slots share: Q [B*n, H*64], Kp and Vp [P, KD], caches Kc and Vc [B, Tm, KD]
+    bf16, pos [B] int32 = absolute position of each slot's first new token (its cache row is pos - P).  Returns O [B*n, H*64] bf16 and
+    the scores' log-sum-exp [B*n, H] fp32."""
+    bf = torch.bfloat16
+    B = need("pos", pos, torch.int32, None).shape[0]
+    Tm, KD = need("Kc", Kc, bf, B, None, None).shape[1:]
+    need("Vc", Vc, bf, B, Tm, KD)
+    P = need("Kp", Kp, bf, None, KD).shape[0]
+    need("Vp", Vp, bf, P, KD)
+    rows = need("Q", Q, bf, None, H * 64).shape[0]
+    if KD % 64 or B == 0 or rows % B:
+        raise ValueError("dec_attn_prefix: %d rows of queries for %d slots, keys of %d columns" % (rows, B, KD))
+    shape = (B, rows // B, P, Tm, H, KD // 64)
+    nbytes = lib().qlmb_dec_attn_prefix_bytes(*shape)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=Q.device)
+    O = torch.empty_like(Q)
+    lse = torch.empty(rows, H, dtype=torch.float32, device=Q.device)
+    calls.dec_attn_prefix(O, lse, Q, Kp, Vp, Kc, Vc, pos, win, *shape, 64, ws, nbytes, stream_ptr())
+    return O, lse

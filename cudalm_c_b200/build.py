@@ -39,6 +39,9 @@ UNITS = {
     "qlmb_comm.cu": [],
     "qlmb_attn.cu": [],
     "qlmb_block.cu": [],
+    "qlmb_prefix.cu": [],
+    "qlmb_verify.cu": [],
+    "qlmb_lora.cu": [],
 }
 COMMON = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
           "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]

@@ -92,6 +92,17 @@ CALL(gnorm, 8, ARG_P(0); ARG_U(1); ARG_P(2); ARG_P(3); ARG_I(4); ARG_I(5); ARG_P
 CALL(dec_step, 2, ARG_P(0); ARG_P(1), p0, p1)
 CALL(dec_greedy, 6, ARG_P(0); ARG_P(1); ARG_P(2); ARG_I(3); ARG_I(4); ARG_P(5), p0, p1, p2, i3, i4, p5)
 
+CALL(dec_rope_kv, 18, ARG_P(0); ARG_P(1); ARG_P(2); ARG_P(3); ARG_P(4); ARG_P(5); ARG_P(6); ARG_P(7); ARG_P(8); ARG_I(9); ARG_I(10);
+     ARG_I(11); ARG_I(12); ARG_I(13); ARG_I(14); ARG_I(15); ARG_I(16); ARG_P(17),
+     p0, p1, p2, p3, p4, p5, p6, p7, p8, i9, i10, i11, i12, i13, i14, i15, i16, p17)
+CALL(dec_attn_prefix, 19, ARG_P(0); ARG_P(1); ARG_P(2); ARG_P(3); ARG_P(4); ARG_P(5); ARG_P(6); ARG_P(7); ARG_I(8); ARG_I(9); ARG_I(10);
+     ARG_I(11); ARG_I(12); ARG_I(13); ARG_I(14); ARG_I(15); ARG_P(16); ARG_U(17); ARG_P(18),
+     p0, p1, p2, p3, p4, p5, p6, p7, i8, i9, i10, i11, i12, i13, i14, i15, p16, (size_t)u17, p18)
+CALL(dec_verify, 16, ARG_P(0); ARG_P(1); ARG_P(2); ARG_P(3); ARG_I(4); ARG_U(5); ARG_P(6); ARG_U(7); ARG_P(8); ARG_P(9); ARG_P(10); ARG_P(11);
+     ARG_I(12); ARG_I(13); ARG_I(14); ARG_P(15), p0, p1, p2, p3, i4, (long long)u5, p6, (long long)u7, p8, p9, p10, p11, i12, i13, i14, p15)
+CALL(lora_add, 17, ARG_P(0); ARG_P(1); ARG_P(2); ARG_I(3); ARG_P(4); ARG_P(5); ARG_P(6); ARG_I(7); ARG_P(8); ARG_P(9); ARG_I(10); ARG_I(11);
+     ARG_I(12); ARG_I(13); ARG_P(14); ARG_U(15); ARG_P(16), p0, p1, p2, i3, p4, p5, p6, i7, p8, p9, i10, i11, i12, i13, p14, (size_t)u15, p16)
+
 static PyObject *set_error_class(PyObject *self, PyObject *cls)
 {
     (void)self;
@@ -105,6 +116,7 @@ static PyMethodDef methods[] = {
     ENTRY(gemv_decode), ENTRY(linear_fwd), ENTRY(linear_dgrad), ENTRY(linear_wgrad), ENTRY(gemm_nt), ENTRY(embed), ENTRY(rmsnorm_fwd),
     ENTRY(rmsnorm_bwd), ENTRY(rope), ENTRY(attn_fwd), ENTRY(attn_bwd), ENTRY(moe_forward), ENTRY(moe_decode), ENTRY(moe_backward), ENTRY(adamw),
     ENTRY(step), ENTRY(gnorm), ENTRY(dec_step), ENTRY(dec_greedy),
+    ENTRY(dec_rope_kv), ENTRY(dec_attn_prefix), ENTRY(dec_verify), ENTRY(lora_add),
     {"set_error_class", set_error_class, METH_O, NULL},
     {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycalls", NULL, -1, methods, NULL, NULL, NULL, NULL};

@@ -6,7 +6,7 @@ KN = codes of W[K,N] (the reference's own [in,out] storage, applied with g_ab),
 NK = codes of W[N,K] (applied with g_abt)."""
 import torch
 
-from ._lib import BF16, F32, KN, NK, Qkv, calls, check, lib, ptr, stream_ptr  # noqa: F401
+from ._lib import BF16, F32, KN, NK, Qkv, calls, check, lib, need, ptr, stream_ptr  # noqa: F401
 
 
 def _dt(t):
@@ -71,4 +71,29 @@ def gemv_decode(X, codes, scales, layout, N, out=None):
     B, K = X.shape
     Y = out if out is not None else X.new_empty((B, N))
     calls.gemv_decode(Y, X, codes, scales, layout, B, K, N, _dt(X), stream_ptr())
+    return Y
+
+
+def lora_order(adapter):
+    """The rows in the order of their adapters (int32), for lora_add: made once for as long as a batch stays the same."""
+    return torch.argsort(adapter, stable=True).to(torch.int32)
+
+
+def lora_add(X, base, A, Bm, scale, adapter, order=None, out=None):
+    """base + scale[a] * (X A[a]^T) Bm[a] row by row, a = adapter[m] (-1: base): X [M, K], base [M, N] (fp32 or bf16), A [n, R, K] and Bm
+    [n, R, N] bf16, scale [n] fp32, adapter [M] int32.  out may be base."""
+    bf = torch.bfloat16
+    M, K = need("X", X, (bf, torch.float32), None, None).shape
+    N = need("base", base, X.dtype, M, None).shape[1]
+    n, R = need("A", A, bf, None, None, K).shape[:2]
+    need("Bm", Bm, bf, n, R, N)
+    need("scale", scale, torch.float32, n)
+    need("adapter", adapter, torch.int32, M)
+    if order is not None:
+        need("order", order, torch.int32, M)
+    Y = torch.empty_like(base) if out is None else need("out", out, X.dtype, M, N)
+    if M:
+        nbytes = lib().qlmb_lora_bytes(M, K, N, R)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=X.device)
+        calls.lora_add(Y, X, base, _dt(X), A, Bm, scale, n, adapter, order, M, K, N, R, ws, nbytes, stream_ptr())
     return Y

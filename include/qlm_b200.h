@@ -661,6 +661,51 @@ int qlmb_dec_sample(int *out, float *lp, const float *logits, const qlmb_dec_sam
  * index on ties), lp[b] = its log-probability. */
 int qlmb_dec_greedy(int *out, float *lp, const float *logits, int B, int V, void *stream);
 
+/* ---- a decode step for many requests at once (no counterpart in the reference, whose slots hold their prompts themselves and
+ * take one token a step) ----
+ * B slots share the keys and values of the first P positions (one prompt in front of all of them) and bring n new tokens each, the
+ * last one picked and drafts behind it.  pos[b] (device) is the absolute position of slot b's first new token; row j of its own
+ * cache [B][Tm][KV*hd] is position P + j.  Rows of q, k, v and O are tokens b*n + i; head dimension 64, bf16.  A slot whose new
+ * tokens do not all lie in its cache is reported through the device error word and left as it is.
+ *
+ * qlmb_dec_rope_kv: qlmb_dec_rope on q and k (position pos[b] + i; tables of Tr rows) and qlmb_dec_kv for n tokens in one launch:
+ * Qo = q rotated (may be q), Kc and Vc receive the rotated keys and the values.  All pointers but pos 16-byte aligned.  Site 305. */
+int qlmb_dec_rope_kv(void *Qo, void *Kc, void *Vc, const void *q, const void *k, const void *v, const float *cosb, const float *sinb,
+                     const int *pos, int B, int n, int P, int Tm, int H, int KV, int hd, int Tr, void *stream);
+/* qlmb_dec_attn over the shared rows Kp, Vp [P][KV*hd] and the slots' own: token i of slot b sees positions
+ * max(0, pos[b]+i-win+1) .. pos[b]+i (win <= 0: all of them from 0), its own and the earlier new tokens' among them, which the
+ * caller has appended.  pos[b] = P - 1 is allowed: the slot's first token then sees shared rows only.  O [B*n][H*hd]; lse (may be
+ * NULL) [B*n][H] = log of the sum of exp(scores); a token that sees nothing gives zeros and -inf.  What lies in rows that a token does not
+ * see has no influence on it, be it infinite or NaN.  P = 0 is allowed (Kp, Vp may then be NULL).  n <= 64; any Tm and P with
+ * P + Tm < 2^30.  ws: qlmb_dec_attn_prefix_bytes(...) bytes (0: the shape is not supported), 16-byte aligned, written and read by
+ * the call only; calls that may overlap need one each.  Site 306. */
+size_t qlmb_dec_attn_prefix_bytes(int B, int n, int P, int Tm, int H, int KV);
+int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const void *Kp, const void *Vp, const void *Kc, const void *Vc, const int *pos,
+                         int win, int B, int n, int P, int Tm, int H, int KV, int hd, void *ws, size_t ws_bytes, void *stream);
+/* Drafted tokens against the model's logits, beside qlmb_dec_sample.  Slot b has nd[b] drafts (nd NULL: n) draft[b][0..] and logits
+ * rows [b][0..nd[b]] of V tokens, fp32 or bf16, `ld` elements apart ([B][n+1][ld]); q [B][n][ldq] are the probabilities the drafts
+ * were drawn from (NULL: they were certain).  With p_i = softmax(logits[b][i] / temp[b]), draft i is taken while
+ * u[b][i] * q_i(draft) < p_i(draft); the first that is not is replaced by a draw from max(0, p_i - q_i) (from p_i where that is all
+ * zero), behind the last comes a draw from p_nd; the draw is the lowest token whose cumulated weight passes u[b][n] times the
+ * whole.  u [B][n+1] are uniform numbers in [0, 1).  temp[b] <= 0: a draft is taken while it is the arg-max (lowest index on ties),
+ * the token behind is the arg-max; q and u do not matter.  Logits of -inf are tokens that are cut (top-k, top-p).
+ * out [B][n+1] = the tokens taken and the one behind them, then -1; count [B] = how many; lp [B][n+1] = their log-probabilities
+ * under the unmodified distribution, 0 behind them.  nd[b] < 0: no slot (count 0, nothing read).  A row that is reached and holds
+ * a NaN, +inf or nothing above -inf (site 309), a draft that is tested and no token (308) and nd[b] > n (310) are reported; the slot
+ * ends in front of it without a draw.  n <= 63. */
+int qlmb_dec_verify(int *out, int *count, float *lp, const void *logits, int lg_dtype, long long ld, const float *q, long long ldq,
+                    const int *draft, const int *nd, const float *u, const float *temp, int B, int n, int V, void *stream);
+/* Low-rank adapters of many requests beside a projection their rows share (qlmb_linear_fwd, qlmb_gemv_decode):
+ * Y[m,:] = base[m,:] + scale[a] * (X[m,:] A[a]^T) Bm[a] with a = adapter[m], Y[m,:] = base[m,:] where a is -1.  X [M][K], base and Y
+ * [M][N] of `dtype` (Y may be base); A [adapters][R][K] and Bm [adapters][R][N] bf16; scale [adapters]; adapter [M] (device).
+ * order (may be NULL): the rows 0 .. M-1 in the order of their adapters; without it rows in any order give the same result, but
+ * 16 neighbouring rows cost as many passes as they have adapters.  K, N and R multiples of 8, R <= 256 (adapters of a lower rank:
+ * zero rows).  Pointers to rows, adapters and ws 16-byte aligned; ws: qlmb_lora_bytes(...) bytes (0: not supported), written and read by
+ * the call only.  An adapter or an entry of order out of range is reported (site 307); the row then takes its base, resp. is left out. */
+size_t qlmb_lora_bytes(int M, int K, int N, int R);
+int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype, const void *A, const void *Bm, const float *scale, int adapters,
+                  const int *adapter, const int *order, int M, int K, int N, int R, void *ws, size_t ws_bytes, void *stream);
+
 /* ---- attention (rows of Q/K/V/O are tokens b*T + t; head h occupies columns [h*hd, (h+1)*hd)) ----
  * e_attn / k_attn_fwd (cudalm.cu:3705-3730; CPU twin cpu_kern.h:166-229): causal attention with an
  * optional window (win > 0: keys t-win+1 .. t), grouped-query heads (head h reads K/V head
