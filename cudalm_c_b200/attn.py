@@ -2,7 +2,7 @@
 attention part of gpu_backward, cudalm.cu:5918-5960) over the C ABI."""
 import torch
 
-from ._lib import calls, check, lib, need, ptr, stream_ptr
+from ._lib import alike, calls, check, device_index, lib, need, ptr, stream_ptr
 
 
 def attn_fwd(Q, K, V, B, T, H, KV, win=0):
@@ -26,10 +26,10 @@ def attn_bwd(Q, K, V, O, dA, lse, B, T, H, KV, win=0, rope=None):
     return dQ, dK, dV, drow
 
 
-def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
-    """Attention of a decode step over a prefix that the slots share: Q [B*n, H*64], Kp and Vp [P, KD], caches Kc and Vc [B, Tm, KD]
-    bf16, pos [B] int32 = absolute position of each slot's first new token (its cache row is pos - P).  Returns O [B*n, H*64] bf16 and
-    the scores' log-sum-exp [B*n, H] fp32."""
+_prefix_ws = {}                                          # bytes of dec_attn_prefix's scratch by device and shape
+
+
+def _dec_attn_prefix_args(Q, Kp, Vp, Kc, Vc, pos, H):
     bf = torch.bfloat16
     B = need("pos", pos, torch.int32, None).shape[0]
     Tm, KD = need("Kc", Kc, bf, B, None, None).shape[1:]
@@ -37,12 +37,30 @@ def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
     P = need("Kp", Kp, bf, None, KD).shape[0]
     need("Vp", Vp, bf, P, KD)
     rows = need("Q", Q, bf, None, H * 64).shape[0]
-    if KD % 64 or B == 0 or rows % B:
-        raise ValueError("dec_attn_prefix: %d rows of queries for %d slots, keys of %d columns" % (rows, B, KD))
+    raise ValueError("dec_attn_prefix: %d rows of queries for %d slots, keys of %d columns, a cache of %d rows" % (rows, B, KD, Tm))
+
+
+def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
+    """Attention of a decode step over a prefix that the slots share: Q [B*n, H*64], Kp and Vp [P, KD], caches Kc and Vc [B, Tm, KD]
+    bf16, pos [B] int32 = absolute position of each slot's first new token (its cache row is pos - P).  Returns O [B*n, H*64] bf16 and
+    the scores' log-sum-exp [B*n, H] fp32."""
+    dev = device_index()
+    try:
+        B, Tm, KD = Kc.shape
+        rows, width = Q.shape
+        P, kd = Kp.shape
+        good = (alike(dev, torch.bfloat16, Q, Kp, Vp, Kc, Vc) and alike(dev, torch.int32, pos) and pos.shape == (B,) and Vc.shape == Kc.shape and
+                Vp.shape == Kp.shape and kd == KD and width == H * 64 and KD % 64 == 0 and B > 0 and rows % B == 0 and rows > 0)
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        _dec_attn_prefix_args(Q, Kp, Vp, Kc, Vc, pos, H)
     shape = (B, rows // B, P, Tm, H, KD // 64)
-    nbytes = lib().qlmb_dec_attn_prefix_bytes(*shape)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=Q.device)
+    nbytes = _prefix_ws.get((dev, shape))
+    if nbytes is None:
+        nbytes = _prefix_ws[(dev, shape)] = lib().qlmb_dec_attn_prefix_bytes(*shape)
     O = torch.empty_like(Q)
-    lse = torch.empty(rows, H, dtype=torch.float32, device=Q.device)
+    lse = torch.empty((rows, H), dtype=torch.float32, device=Q.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device) if nbytes else None
     calls.dec_attn_prefix(O, lse, Q, Kp, Vp, Kc, Vc, pos, win, *shape, 64, ws, nbytes, stream_ptr())
     return O, lse

@@ -2,7 +2,7 @@
 k_embed, k_embed_bwd, k_softmax_ce; cudalm.cu:3630-3645, 5740, 5838, 6000) over the C ABI."""
 import torch
 
-from ._lib import BF16, F32, calls, check, lib, need, ptr, stream_ptr
+from ._lib import BF16, F32, alike, calls, check, device_index, lib, need, ptr, stream_ptr
 
 
 def _dt(t):
@@ -132,10 +132,7 @@ def nggate_bwd(dy, v, hn, kn, g, rh, rk):
     return dv, dk
 
 
-def dec_rope_kv(q, k, v, Kc, Vc, cosb, sinb, pos, H, P=0, out=None):
-    """n new tokens of every slot: q and k rotated by their positions, keys and values into the slots' caches.  q [B*n, H*64], k and v
-    [B*n, KD], caches [B, Tm, KD] bf16 (row j is position P + j), tables [Tr, 32], pos [B] int32 = absolute position of each slot's
-    first new token.  Returns the rotated q (out may be q)."""
+def _dec_rope_kv_args(q, k, v, Kc, Vc, cosb, sinb, pos, H, out):
     bf, f32 = torch.bfloat16, torch.float32
     B = need("pos", pos, torch.int32, None).shape[0]
     Tm, KD = need("Kc", Kc, bf, B, None, None).shape[1:]
@@ -145,31 +142,69 @@ def dec_rope_kv(q, k, v, Kc, Vc, cosb, sinb, pos, H, P=0, out=None):
     need("v", v, bf, rows, KD)
     Tr = need("cosb", cosb, f32, None, 32).shape[0]
     need("sinb", sinb, f32, Tr, 32)
-    if KD % 64 or B == 0 or rows % B:
-        raise ValueError("dec_rope_kv: %d rows for %d slots, keys of %d columns" % (rows, B, KD))
-    Qo = torch.empty_like(q) if out is None else need("out", out, bf, rows, H * 64)
-    if rows:
-        calls.dec_rope_kv(Qo, Kc, Vc, q, k, v, cosb, sinb, pos, B, rows // B, P, Tm, H, KD // 64, 64, Tr, stream_ptr())
-    return Qo
+    need("out", out, bf, rows, H * 64)
+    raise ValueError("dec_rope_kv: %d rows for %d slots, keys of %d columns" % (rows, B, KD))
+
+
+def dec_rope_kv(q, k, v, Kc, Vc, cosb, sinb, pos, H, P=0, out=None):
+    """n new tokens of every slot: q and k rotated by their positions, keys and values into the slots' caches.  q [B*n, H*64], k and v
+    [B*n, KD], caches [B, Tm, KD] bf16 (row j is position P + j), tables [Tr, 32], pos [B] int32 = absolute position of each slot's
+    first new token.  Returns the rotated q (out may be q)."""
+    dev = device_index()
+    try:
+        B, Tm, KD = Kc.shape
+        rows, width = q.shape
+        Tr, half = cosb.shape
+        if out is None:
+            out = torch.empty_like(q)
+        good = (alike(dev, torch.bfloat16, q, k, v, Kc, Vc, out) and alike(dev, torch.float32, cosb, sinb) and alike(dev, torch.int32, pos) and
+                pos.shape == (B,) and Vc.shape == Kc.shape and k.shape == v.shape == (rows, KD) and out.shape == q.shape and
+                sinb.shape == cosb.shape and half == 32 and width == H * 64 and KD % 64 == 0 and B > 0 and rows % B == 0 and rows > 0)
+    except (AttributeError, ValueError, TypeError):
+        good = False
+    if not good:
+        _dec_rope_kv_args(q, k, v, Kc, Vc, cosb, sinb, pos, H, out)
+    calls.dec_rope_kv(out, Kc, Vc, q, k, v, cosb, sinb, pos, B, rows // B, P, Tm, H, KD // 64, 64, Tr, stream_ptr())
+    return out
+
+
+def _dec_verify_args(logits, draft, u, temp, q, nd, V):
+    f32, i32 = torch.float32, torch.int32
+    B, n1, ld = need("logits", logits, (f32, torch.bfloat16), None, None, None).shape
+    need("draft", draft, i32, B, n1 - 1)
+    need("u", u, f32, B, n1)
+    need("temp", temp, f32, B)
+    if q is not None:
+        need("q", q, f32, B, n1 - 1, None)
+    if nd is not None:
+        need("nd", nd, i32, B)
+    raise ValueError("dec_verify: %d slots" % B)
 
 
 def dec_verify(logits, draft, u, temp, q=None, nd=None, V=None):
     """Drafted tokens against the model's logits [B, n+1, ld] (fp32 or bf16; the first V columns are tokens): draft [B, n] int32, u
     [B, n+1] uniform numbers, temp [B] (0: greedy), q [B, n, ldq] the probabilities the drafts were drawn from (None: certain), nd [B] int32
     drafts per slot (None: n).  Returns (tokens [B, n+1], -1 behind the last; how many [B]; log-probabilities [B, n+1])."""
-    f32, i32 = torch.float32, torch.int32
-    B, n1, ld = need("logits", logits, (f32, torch.bfloat16), None, None, None).shape
-    n = n1 - 1
-    V = ld if V is None else V
-    need("draft", draft, i32, B, n)
-    need("u", u, f32, B, n1)
-    need("temp", temp, f32, B)
-    ldq = need("q", q, f32, B, n, None).shape[2] if q is not None else 0
-    if nd is not None:
-        need("nd", nd, i32, B)
-    out = torch.empty(B, n1, dtype=i32, device=logits.device)
-    count = torch.empty(B, dtype=i32, device=logits.device)
-    lp = torch.empty(B, n1, dtype=f32, device=logits.device)
-    if B:
-        calls.dec_verify(out, count, lp, logits, _dt(logits), ld, q if n else None, ldq, draft if n else None, nd, u, temp, B, n, V, stream_ptr())
+    dev = device_index()
+    try:
+        B, n1, ld = logits.shape
+        n = n1 - 1
+        dt = logits.dtype
+        good = (B > 0 and (dt is torch.float32 or dt is torch.bfloat16) and alike(dev, dt, logits) and alike(dev, torch.float32, u, temp) and
+                alike(dev, torch.int32, draft) and draft.shape == (B, n) and u.shape == (B, n1) and temp.shape == (B,))
+        ldq = 0
+        if good and q is not None:
+            ldq = q.shape[2]
+            good = alike(dev, torch.float32, q) and q.shape == (B, n, ldq)
+        if good and nd is not None:
+            good = alike(dev, torch.int32, nd) and nd.shape == (B,)
+    except (AttributeError, ValueError, IndexError):
+        good = False
+    if not good:
+        _dec_verify_args(logits, draft, u, temp, q, nd, V)
+    out = torch.empty((B, n1), dtype=torch.int32, device=logits.device)
+    count = torch.empty_like(temp, dtype=torch.int32)
+    lp = torch.empty_like(u)
+    calls.dec_verify(out, count, lp, logits, F32 if dt is torch.float32 else BF16, ld, q if n else None, ldq, draft if n else None, nd, u, temp,
+                     B, n, ld if V is None else V, stream_ptr())
     return out, count, lp

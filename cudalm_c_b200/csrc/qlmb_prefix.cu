@@ -348,20 +348,29 @@ __global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParam
     if (p.lse && lane == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mref + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Pieces of a call: enough CTAs for the device, at least 128 keys (32 a warp) in each.
-struct PxPlan { int Sp, So, rt_own, rt_pre; };
-static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV)
+// Pieces of a call.
+struct PxPlan { int Sp, So, rt_own, rt_pre, tc, per; };
+static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
 {
-    PxPlan pl;
-    const long long want = 4LL * sm_count();
+    PxPlan pl = {};
+    const long long want = 3LL * sm_count();
+    const long long rows = (long long)B * n * (H / KV);
     pl.rt_own = (n * (H / KV) + 15) / 16;
-    pl.rt_pre = (int)(((long long)B * n * (H / KV) + 15) / 16);
-    const auto pieces = [&](long long items, long long keys) {
-        const long long most = (keys + 127) / 128, s = (want + items - 1) / items;
+    pl.rt_pre = (int)((rows + 15) / 16);
+    const auto pieces = [](long long want, long long items, long long keys) {
+        const long long most = (keys + 127) / 128, s = want / items;
         return (int)(s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s);
     };
-    pl.So = pieces((long long)B * KV * pl.rt_own, Tm);
-    pl.Sp = P > 0 ? pieces((long long)KV * pl.rt_pre, P) : 0;
+    pl.So = pieces(want, (long long)B * KV * pl.rt_own, Tm);
+    if (P > 0) {
+        pl.tc = rows > 16 && win <= 0;
+        if (pl.tc) {
+            const int tiles = (P + 127) / 128, s = pieces(2LL * sm_count(), KV * ((rows + 127) / 128), P);
+            pl.per = (tiles + s - 1) / s;
+            pl.Sp = (tiles + pl.per - 1) / pl.per;
+        } else
+            pl.Sp = pieces(want, (long long)KV * pl.rt_pre, P);
+    }
     return pl;
 }
 static bool px_shape_ok(int B, int n, int P, int Tm, int H, int KV)
@@ -393,8 +402,8 @@ extern "C" int qlmb_dec_rope_kv(void *Qo, void *Kc, void *Vc, const void *q, con
 extern "C" size_t qlmb_dec_attn_prefix_bytes(int B, int n, int P, int Tm, int H, int KV)
 {
     if (!px_shape_ok(B, n, P, Tm, H, KV)) return 0;
-    const PxPlan pl = px_plan(B, n, P, Tm, H, KV);
-    const size_t S = (size_t)pl.Sp + pl.So;
+    const PxPlan pl = px_plan(B, n, P, Tm, H, KV, 0), pw = px_plan(B, n, P, Tm, H, KV, 1);
+    const size_t S = (size_t)pl.So + (pl.Sp > pw.Sp ? pl.Sp : pw.Sp);
     return S * (size_t)B * n * H * (PX_HD + 1) * sizeof(float) + 16;
 }
 
@@ -409,7 +418,7 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
                  "qlmb_dec_attn_prefix: rows, caches and workspace must be 16-byte aligned");
     const size_t need = qlmb_dec_attn_prefix_bytes(B, n, P, Tm, H, KV);
     QLMB_REQUIRE(ws_bytes >= need, "qlmb_dec_attn_prefix: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
-    const PxPlan pl = px_plan(B, n, P, Tm, H, KV);
+    const PxPlan pl = px_plan(B, n, P, Tm, H, KV, win);
     PxParams p = {};
     const size_t rows = (size_t)B * n * H;
     p.O = (bf16 *)O; p.lse = lse; p.Q = (const bf16 *)Q;
@@ -418,12 +427,17 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     p.B = B; p.n = n; p.P = P; p.Tm = Tm; p.H = H; p.KV = KV; p.G = H / KV;
     p.win = win < (1 << 30) ? win : 0;                                 // such a window hides nothing
     p.Sp = pl.Sp; p.So = pl.So; p.rt_own = pl.rt_own; p.rt_pre = pl.rt_pre;
-    const long long own_items = (long long)B * KV * pl.rt_own * pl.So, items = own_items + (long long)KV * pl.rt_pre * pl.Sp;
+    const long long own_items = (long long)B * KV * pl.rt_own * pl.So, items = own_items + (pl.tc ? 0 : (long long)KV * pl.rt_pre * pl.Sp);
     QLMB_REQUIRE(items < (1LL << 31), "qlmb_dec_attn_prefix: %lld pieces are too many", items);
     p.own_items = (int)own_items;
     p.scale_log2 = 1.4426950408889634f * 0.125f;
     p.errword = device_error_word();
     cudaStream_t st = as_stream(stream);
+    if (pl.tc) {
+        const PrefixAttn px = {p.Q, p.part_o, p.part_l, rows, (int)(rows / KV), pl.Sp, pl.per};
+        const int rc = attn_prefix_launch(px, Kp, Vp, P, H, KV, st);
+        if (rc) return rc;
+    }
     QLMB_CUDA(pdl_launch_small(k_px_mma, dim3((unsigned)items), dim3(128), 0, st, p));
     QLMB_LAUNCH_CHECK("k_px_mma");
     if (pl.Sp + pl.So > 1) {
