@@ -1,12 +1,18 @@
 // Verification of drafted tokens against the model's logits (speculative sampling), beside the pick of one token in qlmb_block.cu.
 //
-// Slot b has nd drafted tokens x_0 .. x_{nd-1} from distributions q_i and nd + 1 rows of logits; p_i = softmax(logits_i / T).
-// Token i is taken when u_i q_i(x_i) < p_i(x_i).  At the first that is not, the slot ends with a token drawn from max(0, p_i - q_i)
-// (from p_i where that is nothing), after the last with one from p_nd: the tokens are distributed as the model's own.
-// The draw is the lowest token whose cumulated weight passes u times the whole; weights and sums are in 64 bits, for a draw next
-// to a border is decided by them.
+// Slot b has nd drafted tokens x_0 .. x_{nd-1} from distributions q_i and nd + 1 rows of logits.  With m_i the largest logit of row
+// i, e_i(v) = exp((l_i(v) - m_i) / T) and Z_i their sum, token i is taken when u_i q_i(x_i) Z_i < e_i(x_i).  At the first that is not,
+// the slot ends with a token drawn by the weights max(0, e_i - q_i Z_i) (by e_i where that is nothing), after the last with one drawn by
+// e_nd: the tokens are distributed as the model's own.  The draw is the lowest token whose cumulated weight passes u times the whole.
+// Weights are fp32 (2^-21 of themselves), sums of more than a few of them 64 bits: a cumulated weight of V tokens is then off by
+// about 2^-22 / sqrt(V) of the whole, and a draw differs from the exact one's with a probability of 2^-22 sqrt(V).
+//
+// A slot is a cluster of eight CTAs, a row of logits is cut into runs, one a warp.  A lane keeps maximum, lowest index of it and
+// the two sums (T, and 1 for the log-probability) of what it reads, rescaled as the maximum moves; lanes are joined at the end of a
+// run, warps and CTAs through (distributed) shared memory.  The run that holds the draw is read once more.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
+#include <float.h>
 #include <math.h>
 #include "qlmb_common.cuh"
 #include "qlmb_internal.h"
@@ -16,8 +22,6 @@ namespace cg = cooperative_groups;
 namespace qlmb {
 
 constexpr int VF_C = 8;                       // CTAs of a slot: one cluster
-constexpr int VF_T = 256;
-constexpr int VF_W = VF_T / 32;
 constexpr int VF_ROWS = 64;                   // rows of logits of a slot, at most
 
 struct VerifyParams {
@@ -26,14 +30,37 @@ struct VerifyParams {
     const void *logits;
     const float *q, *u, *temp;
     const int *draft, *nd;
-    int dtype, B, n, V;
+    int B, n, V, group;                       // group: rows that are read before the drafts among them are tested
     long long ld, ldq;                        // elements from a row of logits / of q to the next
     int *errword;
 };
 
-__device__ __forceinline__ float vf_ld(const void *p, int dtype, size_t i)
+__device__ __forceinline__ float vf_ex2(float x)      // 2^x (ex2.approx: 2 ulp; 0 -> 1, -inf -> 0)
 {
-    return dtype == QLMB_F32 ? reinterpret_cast<const float *>(p)[i] : __bfloat162float(reinterpret_cast<const bf16 *>(p)[i]);
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF> __device__ __forceinline__ float vf_ld(const void *p, size_t i)
+{
+    return BF ? __bfloat162float(reinterpret_cast<const bf16 *>(p)[i]) : reinterpret_cast<const float *>(p)[i];
+}
+// Four neighbouring logits, in one load where VEC; -inf from place `end` on.
+template <bool BF, bool VEC> __device__ __forceinline__ float4 vf_ld4(const void *p, size_t base, int v, int end)
+{
+    float4 r = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (VEC && v + 4 <= end) {
+        if (BF) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const bf16 *>(p) + base + v);
+            return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+        }
+        return *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + base + v);
+    }
+    if (v < end) r.x = vf_ld<BF>(p, base + v);
+    if (v + 1 < end) r.y = vf_ld<BF>(p, base + v + 1);
+    if (v + 2 < end) r.z = vf_ld<BF>(p, base + v + 2);
+    if (v + 3 < end) r.w = vf_ld<BF>(p, base + v + 3);
+    return r;
 }
 __device__ __forceinline__ double vf_warp_sum(double x)
 {
@@ -42,21 +69,24 @@ __device__ __forceinline__ double vf_warp_sum(double x)
     return x;
 }
 
-__global__ void __cluster_dims__(VF_C, 1, 1) __launch_bounds__(VF_T) k_dec_verify(const VerifyParams p)
+// A run or a row: its largest logit and the lowest index of it, the sums relative to it, whether all is finite or -inf.
+struct VfPart { double st; float s1, m; int arg, odd; };
+
+// 2^((a - b) it) for maxima a <= b, -inf for "none" (which have no sum)
+__device__ __forceinline__ double vf_scale(float a, float b, double it) { return exp2((fmax((double)a, (double)-FLT_MAX) - fmax((double)b, (double)-FLT_MAX)) * it); }
+
+template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1, 1) __launch_bounds__(32 * VF_W, VF_W == 8 ? 4 : 7) k_dec_verify(const VerifyParams p)
 {
+    constexpr int VF_T = 32 * VF_W, RPL = VF_C * VF_W / 32;      // threads; runs of a row a lane looks at when they are joined
     cg::cluster_group cl = cg::this_cluster();
-    // of this CTA's share of a row: its maximum with the lowest index, whether something in it is no number to draw from, the
-    // sums of exp((l - m) / T) and exp(l - m); of the row that ends the slot: the two sums of weights
-    __shared__ float mx[VF_ROWS];
-    __shared__ int arg[VF_ROWS], odd[VF_ROWS];
-    __shared__ double st[VF_ROWS], s1[VF_ROWS], wsum[2], wpart[2][VF_W];
-    __shared__ float gm[VF_ROWS];
-    __shared__ int garg[VF_ROWS], gbad[VF_ROWS];
-    __shared__ double gst[VF_ROWS], gs1[VF_ROWS];
-    __shared__ float rv[VF_W];
-    __shared__ int ri[VF_W], rodd[VF_W];
-    __shared__ int end_row, end_kind;         // kind 0: draw after the drafts, 1: draw in place of a refused draft, 2: nothing to draw from
+    __shared__ VfPart warp_part[VF_ROWS][VF_W], row_part[VF_ROWS];
+    __shared__ double wtot[VF_W], wleft[VF_W];            // of the row that ends the slot: the runs' weights without the refused draft
+    __shared__ int sx[VF_ROWS];               // the drafts, their logits, u q of each
+    __shared__ float sl[VF_ROWS];
+    __shared__ double suq[VF_ROWS];
     const int b = blockIdx.x / VF_C, c = blockIdx.x % VF_C, tid = threadIdx.x, w = tid >> 5, ln = tid & 31, n = p.n;
+    pdl_trigger();
+    pdl_wait();
     const int nd = p.nd ? p.nd[b] : n;
     int *out = p.out + (size_t)b * (n + 1);
     float *lp = p.lp + (size_t)b * (n + 1);
@@ -69,170 +99,237 @@ __global__ void __cluster_dims__(VF_C, 1, 1) __launch_bounds__(VF_T) k_dec_verif
     }
     const float temp = p.temp[b];
     const bool greedy = !(temp > 0.0f);
-    const double it = greedy ? 1.0 : 1.0 / (double)temp;
-    const int slice = (p.V + VF_C - 1) / VF_C, v0 = min(c * slice, p.V), v1 = min(v0 + slice, p.V);
+    const double it = greedy ? 1.4426950408889634 : 1.4426950408889634 / (double)temp;
+    const float cT = (float)fmin(it, 1e38);
+    const bool unit = cT == 1.4426950408889634f;          // the two sums are one
+    // runs of whole groups of four
+    const int run = ((p.V + 4 * VF_C * VF_W - 1) / (4 * VF_C * VF_W)) * 4;
+    const int w0 = min((c * VF_W + w) * run, p.V), w1 = min(w0 + run, p.V);
     const size_t row0 = (size_t)b * (n + 1) * (size_t)p.ld;
-    for (int i = 0; i <= nd; i++) {
+    if (tid < nd) {
+        const int x = p.draft[(size_t)b * n + tid];
+        const bool in = x >= 0 && x < p.V;
+        sx[tid] = x;
+        sl[tid] = in ? vf_ld<BF>(p.logits, row0 + (size_t)tid * p.ld + x) : 0.0f;
+        suq[tid] = (double)p.u[(size_t)b * (n + 1) + tid] * (p.q && in ? (double)p.q[((size_t)b * n + tid) * p.ldq + x] : 1.0);
+    }
+    const int steps = (run + 511) / 512;      // of a run: 16 logits a lane
+    const auto fetch = [&](int i, int s, float4 d[4]) {   // step s of row i's run, on into the next rows
+        if (s >= steps) { i += s / steps; s %= steps; }
         const size_t base = row0 + (size_t)i * p.ld;
-        float m = -INFINITY; int a = 0x7fffffff, bad = 0;
-        for (int v = v0 + tid; v < v1; v += VF_T) {
-            const float x = vf_ld(p.logits, p.dtype, base + v);
-            bad |= !(x < INFINITY);
-            if (x > m) { m = x; a = v; }
-        }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const float om = __shfl_xor_sync(~0u, m, o); const int oa = __shfl_xor_sync(~0u, a, o);
-            if (om > m || (om == m && oa < a)) { m = om; a = oa; }
-            bad |= __shfl_xor_sync(~0u, bad, o);
-        }
-        if (ln == 0) { rv[w] = m; ri[w] = a; rodd[w] = bad; }
-        __syncthreads();
-        if (tid == 0) {
-            for (int k = 1; k < VF_W; k++) {
-                if (rv[k] > m || (rv[k] == m && ri[k] < a)) { m = rv[k]; a = ri[k]; }
-                bad |= rodd[k];
+        for (int k = 0; k < 4; k++) d[k] = vf_ld4<BF, VEC>(p.logits, base, w0 + s * 512 + 4 * ln + 128 * k, w1);
+    };
+    float4 x[4], y[4];
+    fetch(0, 0, x);
+    int r = 0, kind = -1;
+    for (int i0 = 0; i0 <= nd; i0 += p.group) {
+        const int i1 = min(i0 + p.group, nd + 1);
+        // ---- this warp's run of the rows i0 .. i1 - 1; the next step is requested ahead, the next group's first one too
+        const int total = steps * (i1 - i0);
+        float m = -INFINITY, st = 0.0f, s1 = 0.0f;
+        int arg = 0x7fffffff;
+        for (int s = 0; s < total; s++) {
+            if (s + 1 < total || i1 <= nd) fetch(i0, s + 1, y);
+            const int v = w0 + (s % steps) * 512 + 4 * ln;
+            float mx[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) mx[k] = fmaxf(fmaxf(x[k].x, x[k].y), fmaxf(x[k].z, x[k].w));
+            const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (mn > m) {                     // a new maximum: its place (the lowest of equals)
+                const float was = fmaxf(m, -FLT_MAX), d = was - fmaxf(mn, -FLT_MAX);
+                st *= vf_ex2(d * cT);
+                s1 *= vf_ex2(d * 1.4426950408889634f);
+                m = mn;
+                const int k = mx[0] == mn ? 0 : mx[1] == mn ? 1 : mx[2] == mn ? 2 : 3;
+                const float4 f = k == 0 ? x[0] : k == 1 ? x[1] : k == 2 ? x[2] : x[3];
+                arg = v + 128 * k + (f.x == mn ? 0 : f.y == mn ? 1 : f.z == mn ? 2 : 3);
             }
-            mx[i] = m; arg[i] = a; odd[i] = bad;
-        }
-        __syncthreads();
-    }
-    cl.sync();
-    for (int i = tid; i <= nd; i += VF_T) {
-        float m = -INFINITY; int a = 0x7fffffff, bad = 0;
-        for (int k = 0; k < VF_C; k++) {
-            const float om = *cl.map_shared_rank(&mx[i], k); const int oa = *cl.map_shared_rank(&arg[i], k);
-            if (om > m || (om == m && oa < a)) { m = om; a = oa; }
-            bad |= *cl.map_shared_rank(&odd[i], k);
-        }
-        gm[i] = m; garg[i] = a; gbad[i] = bad || m == -INFINITY;
-    }
-    __syncthreads();
-    for (int i = 0; i <= nd; i++) {
-        const size_t base = row0 + (size_t)i * p.ld;
-        const double m = gm[i];
-        double a = 0.0, d = 0.0;
-        if (!gbad[i])
-            for (int v = v0 + tid; v < v1; v += VF_T) {
-                const double x = (double)vf_ld(p.logits, p.dtype, base + v) - m;
-                a += exp(x * it); d += exp(x);
+            const float ref = fmaxf(m, -FLT_MAX);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float f[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {  // a NaN or +inf makes the sum a NaN
+                    const float d = f[e] - ref;
+                    st += vf_ex2(d * cT);
+                    if (!unit) s1 += vf_ex2(d * 1.4426950408889634f);
+                }
             }
-        a = vf_warp_sum(a); d = vf_warp_sum(d);
-        if (ln == 0) { wpart[0][w] = a; wpart[1][w] = d; }
-        __syncthreads();
-        if (tid == 0) {
-            a = d = 0.0;
-            for (int k = 0; k < VF_W; k++) { a += wpart[0][k]; d += wpart[1][k]; }
-            st[i] = a; s1[i] = d;
-        }
-        __syncthreads();
-    }
-    cl.sync();
-    for (int i = tid; i <= nd; i += VF_T) {
-        double a = 0.0, d = 0.0;
-        for (int k = 0; k < VF_C; k++) { a += *cl.map_shared_rank(&st[i], k); d += *cl.map_shared_rank(&s1[i], k); }
-        gst[i] = a; gs1[i] = d;
-    }
-    __syncthreads();
-    if (tid == 0) {                           // every CTA of the slot comes to the same end
-        int r = 0, kind = 0;
-        for (; r <= nd; r++) {
-            if (gbad[r]) { kind = 2; break; }
-            if (r == nd) break;
-            const int x = p.draft[(size_t)b * n + r];
-            if (x < 0 || x >= p.V) { kind = 3; break; }
-            if (greedy) { if (x != garg[r]) { kind = 1; break; } }
-            else {
-                const double e = exp(((double)vf_ld(p.logits, p.dtype, row0 + (size_t)r * p.ld + x) - (double)gm[r]) * it);
-                const double qx = p.q ? (double)p.q[((size_t)b * n + r) * p.ldq + x] : 1.0;
-                if (!((double)p.u[(size_t)b * (n + 1) + r] * qx * gst[r] < e)) { kind = 1; break; }
+            if (s % steps == steps - 1) {     // the end of a row's run
+                if (unit) s1 = st;
+                VfPart a;
+                a.m = m;
+                a.arg = arg;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) {
+                    const float om = __shfl_xor_sync(~0u, a.m, o); const int oa = __shfl_xor_sync(~0u, a.arg, o);
+                    if (om > a.m || (om == a.m && oa < a.arg)) { a.m = om; a.arg = oa; }
+                }
+                a.odd = __any_sync(~0u, st != st);
+                const float ref = fmaxf(m, -FLT_MAX), wref = fmaxf(a.m, -FLT_MAX);
+                a.st = vf_warp_sum((double)(st * vf_ex2((ref - wref) * cT)));
+                s1 *= vf_ex2((ref - wref) * 1.4426950408889634f);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) s1 += __shfl_xor_sync(~0u, s1, o);
+                a.s1 = s1;
+                if (ln == 0) warp_part[i0 + s / steps][w] = a;
+                m = -INFINITY; st = s1 = 0.0f; arg = 0x7fffffff;
             }
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = y[k];
         }
-        end_row = r; end_kind = kind;
-        if (c == 0 && kind == 2) report_bad_index(p.errword, 309, b, r);
-        if (c == 0 && kind == 3) report_bad_index(p.errword, 308, b, p.draft[(size_t)b * n + r]);
+        cl.sync();
+        for (int i = i0 + w; i < i1; i += VF_W) {         // a warp joins the runs of a row
+            VfPart a[RPL], t;
+#pragma unroll
+            for (int k = 0; k < RPL; k++) a[k] = *cl.map_shared_rank(&warp_part[i][(RPL * ln + k) % VF_W], (RPL * ln + k) / VF_W);
+            t = a[0];
+#pragma unroll
+            for (int k = 1; k < RPL; k++) {
+                if (a[k].m > t.m) { t.m = a[k].m; t.arg = a[k].arg; }
+                t.odd |= a[k].odd;
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const float om = __shfl_xor_sync(~0u, t.m, o); const int oa = __shfl_xor_sync(~0u, t.arg, o);
+                if (om > t.m || (om == t.m && oa < t.arg)) { t.m = om; t.arg = oa; }
+            }
+            t.odd = __any_sync(~0u, t.odd);
+            double zt = 0.0, z1 = 0.0;
+#pragma unroll
+            for (int k = 0; k < RPL; k++) {
+                zt += a[k].st * vf_scale(a[k].m, t.m, it);
+                z1 += (double)(a[k].s1 * vf_ex2((fmaxf(a[k].m, -FLT_MAX) - fmaxf(t.m, -FLT_MAX)) * 1.4426950408889634f));
+            }
+            t.st = vf_warp_sum(zt);
+            t.s1 = (float)vf_warp_sum(z1);
+            if (ln == 0) row_part[i] = t;
+        }
+        __syncthreads();
+        // every warp of the slot comes to the same end: a lane looks at every 32nd row
+        r = VF_ROWS; kind = -1;
+        for (int i = i0 + ln; i < i1 && kind < 0; i += 32) {
+            const VfPart &a = row_part[i];
+            int k = -1;
+            if (a.odd || a.m == -INFINITY) k = 2;
+            else if (i == nd) k = 0;
+            else if (sx[i] < 0 || sx[i] >= p.V) k = 3;
+            else if (greedy ? sx[i] != a.arg : !(suq[i] * a.st < exp2(((double)sl[i] - (double)a.m) * it))) k = 1;
+            if (k >= 0) { r = i; kind = k; }
+        }
+        const int first = __reduce_min_sync(~0u, r), who = __ffs(__ballot_sync(~0u, r == first)) - 1;
+        kind = __shfl_sync(~0u, kind, who);
+        r = first;
+        if (kind >= 0) break;
     }
-    __syncthreads();
-    const int r = end_row, kind = end_kind;
     if (c == 0) {                             // what was taken, and the places behind the end
         for (int i = tid; i <= n; i += VF_T) {
             if (i == r && kind < 2) continue;
-            int x = -1; float l = 0.0f;
-            if (i < r) {
-                x = p.draft[(size_t)b * n + i];
-                l = (float)((double)vf_ld(p.logits, p.dtype, row0 + (size_t)i * p.ld + x) - (double)gm[i] - log(gs1[i]));
-            }
-            out[i] = x; lp[i] = l;
+            out[i] = i < r ? sx[i] : -1;
+            lp[i] = i < r ? (float)((double)sl[i] - (double)row_part[i].m) - logf(row_part[i].s1) : 0.0f;
         }
-        if (tid == 0) p.count[b] = kind < 2 ? r + 1 : r;
+        if (tid == 0) {
+            p.count[b] = kind < 2 ? r + 1 : r;
+            if (kind == 2) report_bad_index(p.errword, 309, b, r);
+            if (kind == 3) report_bad_index(p.errword, 308, b, sx[r]);
+        }
     }
     if (kind >= 2) { cl.sync(); return; }     // nobody reads this CTA's shared memory any more
     const size_t base = row0 + (size_t)r * p.ld;
+    const VfPart row = row_part[r];
     int pick = -1;
     if (greedy) {
-        if (c == 0 && tid == 0) pick = garg[r];
+        if (c == 0 && tid == 0) pick = row.arg;
     } else {
-        const double m = gm[r], Z = gst[r];
-        const float *qr = kind == 1 && p.q ? p.q + ((size_t)b * n + r) * p.ldq : nullptr;
-        const int xr = kind == 1 && !p.q ? p.draft[(size_t)b * n + r] : -1;
-        const auto weight = [&](int v, bool rest) {          // Z times the token's: no quotient to round
-            double e = exp(((double)vf_ld(p.logits, p.dtype, base + v) - m) * it);
-            if (rest) { if (qr) e = fmax(e - (double)qr[v] * Z, 0.0); else if (v == xr) e = 0.0; }
+        const bool rest = kind == 1;
+        const float *qr = rest && p.q ? p.q + ((size_t)b * n + r) * p.ldq : nullptr;
+        const int xr = rest && !p.q ? sx[r] : -1;
+        const auto weight = [&](int v, bool rest) {
+            double e = vf_ex2((vf_ld<BF>(p.logits, base + v) - row.m) * cT);
+            if (rest) { if (qr) e = fmax(fma(-(double)qr[v], row.st, e), 0.0); else if (v == xr) e = 0.0; }
             return e;
         };
-        // a warp's part of the share is one run of tokens
-        const int sub = (v1 - v0 + VF_W - 1) / VF_W, w0 = min(v0 + w * sub, v1), w1 = min(w0 + sub, v1);
-        double a = 0.0, d = 0.0;
-        for (int v = w0 + ln; v < w1; v += 32) { a += weight(v, kind == 1); d += weight(v, false); }
-        a = vf_warp_sum(a); d = vf_warp_sum(d);
-        if (ln == 0) { wpart[0][w] = a; wpart[1][w] = d; }
-        __syncthreads();
-        if (tid == 0) {
-            a = d = 0.0;
-            for (int k = 0; k < VF_W; k++) { a += wpart[0][k]; d += wpart[1][k]; }
-            wsum[0] = a; wsum[1] = d;
+        double a = 0.0;
+        if (rest) {
+#pragma unroll 8
+            for (int v = w0 + ln; v < w1; v += 32) a += weight(v, true);
+            a = vf_warp_sum(a);
+            if (ln == 0) wleft[w] = a;
+            cl.sync();
         }
-        cl.sync();
-        double W[2] = {0.0, 0.0};
-        for (int k = 0; k < VF_C; k++) { W[0] += cl.map_shared_rank(wsum, k)[0]; W[1] += cl.map_shared_rank(wsum, k)[1]; }
-        const int s = W[0] > 0.0 ? 0 : 1;     // nothing is left of p - q: from p
-        const double target = (double)p.u[(size_t)b * (n + 1) + n] * W[s];
-        // the share, then the run, whose end passes the target; the last with a weight where rounding leaves none
-        double acc = 0.0, at = 0.0;
-        int cta = -1;
-        for (int k = 0; k < VF_C; k++) {
-            const double x = cl.map_shared_rank(wsum, k)[s];
-            if (x > 0.0) { cta = k; at = acc; if (acc + x > target) break; }
-            acc += x;
-        }
-        if (cta == c) {
-            int run = -1; double from = 0.0;
-            acc = at;
-            for (int k = 0; k < VF_W; k++) {
-                const double x = wpart[s][k];
-                if (x > 0.0) { run = k; from = acc; if (acc + x > target) break; }
-                acc += x;
-            }
-            if (run == w) {
-                int last = -1;
-                for (int v = w0; v < w1 && pick < 0; v += 32) {
-                    const double e = v + ln < w1 ? weight(v + ln, kind == 1 && s == 0) : 0.0;
-                    double cum = e;
+        // every warp of the slot finds the run whose end passes the target; the last with a weight where rounding leaves none
+        double xs[RPL], mysum = 0.0, all = 0.0;
+        if (rest) {
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(~0u, cum, o); if (ln >= o) cum += y; }
-                    const unsigned some = __ballot_sync(~0u, e > 0.0), past = __ballot_sync(~0u, e > 0.0 && from + cum > target);
-                    if (past) pick = v + __ffs(past) - 1;
-                    if (some) last = v + 31 - __clz(some);
-                    from += __shfl_sync(~0u, cum, 31);
+            for (int k = 0; k < RPL; k++) { xs[k] = *cl.map_shared_rank(&wleft[(RPL * ln + k) % VF_W], (RPL * ln + k) / VF_W); mysum += xs[k]; }
+            all = vf_warp_sum(mysum);
+        }
+        const bool left = all > 0.0;
+        if (!left) {                                      // a draw behind the drafts, or nothing is left: by e
+            mysum = 0.0;
+#pragma unroll
+            for (int k = 0; k < RPL; k++) {
+                const VfPart *o = cl.map_shared_rank(&warp_part[r][(RPL * ln + k) % VF_W], (RPL * ln + k) / VF_W);
+                const float om = o->m;
+                xs[k] = vf_ex2((om - row.m) * cT) > 0.0f ? o->st * vf_scale(om, row.m, it) : 0.0;   // a run whose every weight is 0 below
+                mysum += xs[k];
+            }
+            all = vf_warp_sum(mysum);
+        }
+        const double target = (double)p.u[(size_t)b * (n + 1) + n] * all;
+        double cum = mysum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(~0u, cum, o); if (ln >= o) cum += y; }
+        const unsigned has = __ballot_sync(~0u, mysum > 0.0), over = __ballot_sync(~0u, mysum > 0.0 && cum > target);
+        const int src = over ? __ffs(over) - 1 : 31 - __clz(has);
+        int mine = 0;
+        double from = 0.0, acc = cum - mysum;
+        bool found = false;
+#pragma unroll
+        for (int k = 0; k < RPL; k++) {
+            if (xs[k] > 0.0 && !found) { mine = RPL * ln + k; from = acc; found = acc + xs[k] > target; }
+            acc += xs[k];
+        }
+        mine = __shfl_sync(~0u, mine, src);
+        from = __shfl_sync(~0u, from, src);
+        if (mine / VF_W == c) {
+            // the CTA reads the run again: a lane has `each` neighbouring tokens
+            const int r0 = min(mine * run, p.V), r1 = min(r0 + run, p.V), each = (r1 - r0 + VF_T - 1) / VF_T;
+            const int l0 = min(r0 + tid * each, r1), l1 = min(l0 + each, r1);
+            mysum = 0.0;
+            int last = -1;
+#pragma unroll 4
+            for (int v = l0; v < l1; v++) { const double e = weight(v, left); mysum += e; if (e > 0.0) last = v; }
+            cum = mysum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(~0u, cum, o); if (ln >= o) cum += y; }
+            if (ln == 31) wtot[w] = cum;
+            __syncthreads();
+            int mw = -1;
+            acc = from;
+            for (int k = 0; k < VF_W; k++) {
+                const double t = wtot[k];
+                if (t > 0.0) { mw = k; from = acc; if (acc + t > target) break; }
+                acc += t;
+            }
+            if (mw == w) {
+                const unsigned some = __ballot_sync(~0u, last >= 0), past = __ballot_sync(~0u, last >= 0 && from + cum > target);
+                if (past ? ln == __ffs(past) - 1 : ln == 31 - __clz(some)) {
+                    from += cum - mysum;
+                    pick = last;
+                    for (int v = l0; v <= last; v++) {
+                        const double e = weight(v, left);
+                        from += e;
+                        if (e > 0.0 && from > target) { pick = v; break; }
+                    }
                 }
-                if (pick < 0) pick = last;
-                if (ln) pick = -1;
             }
         }
     }
     if (pick >= 0) {
         out[r] = pick;
-        lp[r] = (float)((double)vf_ld(p.logits, p.dtype, base + pick) - (double)gm[r] - log(gs1[r]));
+        lp[r] = (float)((double)vf_ld<BF>(p.logits, base + pick) - (double)row.m) - logf(row.s1);
     }
     cl.sync();
 }
@@ -249,8 +346,16 @@ extern "C" int qlmb_dec_verify(int *out, int *count, float *lp, const void *logi
     QLMB_REQUIRE(ld >= V && (!q || ldq >= V), "qlmb_dec_verify: rows of %lld and %lld elements, %d tokens", ld, ldq, V);
     if (B <= 0) return QLMB_OK;
     QLMB_REQUIRE(B < (1 << 24), "qlmb_dec_verify: %d slots", B);
-    VerifyParams p = {out, count, lp, logits, q, u, temp, draft, nd, lg_dtype, B, n, V, ld, ldq, device_error_word()};
-    k_dec_verify<<<(unsigned)B * VF_C, VF_T, 0, as_stream(stream)>>>(p);
+    // A round (a group of rows, the cluster's meeting, the test) costs about 3 us beside the reading, and rows behind the end are read for
+    // nothing.  Vocabularies of up to 32768: four warps a CTA, so that the 64 clusters of a full server run at once, and two rows a
+    // round (64 slots of 16384, five rows: 19.4 us; one row a round 21.5, eight warps 24.2, all five rows 20.2).  Above: eight warps
+    // and one row (32 slots of 130001, eight rows: 33.7 us; four warps 44.5, two rows 36.8, sixteen warps 34.0).
+    const bool wide = V > 32768, bf = lg_dtype == QLMB_BF16, vec = ld % 4 == 0 && ((uintptr_t)logits & (bf ? 7 : 15)) == 0;
+    VerifyParams p = {out, count, lp, logits, q, u, temp, draft, nd, B, n, V, wide ? 1 : 2, ld, ldq, device_error_word()};
+    void (*kern)(const VerifyParams);
+    if (wide) kern = bf ? (vec ? k_dec_verify<true, true, 8> : k_dec_verify<true, false, 8>) : (vec ? k_dec_verify<false, true, 8> : k_dec_verify<false, false, 8>);
+    else kern = bf ? (vec ? k_dec_verify<true, true, 4> : k_dec_verify<true, false, 4>) : (vec ? k_dec_verify<false, true, 4> : k_dec_verify<false, false, 4>);
+    QLMB_CUDA(pdl_launch_small(kern, dim3((unsigned)B * VF_C), dim3(wide ? 256 : 128), 0, as_stream(stream), p));
     QLMB_LAUNCH_CHECK("k_dec_verify");
     return QLMB_OK;
 }
