@@ -1,19 +1,22 @@
 // Low-rank adapters of many requests beside a projection that their rows share:
 //   Y[m] = base[m] + s_a (X[m] A_a^T) B_a,   a = adapter[m] (-1: Y[m] = base[m]),   A [n][R][K], B [n][R][N] bf16.
 //
-// Two launches: k_lora_down makes the R inner numbers of every row, in slices of K, k_lora_up adds the slices, multiplies by B and adds
-// the base.  Both take tiles of 16 rows and go through the adapters that occur in the tile; a row's products depend on no other
-// row, so a tile's 16 rows are multiplied by each adapter and only its own rows kept.  With the rows in the order of their
-// adapters (`order`) most tiles have one.
-// The inner numbers stay fp32: they enter the second product as two or three bf16 terms, so does X where it is fp32.
+// Products on mma.m16n8k16, operands from global memory as they lie there: of X and A a thread takes eight neighbouring elements of K
+// where the instruction wants pairs (the order of a contracted dimension is free as long as both operands agree), of B eight
+// neighbouring columns of each of its four inner indices, paired up by byte permutations.
+// A row's products depend on no other row: a tile's rows are multiplied by each adapter that occurs among them, and only the
+// adapter's own rows are kept.  With the rows in the order of their adapters (`order`) most tiles have one.
+// The R inner numbers of a row are sums in fp32; they enter the second product as two bf16 terms (bf16 rows) or three (fp32 rows), and
+// so does X where it is fp32: 16 and 24 bits.
+//
 #include <cuda_bf16.h>
 #include "qlmb_common.cuh"
 #include "qlmb_internal.h"
 
 namespace qlmb {
 
-constexpr int LR_RT = 64;                     // inner columns of a CTA of k_lora_down
-constexpr int LR_NT = 256;                    // output columns of a CTA of k_lora_up
+constexpr int LR_RT = 64;                     // inner columns made at a time
+constexpr int LR_UP = 512;                    // output columns of a CTA of k_lora_up
 
 struct LoraParams {
     void *Y;
@@ -52,185 +55,541 @@ __device__ __forceinline__ void lr_row(const LoraParams &p, int j, int &m, int &
     if (a < -1 || a >= p.adapters) { if (report) report_bad_index(p.errword, 307, m, a); a = -1; }
 }
 
-template <bool F32> __global__ void __launch_bounds__(128) k_lora_down(const __grid_constant__ LoraParams p)
+// c += X A^T for 16 rows (m0: row g, m1: row g + 8 of the thread, -1 for none) and NT tiles of 8 inner columns, over steps of 32 of K:
+// kb, kb + stride, ... below k1.  UK steps are loaded before the first is multiplied.
+template <bool F32, int NT, int UK>
+__device__ __forceinline__ void lr_down(const LoraParams &p, float (&c)[NT][4], const bf16 *A, int ncol, int m0, int m1, int kb, int k1, int stride)
 {
     constexpr int XT = F32 ? 3 : 1;
-    __shared__ float red[4][16][LR_RT + 2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    pdl_trigger();
-    pdl_wait();
-    const int j0 = blockIdx.x * 16, r0 = blockIdx.z * LR_RT, k0 = blockIdx.y * p.kslice, k1 = min(p.K, k0 + p.kslice);
-    int m, a;
-    lr_row(p, j0 + (lane & 15), m, a, false);
-    const int m0 = __shfl_sync(~0u, m, g), m1 = __shfl_sync(~0u, m, g + 8);
-    unsigned left = __ballot_sync(~0u, a >= 0) & 0xffffu;
-    while (left) {
-        const int cur = __shfl_sync(~0u, a, __ffs(left) - 1);
-        const unsigned mine = __ballot_sync(~0u, a == cur) & 0xffffu;
-        left &= ~mine;
-        float c[LR_RT / 8][4] = {};
-        const bf16 *A = p.A + ((size_t)cur * p.R + r0) * p.K;
-        for (int k = k0 + 32 * warp; k < k1; k += 128) {
-            const int kk = k + 8 * q;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    for (; kb < k1; kb += UK * stride) {
+        uint4 x[UK][2][F32 ? 2 : 1], b[UK][NT];
+#pragma unroll
+        for (int u = 0; u < UK; u++) {
+            const int kk = kb + u * stride + 8 * q;
             const bool in = kk < k1;
-            uint32_t x[XT][2][4];                        // [term][row half][pair]
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                b[u][t] = make_uint4(0, 0, 0, 0);
+                if (in && 8 * t < ncol) b[u][t] = *reinterpret_cast<const uint4 *>(A + (size_t)(8 * t + g) * p.K + kk);
+            }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const int mm = e ? m1 : m0;
-                const bool live = in && mm >= 0 && (mine >> (g + 8 * e) & 1);
-                if (F32) {
-                    float4 u = make_float4(0, 0, 0, 0), v = u;
-                    if (live) {
-                        const float4 *s = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.X) + (size_t)mm * p.K + kk);
-                        u = s[0]; v = s[1];
+#pragma unroll
+                for (int h = 0; h < (F32 ? 2 : 1); h++) {
+                    x[u][e][h] = make_uint4(0, 0, 0, 0);
+                    if (in && mm >= 0) {
+                        if (F32) x[u][e][h] = reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(p.X) + (size_t)mm * p.K + kk)[h];
+                        else x[u][e][h] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const bf16 *>(p.X) + (size_t)mm * p.K + kk);
                     }
-                    const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        uint32_t t[XT];
-                        lr_split<XT>(f[2 * w], f[2 * w + 1], t);
-#pragma unroll
-                        for (int i = 0; i < XT; i++) x[i][e][w] = t[i];
-                    }
-                } else {
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (live) u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const bf16 *>(p.X) + (size_t)mm * p.K + kk);
-                    x[0][e][0] = u.x; x[0][e][1] = u.y; x[0][e][2] = u.z; x[0][e][3] = u.w;
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < LR_RT / 8; t++) {
-                uint4 b = make_uint4(0, 0, 0, 0);
-                if (in && r0 + 8 * t < p.R) b = *reinterpret_cast<const uint4 *>(A + (size_t)(8 * t + g) * p.K + kk);
-#pragma unroll
-                for (int i = XT - 1; i >= 0; i--) {
-                    const uint32_t a0[4] = {x[i][0][0], x[i][1][0], x[i][0][1], x[i][1][1]}, a1[4] = {x[i][0][2], x[i][1][2], x[i][0][3], x[i][1][3]};
-                    lr_mma(c[t], a0, b.x, b.y);
-                    lr_mma(c[t], a1, b.z, b.w);
                 }
             }
         }
 #pragma unroll
-        for (int t = 0; t < LR_RT / 8; t++) {
+        for (int u = 0; u < UK; u++) {
+            uint32_t xs[XT][2][4];                       // [term][row half][pair]
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                if (F32) {
+                    const uint32_t f[8] = {x[u][e][0].x, x[u][e][0].y, x[u][e][0].z, x[u][e][0].w, x[u][e][F32].x, x[u][e][F32].y, x[u][e][F32].z, x[u][e][F32].w};
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        uint32_t t[XT];
+                        lr_split<XT>(__uint_as_float(f[2 * w]), __uint_as_float(f[2 * w + 1]), t);
+#pragma unroll
+                        for (int i = 0; i < XT; i++) xs[i][e][w] = t[i];
+                    }
+                } else { xs[0][e][0] = x[u][e][0].x; xs[0][e][1] = x[u][e][0].y; xs[0][e][2] = x[u][e][0].z; xs[0][e][3] = x[u][e][0].w; }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = XT - 1; i >= 0; i--) {
+                    const uint32_t a0[4] = {xs[i][0][0], xs[i][1][0], xs[i][0][1], xs[i][1][1]}, a1[4] = {xs[i][0][2], xs[i][1][2], xs[i][0][3], xs[i][1][3]};
+                    lr_mma(c[t], a0, b[u][t].x, b[u][t].y);
+                    lr_mma(c[t], a1, b[u][t].z, b[u][t].w);
+                }
+        }
+    }
+}
+
+// Columns n0 .. n0 + 63 of 16 rows: base + T B.  A thread asks for B's rows r0 + 2 q, + 1, + 8, + 9, columns n0 + 8 g .. n0 + 8 g + 7.
+__device__ __forceinline__ void lr_up_b(const LoraParams &p, int cur, int n0, int r0, uint4 (&b)[4])
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const int r = r0 + 2 * q + (w & 1) + 8 * (w >> 1), n = n0 + 8 * g;
+        b[w] = make_uint4(0, 0, 0, 0);
+        if (cur >= 0 && n < p.N && r < p.R) b[w] = *reinterpret_cast<const uint4 *>(p.Bm + ((size_t)cur * p.R + r) * p.N + n);
+    }
+}
+// T as bf16 terms in shared memory: [term][row][ldt] pairs, t0 = the pairs of row g
+template <bool F32> __device__ __forceinline__ void lr_up_mul(const LoraParams &p, float (&c)[8][4], const uint4 (&b)[4], const uint32_t *t0, int ldt, int r0)
+{
+    constexpr int TT = F32 ? 3 : 2;
+    const int q = threadIdx.x & 3;
+    uint32_t ta[TT][4];
+#pragma unroll
+    for (int i = 0; i < TT; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) ta[i][2 * h + e] = r0 + 8 * h < p.R ? t0[(i * 16 + 8 * e) * ldt + (r0 + 8 * h) / 2 + q] : 0u;
+    const uint32_t *b0 = &b[0].x, *b1 = &b[1].x, *b2 = &b[2].x, *b3 = &b[3].x;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+        const uint32_t x = __byte_perm(b0[j >> 1], b1[j >> 1], sel), y = __byte_perm(b2[j >> 1], b3[j >> 1], sel);
+#pragma unroll
+        for (int i = TT - 1; i >= 0; i--) lr_mma(c[j], ta[i], x, y);
+    }
+}
+// columns 16 q .. 16 q + 15 of the warp's 64 end up with a thread, for its two rows; `keep`: which of them are this adapter's
+template <bool F32> __device__ __forceinline__ void lr_up_base(const LoraParams &p, uint4 (&base)[2][2][F32 ? 2 : 1], int n0, const int (&mrow)[2], const bool (&keep)[2])
+{
+    const int q = threadIdx.x & 3;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int col = n0 + 16 * q + 8 * h;
+            if (keep[e] && col < p.N)
+#pragma unroll
+                for (int k = 0; k < (F32 ? 2 : 1); k++)
+                    base[e][h][k] = reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(p.base) + ((size_t)mrow[e] * p.N + col) * (F32 ? 4 : 2))[k];
+        }
+}
+template <bool F32> __device__ __forceinline__ void lr_up_store(const LoraParams &p, const float (&c)[8][4], const uint4 (&base)[2][2][F32 ? 2 : 1], int cur, int n0, const int (&mrow)[2], const bool (&keep)[2])
+{
+    const int q = threadIdx.x & 3;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        if (!keep[e] || (cur < 0 && p.Y == p.base)) continue;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int col = n0 + 16 * q + 8 * h;
+            if (col >= p.N) continue;
+            uint32_t w[8];
+            const uint32_t *s = &base[e][h][0].x, *s2 = &base[e][h][F32 ? 1 : 0].x;
+#pragma unroll
+            for (int k = 0; k < 4; k++) { w[k] = s[k]; w[4 + k] = s2[k]; }
+            if (cur >= 0) {
+                if (F32) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) w[k] = __float_as_uint(__uint_as_float(w[k]) + c[k][2 * e + h]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(w[k] << 16) + c[2 * k][2 * e + h], __uint_as_float(w[k] & 0xffff0000u) + c[2 * k + 1][2 * e + h]);
+                        w[k] = *reinterpret_cast<const uint32_t *>(&h2);
+                    }
+                }
+            }
+            uint4 *d = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.Y) + ((size_t)mrow[e] * p.N + col) * (F32 ? 4 : 2));
+            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (F32) d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+    }
+}
+template <bool F32>
+__device__ __forceinline__ void lr_up(const LoraParams &p, const uint32_t *t0, int ldt, int cur, int n0, const int (&mrow)[2], const bool (&keep)[2])
+{
+    uint4 base[2][2][F32 ? 2 : 1];
+    lr_up_base<F32>(p, base, n0, mrow, keep);
+    float c[8][4] = {};
+    if (cur >= 0) {
+#pragma unroll 2
+        for (int r0 = 0; r0 < p.R; r0 += 16) {
+            uint4 b[4];
+            lr_up_b(p, cur, n0, r0, b);
+            lr_up_mul<F32>(p, c, b, t0, ldt, r0);
+        }
+    }
+    lr_up_store<F32>(p, c, base, cur, n0, mrow, keep);
+}
+
+// ---- many rows.  A CTA of eight warps (four row groups of 16 times two halves of 32 columns) has 64 rows: the products' operands come
+// through a ring of four stages in shared memory, a stage being 64 x 64 elements of X (or of the base) and of A (or B), in 16-byte
+// pieces whose place is turned by the row.  First the inner numbers over K, 64 at a time, kept as bf16 terms; then Y, 64 columns at a
+// time: the base lies in the stage, the sum takes its place there and leaves in whole pieces.
+constexpr int LT_M = 64, LT_NS = 4, LT_W = 64 * 64 * 2;      // rows, stages, bytes of a stage's weights
+template <bool F32> constexpr int lt_x() { return LT_M * 64 * (F32 ? 4 : 2); }
+template <bool F32> static size_t lt_smem(int R) { return (size_t)LT_NS * (lt_x<F32>() + LT_W) + (size_t)(F32 ? 3 : 2) * LT_M * ((R + 15) / 16 * 8 + 4) * sizeof(uint32_t); }
+
+__device__ __forceinline__ uint32_t lt_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void lt_copy(uint32_t dst, const void *src, bool in)      // 16 bytes, zeros where !in
+{ asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); }
+__device__ __forceinline__ void lt_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void lt_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void lt_ldm(uint32_t a, uint32_t v[4])
+{ asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory"); }
+__device__ __forceinline__ void lt_ldmt(uint32_t a, uint32_t v[4])
+{ asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory"); }
+
+// SMALL (R <= 64): a warp keeps the terms of its 16 rows in registers while it goes through the columns.
+// blockIdx.z: a tile's adapters are dealt out to LT_Z CTAs, so that the tiles at the border of two prompts take no longer than the others.
+constexpr int LT_Z = 4;
+template <bool F32, bool SMALL> __global__ void __launch_bounds__(256, 2) k_lora_tile(const __grid_constant__ LoraParams p)
+{
+    constexpr int XT = F32 ? 3 : 1, TT = F32 ? 3 : 2, XB = lt_x<F32>(), STAGE = XB + LT_W, XP = F32 ? 16 : 8, EB = F32 ? 4 : 2;   // XP: pieces of a row of 64
+    extern __shared__ __align__(128) uint8_t lt_s[];
+    __shared__ int srow[LT_M];                            // the rows of the present adapter, -1 for the others
+    uint32_t *ts = reinterpret_cast<uint32_t *>(lt_s + LT_NS * STAGE);       // [term][row][ldt] pairs of bf16
+    const int ldt = (p.R + 15) / 16 * 8 + 4;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3, rg = (warp >> 1) * 16, nh = (warp & 1) * 32;
+    pdl_trigger();
+    pdl_wait();
+    const int j0 = blockIdx.x * LT_M;
+    int m[2], a[2];                                       // rows lane and lane + 32
+#pragma unroll
+    for (int e = 0; e < 2; e++) lr_row(p, j0 + lane + 32 * e, m[e], a[e], blockIdx.y == 0 && blockIdx.z == 0 && warp == 0);
+    const int per = (p.N + 64 * gridDim.y - 1) / (64 * gridDim.y) * 64, c0 = blockIdx.y * per, c1 = min(p.N, c0 + per);
+    if (c0 >= p.N) return;
+    unsigned todo[2] = {__ballot_sync(~0u, a[0] >= 0), __ballot_sync(~0u, a[1] >= 0)};
+    for (int nth = 0; todo[0] | todo[1]; nth++) {
+        const int cur = todo[0] ? __shfl_sync(~0u, a[0], __ffs(todo[0]) - 1) : __shfl_sync(~0u, a[1], __ffs(todo[1]) - 1);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            todo[e] &= ~__ballot_sync(~0u, a[e] == cur);
+            if (warp == 0 && nth % LT_Z == blockIdx.z) srow[lane + 32 * e] = a[e] == cur ? m[e] : -1;
+        }
+        if (nth % LT_Z != blockIdx.z) continue;
+        __syncthreads();
+        const float scale = p.scale[cur];
+        const bf16 *A = p.A + (size_t)cur * p.R * p.K, *Bm = p.Bm + (size_t)cur * p.R * p.N;
+        // A thread's pieces of a stage are the same in every step: rows xr + 256 / XP i of X (or the base), rows wr + 32 i of A (or B).
+        constexpr int NX = LT_M * XP / 256;
+        const int xr = tid / XP, xc = tid % XP, wr = tid >> 3, wc = tid & 7;
+        const uint32_t s0 = lt_addr(lt_s), xd = s0 + xr * (XP * 16) + ((xc ^ (xr & 7)) << 4), wd = s0 + XB + wr * 128 + ((wc ^ (wr & 7)) << 4);
+        int xrow[NX];
+#pragma unroll
+        for (int i = 0; i < NX; i++) xrow[i] = srow[xr + 256 / XP * i];
+        // ---- inner numbers: 64 of K at a time, block of 64 inner columns by block
+        int lrc = 0, lk = 0, ls = 0;                      // the next step to be requested, and its stage
+        const auto load1 = [&]() {
+            if (lrc < p.R) {
+                const int k = lk + xc * (16 / EB), kw = lk + wc * 8;
+                const uint32_t so = ls * STAGE;
+#pragma unroll
+                for (int i = 0; i < NX; i++) {
+                    const bool in = xrow[i] >= 0 && k < p.K;
+                    lt_copy(xd + so + i * (256 * 16), reinterpret_cast<const uint8_t *>(p.X) + (in ? ((size_t)xrow[i] * p.K + k) * EB : 0), in);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int r = lrc + wr + 32 * i;
+                    const bool in = r < p.R && kw < p.K;
+                    lt_copy(wd + so + i * (32 * 128), A + (in ? (size_t)r * p.K + kw : 0), in);
+                }
+                lk += 64;
+                if (lk >= p.K) { lk = 0; lrc += 64; }
+            }
+            ls = (ls + 1) % LT_NS;
+            lt_commit();
+        };
+        for (int st = 0; st < LT_NS - 1; st++) load1();
+        float c[4][4] = {};
+        for (int st = 0, rc = 0, k0 = 0; rc < p.R; st = (st + 1) % LT_NS) {
+            lt_wait<LT_NS - 2>();
+            __syncthreads();                              // the step has landed for everyone, and everyone is done with the one before
+            load1();
+            const uint8_t *sx = lt_s + st * STAGE, *sw = sx + XB;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                uint32_t x[XT][4], w[2][4];
+                if (F32) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int r = rg + g + 8 * e, k = 16 * s + 8 * h + 2 * q;
+                            const float2 f = *reinterpret_cast<const float2 *>(sx + r * 256 + (((k >> 2) ^ (r & 7)) << 4) + (k & 3) * 4);
+                            uint32_t t[XT];
+                            lr_split<XT>(f.x, f.y, t);
+#pragma unroll
+                            for (int i = 0; i < XT; i++) x[i][2 * h + e] = t[i];
+                        }
+                } else {
+                    const int r = rg + (lane & 15), cc = 2 * s + (lane >> 4);
+                    lt_ldm(lt_addr(sx + r * 128 + ((cc ^ (r & 7)) << 4)), x[0]);
+                }
+#pragma unroll
+                for (int t = 0; t < 2; t++) {             // two tiles of 8 inner columns: rows of A, their 16 elements of K in two pieces
+                    const int r = nh + 16 * t + (lane & 7) + 8 * (lane >> 4), cc = 2 * s + ((lane >> 3) & 1);
+                    lt_ldm(lt_addr(sw + r * 128 + ((cc ^ (r & 7)) << 4)), w[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = XT - 1; i >= 0; i--) lr_mma(c[t], x[i], w[t >> 1][2 * (t & 1)], w[t >> 1][2 * (t & 1) + 1]);
+            }
+            k0 += 64;
+            if (k0 >= p.K) {                              // the block's sums are whole
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int col = rc + nh + 8 * t;
+                    if (col < p.R)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            uint32_t v[TT];
+                            lr_split<TT>(c[t][2 * e] * scale, c[t][2 * e + 1] * scale, v);
+#pragma unroll
+                            for (int i = 0; i < TT; i++) ts[(i * LT_M + rg + g + 8 * e) * ldt + col / 2 + q] = v[i];
+                        }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) c[t][k] = 0.0f;
+                }
+                k0 = 0; rc += 64;
+            }
+        }
+        lt_wait<0>();
+        __syncthreads();
+        // ---- Y: 64 inner indices at a time, block of 64 columns by block; the base comes with a block's last step
+        int ln = c0;
+        lrc = 0; ls = 0;
+        const auto load2 = [&]() {
+            if (ln < c1) {
+                const int n = ln + xc * (16 / EB), nw = ln + wc * 8;
+                const uint32_t so = ls * STAGE;
+                if (lrc + 64 >= p.R && n < c1)
+#pragma unroll
+                    for (int i = 0; i < NX; i++)
+                        if (xrow[i] >= 0) lt_copy(xd + so + i * (256 * 16), reinterpret_cast<const uint8_t *>(p.base) + ((size_t)xrow[i] * p.N + n) * EB, true);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int r = lrc + wr + 32 * i;
+                    const bool in = r < p.R && nw < c1;
+                    lt_copy(wd + so + i * (32 * 128), Bm + (in ? (size_t)r * p.N + nw : 0), in);
+                }
+                lrc += 64;
+                if (lrc >= p.R) { lrc = 0; ln += 64; }
+            }
+            ls = (ls + 1) % LT_NS;
+            lt_commit();
+        };
+        for (int st = 0; st < LT_NS - 1; st++) load2();
+        const auto terms = [&](int r0, uint32_t (&x)[TT][4]) {            // 16 inner numbers of rows g and g + 8 as an A operand
+#pragma unroll
+            for (int i = 0; i < TT; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) x[i][2 * h + e] = r0 + 8 * h < p.R ? ts[(i * LT_M + rg + g + 8 * e) * ldt + (r0 + 8 * h) / 2 + q] : 0u;
+        };
+        uint32_t held[SMALL ? 4 : 1][TT][4];
+        if (SMALL)
+#pragma unroll
+            for (int s = 0; s < 4; s++) terms(16 * s, held[SMALL ? s : 0]);
+        for (int st = 0, rc = 0, n0 = c0; n0 < c1; st = (st + 1) % LT_NS) {
+            lt_wait<LT_NS - 2>();
+            __syncthreads();
+            load2();
+            uint8_t *sx = lt_s + st * STAGE;
+            const uint8_t *sw = sx + XB;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                if (rc + 16 * s >= p.R) break;
+                uint32_t w[2][4];
+                if (!SMALL) terms(rc + 16 * s, held[0]);
+                const uint32_t (&x)[TT][4] = held[SMALL ? s : 0];
+#pragma unroll
+                for (int t = 0; t < 2; t++) {             // two tiles of 8 columns: 16 rows of B
+                    const int r = 16 * s + (lane & 15), cc = (nh >> 3) + 2 * t + (lane >> 4);
+                    lt_ldmt(lt_addr(sw + r * 128 + ((cc ^ (r & 7)) << 4)), w[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = TT - 1; i >= 0; i--) lr_mma(c[t], x[i], w[t >> 1][2 * (t & 1)], w[t >> 1][2 * (t & 1) + 1]);
+            }
+            rc += 64;
+            if (rc >= p.R) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int r = rg + g + 8 * e, col = nh + 8 * t + 2 * q;
+                        uint8_t *d = sx + r * (XP * 16) + (((col * EB >> 4) ^ (r & 7)) << 4) + (col * EB & 15);
+                        if (F32) {
+                            float2 *f = reinterpret_cast<float2 *>(d);
+                            *f = make_float2(f->x + c[t][2 * e], f->y + c[t][2 * e + 1]);
+                        } else {
+                            const uint32_t v = *reinterpret_cast<const uint32_t *>(d);
+                            const __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(v << 16) + c[t][2 * e], __uint_as_float(v & 0xffff0000u) + c[t][2 * e + 1]);
+                            *reinterpret_cast<uint32_t *>(d) = *reinterpret_cast<const uint32_t *>(&h2);
+                        }
+                        c[t][2 * e] = c[t][2 * e + 1] = 0.0f;
+                    }
+                __syncwarp();                             // the warp's own 16 x 32 numbers
+#pragma unroll
+                for (int i = lane; i < 16 * XP / 2; i += 32) {
+                    const int r = rg + i / (XP / 2), cc = nh * EB / 16 + i % (XP / 2), row = srow[r], n = n0 + cc * (16 / EB);
+                    if (row >= 0 && n < c1)
+                        *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p.Y) + ((size_t)row * p.N + n) * EB) = *reinterpret_cast<const uint4 *>(sx + r * (XP * 16) + ((cc ^ (r & 7)) << 4));
+                }
+                rc = 0; n0 += 64;
+            }
+        }
+        lt_wait<0>();
+        __syncthreads();
+    }
+    // rows without an adapter
+    if (p.Y != p.base && blockIdx.z == 0)
+        for (int r = warp; r < LT_M; r += 8) {
+            const int row = __shfl_sync(~0u, r < 32 ? m[0] : m[1], r & 31), ad = __shfl_sync(~0u, r < 32 ? a[0] : a[1], r & 31);
+            if (row < 0 || ad >= 0) continue;
+            for (int n = c0 + lane * (16 / EB); n < c1; n += 32 * (16 / EB))
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p.Y) + ((size_t)row * p.N + n) * EB) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p.base) + ((size_t)row * p.N + n) * EB);
+        }
+}
+
+// ---- few rows, small adapters: one launch.  blockIdx.x = 16 tile + place: the CTA of a place that is the first of its adapter in the
+// tile does that adapter's rows, every block of columns making the inner numbers for itself.  Eight warps share K, then the columns.
+template <bool F32, int NT, int UK> __global__ void __launch_bounds__(256) k_lora_one(const __grid_constant__ LoraParams p)
+{
+    constexpr int TT = F32 ? 3 : 2;
+    __shared__ float red[8][16][8 * NT + 2];
+    __shared__ uint32_t ts[TT * 16 * (4 * NT + 4)];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, ldt = (p.R + 15) / 16 * 8 + 4;
+    pdl_trigger();
+    pdl_wait();
+    const int j0 = (int)blockIdx.x / 16 * 16, place = blockIdx.x % 16;
+    int m, a;
+    lr_row(p, j0 + (lane & 15), m, a, blockIdx.y == 0 && place == 0 && threadIdx.x < 16);
+    const int cur = __shfl_sync(~0u, a, place);
+    const unsigned mine = __ballot_sync(~0u, m >= 0 && a == cur) & 0xffffu;
+    if (__ffs(mine) - 1 != place) return;
+    const int rows[2] = {__shfl_sync(~0u, m, g), __shfl_sync(~0u, m, g + 8)};
+    const bool keep[2] = {(mine >> g & 1) != 0, (mine >> (g + 8) & 1) != 0};
+    if (cur >= 0) {
+        float c[NT][4] = {};
+        lr_down<F32, NT, UK>(p, c, p.A + (size_t)cur * p.R * p.K, p.R, keep[0] ? rows[0] : -1, keep[1] ? rows[1] : -1, 32 * warp, p.K, 256);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
             *reinterpret_cast<float2 *>(&red[warp][g][8 * t + 2 * q]) = make_float2(c[t][0], c[t][1]);
             *reinterpret_cast<float2 *>(&red[warp][g + 8][8 * t + 2 * q]) = make_float2(c[t][2], c[t][3]);
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * LR_RT; i += 128) {
-            const int r = i / LR_RT, col = i % LR_RT;
-            if ((mine >> r & 1) && r0 + col < p.R)
-                p.part[((size_t)blockIdx.y * p.M + j0 + r) * p.R + r0 + col] = (red[0][r][col] + red[1][r][col]) + (red[2][r][col] + red[3][r][col]);
+        const float scale = p.scale[cur];
+        for (int i = threadIdx.x; i < 16 * p.R / 2; i += 256) {
+            const int r = i / (p.R / 2), col = 2 * (i % (p.R / 2));
+            float x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) { const float2 v = *reinterpret_cast<const float2 *>(&red[k][r][col]); x += v.x; y += v.y; }
+            uint32_t t[TT];
+            lr_split<TT>(x * scale, y * scale, t);
+#pragma unroll
+            for (int k = 0; k < TT; k++) ts[(k * 16 + r) * ldt + col / 2] = t[k];
         }
         __syncthreads();
     }
+    const int n1 = min(p.N, ((int)blockIdx.y + 1) * LR_UP);
+    for (int n0 = blockIdx.y * LR_UP + 64 * warp; n0 < n1; n0 += 512) lr_up<F32>(p, ts + g * ldt, ldt, cur, n0, rows, keep);
 }
 
-template <bool F32> __global__ void __launch_bounds__(128) k_lora_up(const __grid_constant__ LoraParams p)
+// ---- few rows, large adapters: two launches, CTAs of places again; first the inner numbers in slices of K, then blocks of columns.
+template <bool F32, int NT, int UK> __global__ void __launch_bounds__(128) k_lora_down(const __grid_constant__ LoraParams p)
 {
-    constexpr int TT = F32 ? 3 : 2;
-    extern __shared__ float lr_t[];                      // [16][R + 4]
+    __shared__ float red[4][16][8 * NT + 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     pdl_trigger();
     pdl_wait();
-    const int j0 = blockIdx.x * 16, n0 = blockIdx.y * LR_NT + warp * 64, ldt = p.R + 4;
+    const int j0 = (int)blockIdx.x / 16 * 16, place = blockIdx.x % 16, r0 = blockIdx.z * (8 * NT), k0 = blockIdx.y * p.kslice, k1 = min(p.K, k0 + p.kslice);
     int m, a;
-    lr_row(p, j0 + (lane & 15), m, a, blockIdx.y == 0 && threadIdx.x < 16);
-    const int mrow[2] = {__shfl_sync(~0u, m, g), __shfl_sync(~0u, m, g + 8)};
-    for (int i = threadIdx.x; i < 16 * p.R; i += 128) {
-        const int r = i / p.R, col = i % p.R;
-        int mm, aa;
-        lr_row(p, j0 + r, mm, aa, false);
-        float t = 0.0f;
-        if (aa >= 0) {
-            for (int s = 0; s < p.S; s++) t += p.part[((size_t)s * p.M + j0 + r) * p.R + col];
-            t *= p.scale[aa];
-        }
-        lr_t[r * ldt + col] = t;
+    lr_row(p, j0 + (lane & 15), m, a, false);
+    const int cur = __shfl_sync(~0u, a, place);
+    const unsigned mine = __ballot_sync(~0u, a == cur) & 0xffffu;
+    if (cur < 0 || __ffs(mine) - 1 != place) return;
+    const int ra = __shfl_sync(~0u, m, g), rb = __shfl_sync(~0u, m, g + 8);
+    float c[NT][4] = {};
+    lr_down<F32, NT, UK>(p, c, p.A + ((size_t)cur * p.R + r0) * p.K, p.R - r0, mine >> g & 1 ? ra : -1, mine >> (g + 8) & 1 ? rb : -1, k0 + 32 * warp, k1, 128);
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        *reinterpret_cast<float2 *>(&red[warp][g][8 * t + 2 * q]) = make_float2(c[t][0], c[t][1]);
+        *reinterpret_cast<float2 *>(&red[warp][g + 8][8 * t + 2 * q]) = make_float2(c[t][2], c[t][3]);
     }
     __syncthreads();
-    unsigned left = __ballot_sync(~0u, m >= 0) & 0xffffu;
-    while (left) {
-        const int cur = __shfl_sync(~0u, a, __ffs(left) - 1);
-        const unsigned mine = __ballot_sync(~0u, m >= 0 && a == cur) & 0xffffu;
-        left &= ~mine;
-        float c[8][4] = {};
-        if (cur >= 0) {
-            const bf16 *Bm = p.Bm + (size_t)cur * p.R * p.N + n0 + 8 * g;
-            const bool in = n0 + 8 * g < p.N;
-            for (int r0 = 0; r0 < p.R; r0 += 16) {
-                uint32_t ta[TT][4];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float2 v = make_float2(0.0f, 0.0f);
-                        if (r0 + 8 * h < p.R) v = *reinterpret_cast<const float2 *>(lr_t + (g + 8 * e) * ldt + r0 + 8 * h + 2 * q);
-                        uint32_t t[TT];
-                        lr_split<TT>(v.x, v.y, t);
-#pragma unroll
-                        for (int i = 0; i < TT; i++) ta[i][2 * h + e] = t[i];
-                    }
-                uint4 b[4];
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const int r = r0 + 2 * q + (w & 1) + 8 * (w >> 1);
-                    b[w] = make_uint4(0, 0, 0, 0);
-                    if (in && r < p.R) b[w] = *reinterpret_cast<const uint4 *>(Bm + (size_t)r * p.N);
-                }
-                const uint32_t *b0 = &b[0].x, *b1 = &b[1].x, *b2 = &b[2].x, *b3 = &b[3].x;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-                    const uint32_t x = __byte_perm(b0[j >> 1], b1[j >> 1], sel), y = __byte_perm(b2[j >> 1], b3[j >> 1], sel);
-#pragma unroll
-                    for (int i = TT - 1; i >= 0; i--) lr_mma(c[j], ta[i], x, y);
-                }
-            }
-        }
-        // columns 16 q .. 16 q + 15 of the warp's 64, rows g and g + 8
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            if (!(mine >> (g + 8 * e) & 1) || (cur < 0 && p.Y == p.base)) continue;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int col = n0 + 16 * q + 8 * h;
-                if (col >= p.N) continue;
-                const size_t at = (size_t)mrow[e] * p.N + col;
-                float f[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) f[j] = c[j][2 * e + h];
-                if (F32) {
-                    const float4 *s = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.base) + at);
-                    float4 *d = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.Y) + at);
-                    const float4 u = s[0], v = s[1];
-                    d[0] = cur < 0 ? u : make_float4(u.x + f[0], u.y + f[1], u.z + f[2], u.w + f[3]);
-                    d[1] = cur < 0 ? v : make_float4(v.x + f[4], v.y + f[5], v.z + f[6], v.w + f[7]);
-                } else {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const bf16 *>(p.base) + at);
-                    uint32_t w[4] = {u.x, u.y, u.z, u.w};
-                    if (cur >= 0)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(w[k] << 16) + f[2 * k], __uint_as_float(w[k] & 0xffff0000u) + f[2 * k + 1]);
-                            w[k] = *reinterpret_cast<const uint32_t *>(&h2);
-                        }
-                    *reinterpret_cast<uint4 *>(reinterpret_cast<bf16 *>(p.Y) + at) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-        }
+    for (int i = threadIdx.x; i < 16 * 8 * NT; i += 128) {
+        const int r = i / (8 * NT), col = i % (8 * NT);
+        if ((mine >> r & 1) && r0 + col < p.R)
+            p.part[((size_t)blockIdx.y * p.M + j0 + r) * p.R + r0 + col] = (red[0][r][col] + red[1][r][col]) + (red[2][r][col] + red[3][r][col]);
     }
 }
-
-// Slices of K: enough CTAs for the device, each warp at least one step of 32.
-static void lora_plan(int M, int K, int R, int *S, int *kslice)
+// AHEAD (R <= 16): a warp's four blocks of 64 columns of B are requested before anything is multiplied.
+template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, AHEAD ? 4 : 3) k_lora_up(const __grid_constant__ LoraParams p)
 {
-    const long long tiles = ((long long)M + 15) / 16 * ((R + LR_RT - 1) / LR_RT);
-    long long s = (2LL * sm_count() + tiles - 1) / tiles;
-    const long long most = (K + 127) / 128;
+    constexpr int TT = F32 ? 3 : 2, UP = AHEAD ? 1024 : LR_UP;
+    extern __shared__ __align__(16) uint32_t lr_t[];     // [term][16][ldt] pairs of bf16
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, ldt = (p.R + 15) / 16 * 8 + 4;
+    pdl_trigger();
+    pdl_wait();
+    const int j0 = (int)blockIdx.x / 16 * 16, place = blockIdx.x % 16;
+    int m, a;
+    lr_row(p, j0 + (lane & 15), m, a, blockIdx.y == 0 && place == 0 && threadIdx.x < 16);
+    const int cur = __shfl_sync(~0u, a, place);
+    const unsigned mine = __ballot_sync(~0u, m >= 0 && a == cur) & 0xffffu;
+    if (__ffs(mine) - 1 != place) return;
+    const int rows[2] = {__shfl_sync(~0u, m, g), __shfl_sync(~0u, m, g + 8)};
+    const bool keep[2] = {(mine >> g & 1) != 0, (mine >> (g + 8) & 1) != 0};
+    uint4 b[AHEAD ? 4 : 1][4];
+    if (AHEAD)
+#pragma unroll
+        for (int i = 0; i < 4; i++) lr_up_b(p, cur, blockIdx.y * UP + 256 * i + 64 * warp, 0, b[AHEAD ? i : 0]);
+    if (cur >= 0) {
+        const float scale = p.scale[cur];
+        for (int i = threadIdx.x; i < 16 * p.R / 2; i += 128) {
+            const int r = i / (p.R / 2), col = 2 * (i % (p.R / 2));
+            if (!(mine >> r & 1)) continue;
+            float x = 0.0f, y = 0.0f;
+            const float *src = p.part + (size_t)(j0 + r) * p.R + col;
+#pragma unroll 8
+            for (int s = 0; s < p.S; s++) { const float2 v = *reinterpret_cast<const float2 *>(src + (size_t)s * p.M * p.R); x += v.x; y += v.y; }
+            uint32_t t[TT];
+            lr_split<TT>(x * scale, y * scale, t);
+#pragma unroll
+            for (int k = 0; k < TT; k++) lr_t[(k * 16 + r) * ldt + col / 2] = t[k];
+        }
+        __syncthreads();
+    }
+    if (AHEAD) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int n0 = blockIdx.y * UP + 256 * i + 64 * warp;
+            if (n0 >= p.N) break;
+            uint4 base[2][2][F32 ? 2 : 1];
+            lr_up_base<F32>(p, base, n0, rows, keep);
+            float c[8][4] = {};
+            if (cur >= 0) lr_up_mul<F32>(p, c, b[AHEAD ? i : 0], lr_t + g * ldt, ldt, 0);
+            lr_up_store<F32>(p, c, base, cur, n0, rows, keep);
+        }
+        return;
+    }
+    const int n1 = min(p.N, ((int)blockIdx.y + 1) * UP);
+    for (int n0 = blockIdx.y * UP + 64 * warp; n0 < n1; n0 += 256) lr_up<F32>(p, lr_t + g * ldt, ldt, cur, n0, rows, keep);
+}
+
+// Which form, and the slices of K of LORA_TWO.  Us, on both sides of each border (bf16, M rows on so many adapters):
+//   TILE above 2048 rows      K 768, N 1536, R 64: 2048 / 8 rows 19.6 as tiles, 26.9 as places; 8192 / 9 32.7 and 81.6
+//                             K 768, N 768, R 16: 2048 / 8 14.7 and 12.3, 8192 / 9 22.2 and 30.0; K 4096, N 4096, R 32: 1024 / 64
+//                             (runs of 16) 135 and 58, 8192 / 9 84 and 174
+//   ONE up to 256 rows and K R of 32768, where making the inner numbers once per 512 columns costs less than a launch
+//                             K 768, N 768, R 16: 64 rows 3.7 instead of 6.9, 256 / 2 4.7 and 7.0, 512 / 64 10.5 and 9.7
+//                             K 768, N 1536, R 64 (K R 49152): 64 rows 14.2 and 13.3
+enum LoraForm { LORA_ONE, LORA_TWO, LORA_TILE };
+static LoraForm lora_form(int M, int K, int R, int *S, int *kslice)
+{
+    *kslice = K; *S = 0;
+    if (M > 2048) return LORA_TILE;
+    if (M <= 256 && R <= 64 && (long long)K * R <= 32768) return LORA_ONE;
+    long long s = (4LL * sm_count() + M - 1) / M;
+    const long long most = (K + 511) / 512;              // four warps with four steps of 32 each
     if (s > most) s = most;
     if (s < 1) s = 1;
-    *kslice = (int)(((K + s - 1) / s + 31) / 32 * 32);
+    *kslice = (int)(((K + s - 1) / s + 127) / 128 * 128);
     *S = (K + *kslice - 1) / *kslice;
+    return LORA_TWO;
 }
 
 }  // namespace qlmb
@@ -244,27 +603,55 @@ extern "C" size_t qlmb_lora_bytes(int M, int K, int N, int R)
 {
     if (!lora_shape_ok(M, K, N, R)) return 0;
     int S, ks;
-    lora_plan(M, K, R, &S, &ks);
-    return (size_t)S * M * R * sizeof(float);
+    return lora_form(M, K, R, &S, &ks) == LORA_TWO ? (size_t)S * M * R * sizeof(float) : 16;
+}
+template <bool F32> static int lora_launch(const LoraParams &p, LoraForm form, cudaStream_t st)
+{
+    if (form == LORA_TILE) {
+        static bool configured_dev[64];                  // the attribute belongs to a device's copy of the kernel
+        int dev = 0;
+        QLMB_CUDA(cudaGetDevice(&dev));
+        QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
+        if (!configured_dev[dev]) {
+            QLMB_CUDA(cudaFuncSetAttribute(k_lora_tile<F32, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lt_smem<F32>(64)));
+            QLMB_CUDA(cudaFuncSetAttribute(k_lora_tile<F32, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lt_smem<F32>(256)));
+            configured_dev[dev] = true;
+        }
+        const int tiles = (p.M + LT_M - 1) / LT_M, most = (p.N + 63) / 64;
+        const int want = (3 * sm_count() / 2 + tiles / 2) / tiles;        // one to two CTAs an SM: each makes the inner numbers for itself
+        const dim3 grid((unsigned)tiles, (unsigned)(want < 1 ? 1 : want > most ? most : want), LT_Z);
+        QLMB_CUDA(pdl_launch_small(p.R <= 64 ? k_lora_tile<F32, true> : k_lora_tile<F32, false>, grid, dim3(256), lt_smem<F32>(p.R), st, p));
+        QLMB_LAUNCH_CHECK("k_lora_tile");
+        return QLMB_OK;
+    }
+    if (form == LORA_ONE) {
+        const dim3 grid((unsigned)((p.M + 15) / 16 * 16), (unsigned)((p.N + LR_UP - 1) / LR_UP));
+        QLMB_REQUIRE(grid.y < 65536, "qlmb_lora_add: N %d", p.N);
+        QLMB_CUDA(pdl_launch_small(p.R <= 16 ? k_lora_one<F32, 2, 4> : k_lora_one<F32, 8, 1>, grid, dim3(256), 0, st, p));
+        QLMB_LAUNCH_CHECK("k_lora_one");
+        return QLMB_OK;
+    }
+    const bool narrow = p.R <= 16;
+    const unsigned units = (unsigned)((p.M + 15) / 16 * 16);
+    const dim3 gd(units, (unsigned)p.S, (unsigned)(narrow ? 1 : (p.R + LR_RT - 1) / LR_RT)), gu(units, (unsigned)(narrow ? (p.N + 1023) / 1024 : (p.N + LR_UP - 1) / LR_UP));
+    QLMB_REQUIRE(gd.y < 65536 && gu.y < 65536, "qlmb_lora_add: K %d, N %d", p.K, p.N);
+    QLMB_CUDA(pdl_launch_small(narrow ? k_lora_down<F32, 2, 4> : k_lora_down<F32, LR_RT / 8, 1>, gd, dim3(128), 0, st, p));
+    QLMB_LAUNCH_CHECK("k_lora_down");
+    QLMB_CUDA(pdl_launch_small(narrow ? k_lora_up<F32, true> : k_lora_up<F32, false>, gu, dim3(128), (size_t)(F32 ? 3 : 2) * 16 * ((p.R + 15) / 16 * 8 + 4) * sizeof(uint32_t), st, p));
+    QLMB_LAUNCH_CHECK("k_lora_up");
+    return QLMB_OK;
 }
 extern "C" int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype, const void *A, const void *Bm, const float *scale, int adapters,
                              const int *adapter, const int *order, int M, int K, int N, int R, void *ws, size_t ws_bytes, void *stream)
 {
-    QLMB_REQUIRE(Y && X && base && A && Bm && scale && adapter && ws, "qlmb_lora_add: NULL argument");
+    QLMB_REQUIRE(Y && X && base && A && Bm && scale && adapter, "qlmb_lora_add: NULL argument");
     QLMB_REQUIRE(dtype == QLMB_F32 || dtype == QLMB_BF16, "qlmb_lora_add: rows of type %d", dtype);
     if (M <= 0) return QLMB_OK;
     QLMB_REQUIRE(lora_shape_ok(M, K, N, R) && adapters > 0, "qlmb_lora_add: M %d, K %d and N %d (multiples of 8), rank %d (a multiple of 8 up to 256), %d adapters", M, K, N, R, adapters);
     QLMB_REQUIRE((((uintptr_t)Y | (uintptr_t)X | (uintptr_t)base | (uintptr_t)A | (uintptr_t)Bm | (uintptr_t)ws) & 15) == 0, "qlmb_lora_add: rows, adapters and workspace must be 16-byte aligned");
     const size_t need = qlmb_lora_bytes(M, K, N, R);
-    QLMB_REQUIRE(ws_bytes >= need, "qlmb_lora_add: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
+    QLMB_REQUIRE(need <= 16 || (ws && ws_bytes >= need), "qlmb_lora_add: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
     LoraParams p = {Y, X, base, (const bf16 *)A, (const bf16 *)Bm, scale, adapter, order, (float *)ws, M, K, N, R, adapters, 0, 0, device_error_word()};
-    lora_plan(M, K, R, &p.S, &p.kslice);
-    cudaStream_t st = as_stream(stream);
-    const dim3 gd((unsigned)((M + 15) / 16), (unsigned)p.S, (unsigned)((R + LR_RT - 1) / LR_RT)), gu((unsigned)((M + 15) / 16), (unsigned)((N + LR_NT - 1) / LR_NT));
-    QLMB_REQUIRE(gd.y < 65536 && gu.y < 65536, "qlmb_lora_add: K %d, N %d", K, N);
-    QLMB_CUDA(pdl_launch_small(dtype == QLMB_F32 ? k_lora_down<true> : k_lora_down<false>, gd, dim3(128), 0, st, p));
-    QLMB_LAUNCH_CHECK("k_lora_down");
-    QLMB_CUDA(pdl_launch_small(dtype == QLMB_F32 ? k_lora_up<true> : k_lora_up<false>, gu, dim3(128), (size_t)16 * (R + 4) * sizeof(float), st, p));
-    QLMB_LAUNCH_CHECK("k_lora_up");
-    return QLMB_OK;
+    const LoraForm form = lora_form(M, K, R, &p.S, &p.kslice);
+    return dtype == QLMB_F32 ? lora_launch<true>(p, form, as_stream(stream)) : lora_launch<false>(p, form, as_stream(stream));
 }

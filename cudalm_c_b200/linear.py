@@ -98,7 +98,7 @@ def _lora_add_args(X, base, A, Bm, scale, adapter, order, out):
 
 def lora_add(X, base, A, Bm, scale, adapter, order=None, out=None):
     """base + scale[a] * (X A[a]^T) Bm[a] row by row, a = adapter[m] (-1: base): X [M, K], base [M, N] (fp32 or bf16), A [n, R, K] and Bm
-    [n, R, N] bf16, scale [n] fp32, adapter [M] int32.  out may be base."""
+    [n, R, N] bf16, scale [n] fp32, adapter [M] int32.  out may be base (not X)."""
     dev = device_index()
     try:
         dt = X.dtype
@@ -120,6 +120,6 @@ def lora_add(X, base, A, Bm, scale, adapter, order=None, out=None):
     nbytes = _lora_ws.get((dev, shape))
     if nbytes is None:
         nbytes = _lora_ws[(dev, shape)] = lib().qlmb_lora_bytes(*shape)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=X.device) if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=X.device) if nbytes > 16 else None
     calls.lora_add(out, X, base, F32 if dt is torch.float32 else BF16, A, Bm, scale, n, adapter, order, M, K, N, R, ws, nbytes, stream_ptr())
     return out

@@ -45,7 +45,7 @@ def test_refusals_of_the_entry_points():
         (lambda: attn(nbytes=ctypes.c_size_t(16)), b"workspace of 16 bytes"),
         (lambda: verify(out=None), b"NULL"), (lambda: verify(draft=None), b"NULL"), (lambda: verify(dt=2), b"type"), (lambda: verify(n=-1), b"n -1"),
         (lambda: verify(n=64), b"n 64"), (lambda: verify(V=0), b"V 0"), (lambda: verify(ld=15), b"rows of 15"), (lambda: verify(ldq=15), b"and 15"),
-        (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None), b"NULL"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
+        (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None), b"workspace"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
         (lambda: lora(K=60), b"multiples of 8"), (lambda: lora(N=63), b"multiples of 8"), (lambda: lora(R=12), b"rank 12"), (lambda: lora(R=264), b"rank 264"),
         (lambda: lora(R=0), b"rank 0"), (lambda: lora(X=odd), b"aligned"), (lambda: lora(nbytes=ctypes.c_size_t(4)), b"workspace of 4 bytes"),
     ]
