@@ -5,6 +5,7 @@
 //   P + j is row j of the slot's cache.
 #include <cuda_bf16.h>
 #include <math.h>
+#include <stdlib.h>
 #include "qlmb_common.cuh"
 #include "qlmb_internal.h"
 
@@ -69,7 +70,8 @@ struct PxParams {
     const int *pos;
     float *part_o, *part_l;                   // [Sp + So][B*n*H][64] and [Sp + So][B*n*H]
     int B, n, P, Tm, H, KV, G, win;
-    int Sp, So, own_items, rt_own, rt_pre;    // pieces; items of the slots' own rows come first; row tiles a (slot, kv head) / a kv head
+    int Sp, So, own_items;                    // pieces of the shared and of the slots' own rows; items of the latter come first
+    int rg_own, rg_pre, lw_own, lw_pre;       // groups of 2^lw tiles of 16 rows a (slot, kv head), resp. a kv head
     float scale_log2;                         // log2(e) / sqrt(64)
     int *errword;
 };
@@ -89,38 +91,51 @@ __device__ __forceinline__ void px_mma(float c[4], const uint32_t a[4], uint32_t
 __device__ __forceinline__ bool px_slot_ok(long long t0, int n, int P, int Tm) { return t0 - P >= -1 && t0 - P + n <= Tm; }
 __device__ __forceinline__ bool px_nonfinite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
-// One tile of 16 query rows against the keys of a piece: four warps take blocks of 32 keys in turn, each with maximum, sum and
-// output of its own, joined through shared memory at the end.  Products on mma.m16n8k16, fed from global memory without a
-// detour: the order of the contracted dimension is free as long as both operands agree, so a thread takes 16 bytes of a key's
-// row (dimensions 8 q .. and 32 + 8 q ..) where the instruction wants pairs, and of V eight neighbouring dimensions of each of
-// its four keys, paired up by byte permutations.
-__global__ void __launch_bounds__(128) k_px_mma(const __grid_constant__ PxParams p)
+// A group of one, two or four tiles of 16 query rows against the keys of a piece: a warp has one tile, and where there are fewer than
+// four they share the keys in blocks of 32, each with maximum, sum and output of its own, joined through shared memory at the end.
+// A warp's blocks come through a ring of its own, three blocks of keys and values in 16-byte pieces whose place in the row is turned
+// by the key; two are under way while one is multiplied on mma.m16n8k16.
+constexpr int PX_NS = 3, PX_BLK = 32 * 128;              // stages, bytes of a block's keys (its values lie behind them)
+constexpr int PX_SMEM = 4 * PX_NS * 2 * PX_BLK;
+__device__ __forceinline__ uint32_t px_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void px_copy(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void px_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void px_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void px_ldm(uint32_t a, uint32_t v[4])
+{ asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory"); }
+__device__ __forceinline__ void px_ldmt(uint32_t a, uint32_t v[4])
+{ asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory"); }
+
+__global__ void __launch_bounds__(128, 2) k_px_mma(const __grid_constant__ PxParams p)
 {
-    __shared__ float so[4][16][PX_HD + 4];
+    extern __shared__ __align__(128) uint8_t px_s[];
     __shared__ float sm[4][16], sl[4][16];
+    float (*so)[16][PX_HD + 4] = reinterpret_cast<float (*)[16][PX_HD + 4]>(px_s);       // at the end, over the rings
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     pdl_trigger();
     pdl_wait();
     const int KD = p.KV * PX_HD, rows_slot = p.n * p.G;
     const bool own = (int)blockIdx.x < p.own_items;
     int it = own ? blockIdx.x : blockIdx.x - p.own_items;
-    int b = 0, kvh, rt, piece, npiece;
+    int b = 0, kvh, rg, piece;
+    const int npiece = own ? p.So : p.Sp, lw = own ? p.lw_own : p.lw_pre;
     const bf16 *K, *V;
     if (own) {
-        piece = it % p.So; it /= p.So; npiece = p.So;
-        rt = it % p.rt_own; it /= p.rt_own;
+        piece = it % p.So; it /= p.So;
+        rg = it % p.rg_own; it /= p.rg_own;
         kvh = it % p.KV; b = it / p.KV;
         K = p.Kc + (size_t)b * p.Tm * KD; V = p.Vc + (size_t)b * p.Tm * KD;
         if (!px_slot_ok(p.pos[b], p.n, p.P, p.Tm)) {
-            if (threadIdx.x == 0 && kvh == 0 && rt == 0 && piece == 0) report_bad_index(p.errword, 306, b, p.pos[b]);
+            if (threadIdx.x == 0 && kvh == 0 && rg == 0 && piece == 0) report_bad_index(p.errword, 306, b, p.pos[b]);
             return;
         }
     } else {
-        piece = it % p.Sp; it /= p.Sp; npiece = p.Sp;
-        rt = it % p.rt_pre; kvh = it / p.rt_pre;
+        rg = it % p.rg_pre; it /= p.rg_pre;               // groups that read the same keys side by side
+        piece = it % p.Sp; kvh = it / p.Sp;
         K = p.Kp; V = p.Vp;
     }
     K += kvh * PX_HD; V += kvh * PX_HD;
+    const int share = warp >> lw, shares = 4 >> lw, rt = (rg << lw) + (warp & ((1 << lw) - 1));      // the warp's part of the keys, its tile
     // the keys lo .. hi of the two rows this thread holds, and of the tile; orow: the row's place in O / 64, -1 where there is none
     int lo[2], hi[2];
     long long orow[2];
@@ -160,38 +175,52 @@ __global__ void __launch_bounds__(128) k_px_mma(const __grid_constant__ PxParams
         const int nblk = (thi - tlo) / 32 + 1, per = (nblk + npiece - 1) / npiece;
         k0 = tlo + min(piece * per, nblk) * 32; k1 = min(thi + 1, tlo + min((piece + 1) * per, nblk) * 32);
     }
+    const int step = 32 * shares;
+    // a lane's pieces of a block: keys kr + 4 i, 16 bytes kc of the row
+    const int kr = lane >> 3, kc = lane & 7;
+    const uint32_t ring = px_addr(px_s) + warp * (PX_NS * 2 * PX_BLK);
+    int lb = k0 + 32 * share, ls = 0;                                  // the next block to be requested, and its stage
+    const auto load = [&]() {
+        if (lb < k1) {
+            const uint32_t d = ring + ls * (2 * PX_BLK) + kr * 128;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const size_t o = (size_t)min(lb + kr + 4 * i, k1 - 1) * KD + 8 * kc;      // keys behind the last: the last once more
+                const uint32_t at = d + i * 512 + ((kc ^ ((kr + 4 * i) & 7)) << 4);
+                px_copy(at, K + o);
+                px_copy(at + PX_BLK, V + o);
+            }
+            lb += step;
+        }
+        ls = ls + 1 == PX_NS ? 0 : ls + 1;
+        px_commit();
+    };
+    load(); load();
     uint32_t qa[4][4];
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        uint4 x = make_uint4(0, 0, 0, 0), y = x;
-        if (orow[e] >= 0) {
-            const bf16 *r = p.Q + (size_t)orow[e] * PX_HD + 8 * q;
-            x = *reinterpret_cast<const uint4 *>(r); y = *reinterpret_cast<const uint4 *>(r + 32);
-        }
-        qa[0][e] = x.x; qa[0][2 + e] = x.y; qa[1][e] = x.z; qa[1][2 + e] = x.w;
-        qa[2][e] = y.x; qa[2][2 + e] = y.y; qa[3][e] = y.z; qa[3][2 + e] = y.w;
-    }
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) qa[s][2 * h + e] = orow[e] >= 0 ? *reinterpret_cast<const uint32_t *>(p.Q + (size_t)orow[e] * PX_HD + 16 * s + 8 * h + 2 * q) : 0u;
     float oc[8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    for (int kb = k0 + 32 * warp; kb < k1; kb += 128) {
-        uint4 kx[4][2], vx[2][4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const bf16 *r = K + (size_t)min(kb + 8 * t + g, k1 - 1) * KD + 8 * q;
-            kx[t][0] = *reinterpret_cast<const uint4 *>(r); kx[t][1] = *reinterpret_cast<const uint4 *>(r + 32);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int w = 0; w < 4; w++)
-                vx[t][w] = *reinterpret_cast<const uint4 *>(V + (size_t)min(kb + 16 * t + 2 * q + (w & 1) + 8 * (w >> 1), k1 - 1) * KD + 8 * g);
+    int stage = 0;
+    for (int kb = k0 + 32 * share; kb < k1; kb += step) {
+        px_wait<1>();
+        __syncwarp();
+        load();                                                        // into the place of the block before this one
+        const uint32_t sk = ring + stage * (2 * PX_BLK), sv = sk + PX_BLK;
+        stage = stage + 1 == PX_NS ? 0 : stage + 1;
         float s[4][4] = {};
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            px_mma(s[t], qa[0], kx[t][0].x, kx[t][0].y);
-            px_mma(s[t], qa[1], kx[t][0].z, kx[t][0].w);
-            px_mma(s[t], qa[2], kx[t][1].x, kx[t][1].y);
-            px_mma(s[t], qa[3], kx[t][1].z, kx[t][1].w);
-        }
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {                              // eight keys, dimensions 32 h .. 32 h + 31
+                uint32_t w[4];
+                px_ldm(sk + (8 * t + (lane & 7)) * 128 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4), w);
+                px_mma(s[t], qa[2 * h], w[0], w[1]);
+                px_mma(s[t], qa[2 * h + 1], w[2], w[3]);
+            }
         const bool edge = kb < alo || kb + 31 > ahi || kb + 32 > k1;   // some row does not see some key
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -226,72 +255,68 @@ __global__ void __launch_bounds__(128) k_px_mma(const __grid_constant__ PxParams
                 const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
                 pa[t >> 1][2 * (t & 1) + e] = *reinterpret_cast<const uint32_t *>(&h2);
             }
+        uint32_t vw[2][4][4];                                          // [16 keys][16 dimensions]: two pairs of operands
         bool odd = false;                                              // an infinity or a NaN that some row must not see
-        if (edge) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                px_ldmt(sv + (16 * t + (lane & 15)) * 128 + (((2 * j + (lane >> 4)) ^ (lane & 7)) << 4), vw[t][j]);
+                if (edge) odd |= px_nonfinite(vw[t][j][0]) | px_nonfinite(vw[t][j][1]) | px_nonfinite(vw[t][j][2]) | px_nonfinite(vw[t][j][3]);
+            }
+        if (!edge || !__any_sync(~0u, odd)) {
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) odd |= px_nonfinite(vx[t][w].x) | px_nonfinite(vx[t][w].y) | px_nonfinite(vx[t][w].z) | px_nonfinite(vx[t][w].w);
-            odd = __any_sync(~0u, odd);
-        }
-        if (!odd) {
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint32_t w0[4] = {vx[t][0].x, vx[t][0].y, vx[t][0].z, vx[t][0].w}, w1[4] = {vx[t][1].x, vx[t][1].y, vx[t][1].z, vx[t][1].w};
-                const uint32_t w2[4] = {vx[t][2].x, vx[t][2].y, vx[t][2].z, vx[t][2].w}, w3[4] = {vx[t][3].x, vx[t][3].y, vx[t][3].z, vx[t][3].w};
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-                    px_mma(oc[j], pa[t], __byte_perm(w0[j >> 1], w1[j >> 1], sel), __byte_perm(w2[j >> 1], w3[j >> 1], sel));
-                }
-            }
+                for (int j = 0; j < 4; j++) { px_mma(oc[2 * j], pa[t], vw[t][j][0], vw[t][j][1]); px_mma(oc[2 * j + 1], pa[t], vw[t][j][2], vw[t][j][3]); }
         } else {
-            // 0 * inf is not 0: row by row, with the keys the row does not see taken as zeros
+            // 0 * inf is not 0: row by row, with the keys the row does not see taken as zeros (a register holds keys 2 q and 2 q + 1 of eight)
             for (int r = 0; r < 16; r++) {
                 const int rlo = __shfl_sync(~0u, r < 8 ? lo[0] : lo[1], (r & 7) * 4), rhi = __shfl_sync(~0u, r < 8 ? hi[0] : hi[1], (r & 7) * 4);
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    bool see[4];
+                    uint32_t see[2];
 #pragma unroll
-                    for (int w = 0; w < 4; w++) { const int key = kb + 16 * t + 2 * q + (w & 1) + 8 * (w >> 1); see[w] = key >= rlo && key <= rhi && key < k1; }
-                    const uint32_t *v0 = &vx[t][0].x, *v1 = &vx[t][1].x, *v2 = &vx[t][2].x, *v3 = &vx[t][3].x;
+                    for (int h = 0; h < 2; h++) {
+                        const int key = kb + 16 * t + 8 * h + 2 * q;
+                        see[h] = (key >= rlo && key <= rhi && key < k1 ? 0xffffu : 0u) | (key + 1 >= rlo && key + 1 <= rhi && key + 1 < k1 ? 0xffff0000u : 0u);
+                    }
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
                         float c[4] = {};
-                        px_mma(c, pa[t], __byte_perm(see[0] ? v0[j >> 1] : 0u, see[1] ? v1[j >> 1] : 0u, sel),
-                               __byte_perm(see[2] ? v2[j >> 1] : 0u, see[3] ? v3[j >> 1] : 0u, sel));
+                        px_mma(c, pa[t], vw[t][j >> 1][2 * (j & 1)] & see[0], vw[t][j >> 1][2 * (j & 1) + 1] & see[1]);
                         if (r == g) { oc[j][0] += c[0]; oc[j][1] += c[1]; }
                         if (r == g + 8) { oc[j][2] += c[2]; oc[j][3] += c[3]; }
                     }
                 }
             }
         }
+        __syncwarp();                                                  // the block is read: the next copies may take its place
     }
-    // the four warps' shares; a thread holds columns 16 q .. 16 q + 15 of its rows (column 8 c + j of product j)
+    px_wait<0>();
+    __syncthreads();
+    // a thread holds columns 8 j + 2 q and the next of its rows
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         l[e] += __shfl_xor_sync(~0u, l[e], 1);
         l[e] += __shfl_xor_sync(~0u, l[e], 2);
         if (q == 0) { sm[warp][g + 8 * e] = m[e]; sl[warp][g + 8 * e] = l[e]; }
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            float *d = &so[warp][g + 8 * e][16 * q + 8 * c];
-            *reinterpret_cast<float4 *>(d) = make_float4(oc[0][2 * e + c], oc[1][2 * e + c], oc[2][2 * e + c], oc[3][2 * e + c]);
-            *reinterpret_cast<float4 *>(d + 4) = make_float4(oc[4][2 * e + c], oc[5][2 * e + c], oc[6][2 * e + c], oc[7][2 * e + c]);
-        }
+        for (int j = 0; j < 8; j++) *reinterpret_cast<float2 *>(&so[warp][g + 8 * e][8 * j + 2 * q]) = make_float2(oc[j][2 * e], oc[j][2 * e + 1]);
     }
     __syncthreads();
-    const int r = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8, rr = rt * 16 + r;
+    // the tiles' rows, eight threads each, over the shares
+    for (int tile = 0; tile < 1 << lw; tile++) {
+    const int r = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8, rr = ((rg << lw) + tile) * 16 + r;
     long long at = -1;
     if (own) { if (rr < rows_slot) at = ((long long)b * p.n + rr / p.G) * p.H + kvh * p.G + rr % p.G; }
     else if (rr < p.B * rows_slot && px_slot_ok(p.pos[rr / p.G / p.n], p.n, p.P, p.Tm)) at = (long long)(rr / p.G) * p.H + kvh * p.G + rr % p.G;
-    if (at < 0) return;
-    float mm = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+    if (at < 0) continue;
+    float mm = -INFINITY;
+    for (int w = tile; w < 4; w += 1 << lw) mm = fmaxf(mm, sm[w][r]);
     const float mref = mm == -INFINITY ? 0.0f : mm;
     float ll = 0.0f, a[8] = {};
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = tile; w < 4; w += 1 << lw) {
         if (sm[w][r] == -INFINITY && sl[w][r] == 0.0f) continue;       // this warp saw nothing (a NaN among the scores leaves a sum of NaN)
         const float f = px_ex2(sm[w][r] - mref);
         ll += sl[w][r] * f;
@@ -309,14 +334,15 @@ __global__ void __launch_bounds__(128) k_px_mma(const __grid_constant__ PxParams
         }
         *reinterpret_cast<uint4 *>(p.O + (size_t)at * PX_HD + c8) = make_uint4(w[0], w[1], w[2], w[3]);
         if (p.lse && c8 == 0) p.lse[at] = lg * 0.6931471805599453f;
-        return;
+        continue;
     }
     const size_t po = (size_t)(own ? p.Sp + piece : piece) * ((size_t)p.B * p.n * p.H) + (size_t)at;
     if (c8 == 0) p.part_l[po] = lg;
-    if (none) return;                                                  // the join does not read it
+    if (none) continue;                                                // the join does not read it
     float *d = p.part_o + po * PX_HD + c8;
     *reinterpret_cast<float4 *>(d) = make_float4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
     *reinterpret_cast<float4 *>(d + 4) = make_float4(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv);
+    }
 }
 
 // A warp per row of O: the pieces' outputs weighted by 2^(their logarithm - the largest), in ascending order.
@@ -333,43 +359,64 @@ __global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParam
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
     const float mref = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f, x = 0.0f, y = 0.0f;
+    // half a warp has the 64 columns of a piece, four of its pieces are under way at a time; an empty one's output was not written
+    const int half = lane >> 4, c4 = 4 * (lane & 15);
+    float sum = 0.0f, x[4] = {};
     for (int s0 = 0; s0 < S; s0 += 32) {
         const float w = s0 + lane < S ? px_ex2(p.part_l[(s0 + lane) * rows + at] - mref) : 0.0f;
-        for (int k = 0; k < 32 && s0 + k < S; k++) {
-            const float wk = __shfl_sync(~0u, w, k);
-            if (wk == 0.0f) continue;                                  // an empty piece's output was not written
-            const float2 o = *reinterpret_cast<const float2 *>(p.part_o + ((s0 + k) * rows + at) * PX_HD + 2 * lane);
-            sum += wk; x += wk * o.x; y += wk * o.y;
+        for (int k0 = 0; k0 < 32 && s0 + k0 < S; k0 += 8) {
+            float wk[4];
+            float4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int s = k0 + 2 * k + half;
+                wk[k] = __shfl_sync(~0u, w, s);
+                o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (wk[k] != 0.0f) o[k] = *reinterpret_cast<const float4 *>(p.part_o + ((s0 + s) * rows + at) * PX_HD + c4);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) { sum += wk[k]; x[0] += wk[k] * o[k].x; x[1] += wk[k] * o[k].y; x[2] += wk[k] * o[k].z; x[3] += wk[k] * o[k].w; }
         }
     }
+    sum += __shfl_xor_sync(~0u, sum, 16);
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[k] += __shfl_xor_sync(~0u, x[k], 16);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<__nv_bfloat162 *>(p.O + at * PX_HD + 2 * lane) = __floats2bfloat162_rn(x * inv, y * inv);
+    if (half == 0) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0] * inv, x[1] * inv), b = __floats2bfloat162_rn(x[2] * inv, x[3] * inv);
+        *reinterpret_cast<uint2 *>(p.O + at * PX_HD + c4) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
     if (p.lse && lane == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mref + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Pieces of a call.
-struct PxPlan { int Sp, So, rt_own, rt_pre, tc, per; };
+struct PxPlan { int Sp, So, rg_own, rg_pre, lw_own, lw_pre, tc, per; };
 static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
 {
     PxPlan pl = {};
-    const long long want = 3LL * sm_count();
     const long long rows = (long long)B * n * (H / KV);
-    pl.rt_own = (n * (H / KV) + 15) / 16;
-    pl.rt_pre = (int)((rows + 15) / 16);
+    const auto tiles = [](long long rows, int *lw, int *rg) {
+        const long long t = (rows + 15) / 16;
+        *lw = t <= 1 ? 0 : t <= 2 ? 1 : 2;
+        *rg = (int)((t + (1 << *lw) - 1) >> *lw);
+    };
+    tiles((long long)n * (H / KV), &pl.lw_own, &pl.rg_own);
+    tiles(rows, &pl.lw_pre, &pl.rg_pre);
     const auto pieces = [](long long want, long long items, long long keys) {
         const long long most = (keys + 127) / 128, s = want / items;
         return (int)(s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s);
     };
-    pl.So = pieces(want, (long long)B * KV * pl.rt_own, Tm);
+    int w1 = 3, w2 = 3, lim = 64;
+    { const char *e = getenv("PX_W1"); if (e) w1 = atoi(e); e = getenv("PX_W2"); if (e) w2 = atoi(e); e = getenv("PX_LIM"); if (e) lim = atoi(e); }
+    pl.So = pieces((long long)w1 * sm_count(), (long long)B * KV * pl.rg_own, Tm);
     if (P > 0) {
-        pl.tc = rows > 16 && win <= 0;
+        pl.tc = rows > lim && win <= 0;
         if (pl.tc) {
-            const int tiles = (P + 127) / 128, s = pieces(2LL * sm_count(), KV * ((rows + 127) / 128), P);
-            pl.per = (tiles + s - 1) / s;
-            pl.Sp = (tiles + pl.per - 1) / pl.per;
+            const int t = (P + 127) / 128, s = pieces(2LL * sm_count(), KV * ((rows + 127) / 128), P);
+            pl.per = (t + s - 1) / s;
+            pl.Sp = (t + pl.per - 1) / pl.per;
         } else
-            pl.Sp = pieces(want, (long long)KV * pl.rt_pre, P);
+            pl.Sp = pieces((long long)w2 * sm_count(), (long long)KV * pl.rg_pre, P);
     }
     return pl;
 }
@@ -426,8 +473,8 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     p.part_o = (float *)ws; p.part_l = p.part_o + (size_t)(pl.Sp + pl.So) * rows * PX_HD;
     p.B = B; p.n = n; p.P = P; p.Tm = Tm; p.H = H; p.KV = KV; p.G = H / KV;
     p.win = win < (1 << 30) ? win : 0;                                 // such a window hides nothing
-    p.Sp = pl.Sp; p.So = pl.So; p.rt_own = pl.rt_own; p.rt_pre = pl.rt_pre;
-    const long long own_items = (long long)B * KV * pl.rt_own * pl.So, items = own_items + (pl.tc ? 0 : (long long)KV * pl.rt_pre * pl.Sp);
+    p.Sp = pl.Sp; p.So = pl.So; p.rg_own = pl.rg_own; p.rg_pre = pl.rg_pre; p.lw_own = pl.lw_own; p.lw_pre = pl.lw_pre;
+    const long long own_items = (long long)B * KV * pl.rg_own * pl.So, items = own_items + (pl.tc ? 0 : (long long)KV * pl.rg_pre * pl.Sp);
     QLMB_REQUIRE(items < (1LL << 31), "qlmb_dec_attn_prefix: %lld pieces are too many", items);
     p.own_items = (int)own_items;
     p.scale_log2 = 1.4426950408889634f * 0.125f;
@@ -438,7 +485,15 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
         const int rc = attn_prefix_launch(px, Kp, Vp, P, H, KV, st);
         if (rc) return rc;
     }
-    QLMB_CUDA(pdl_launch_small(k_px_mma, dim3((unsigned)items), dim3(128), 0, st, p));
+    static bool configured_dev[64];                                    // the attribute belongs to a device's copy of the kernel
+    int dev = 0;
+    QLMB_CUDA(cudaGetDevice(&dev));
+    QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
+    if (!configured_dev[dev]) {
+        QLMB_CUDA(cudaFuncSetAttribute(k_px_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM));
+        configured_dev[dev] = true;
+    }
+    QLMB_CUDA(pdl_launch_small(k_px_mma, dim3((unsigned)items), dim3(128), PX_SMEM, st, p));
     QLMB_LAUNCH_CHECK("k_px_mma");
     if (pl.Sp + pl.So > 1) {
         QLMB_CUDA(pdl_launch(true, k_px_join, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p));
