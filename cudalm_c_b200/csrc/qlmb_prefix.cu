@@ -3,11 +3,14 @@
 //
 //   t = pos[b] + i is the position of token i of slot b; positions below P are rows of Kp, Vp (one copy for all slots), position
 //   P + j is row j of the slot's cache.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <math.h>
+#include <string.h>
 #include <stdlib.h>
 #include "qlmb_common.cuh"
-#include "qlmb_internal.h"
+#include "qlmb_gemm.cuh"
+#include "qlmb_attn.cuh"
 
 namespace qlmb {
 
@@ -60,28 +63,31 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 }
 
 // ------------------------------------------------------------------ attention
-// The keys of a row are cut into pieces: the shared rows into Sp, the slot's own into So.  A piece of a tile of 16 query rows is
-// one CTA's; it leaves the piece's output, normalised, and the logarithm (base 2) of its sum, and k_px_join adds the pieces up.
-// Rows of one kv head that stand side by side: the G = H / KV heads of a token, then the next token's (prefix: of all slots).
+// Rows of queries of one kv head stand side by side in tiles of 16: the G = H / KV heads of a token, then the next token's.  An item
+// is a tile and the keys its rows may see: a slot's own rows (tiles of the slot's n G rows), or the shared ones (tiles of all slots').
+// Keys come in blocks of 32.  The blocks of all items, one after the other, are dealt out evenly to the warps of the device, a run
+// each, whatever the slots' lengths: a warp goes through its run with a ring of asynchronous copies that does not stop at the
+// items' borders, and leaves of each item that it meets a segment: output in fp32, normalised, and the logarithm (base 2) of its
+// sum.  Segment number = item + warp, which no two share.  k_px_join adds the segments of a row up.
+//
+// With many rows a kv head the shared keys are k_attn_fwd's (qlmb_attn.cu: 128 rows a tile on tcgen05), in pieces of their own.
+constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
+constexpr int PX_MAXB = 1024;                             // slots: every CTA keeps their positions and block counts
 struct PxParams {
+    alignas(64) CUtensorMap kc_map, vc_map, kp_map, vp_map;
     bf16 *O;
     float *lse;
-    const bf16 *Q, *Kp, *Vp, *Kc, *Vc;
+    const bf16 *Q;
     const int *pos;
-    float *part_o, *part_l;                   // [Sp + So][B*n*H][64] and [Sp + So][B*n*H]
+    float *seg_o, *seg_l;                     // [items + warps][16][64] and [items + warps][16]
+    float *part_o, *part_l;                   // the shared keys' pieces of k_attn_fwd: [Sp][B*n*H][64] and [Sp][B*n*H]
+    int *table;                               // for the join: blocks ahead of each slot's items [B + 1], then of a shared item, then a warp's
     int B, n, P, Tm, H, KV, G, win;
-    int Sp, So, own_items;                    // pieces of the shared and of the slots' own rows; items of the latter come first
-    int rg_own, rg_pre, lw_own, lw_pre;       // groups of 2^lw tiles of 16 rows a (slot, kv head), resp. a kv head
+    int Sp, t_own, t_pre, warps, least;       // least: blocks of a warp at least; pieces of k_attn_fwd (0: the shared keys are items); tiles a (slot, kv head) / a kv head
     float scale_log2;                         // log2(e) / sqrt(64)
     int *errword;
 };
 
-__device__ __forceinline__ float px_ex2(float x)      // 2^x (ex2.approx: 2 ulp, -inf -> 0)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void px_mma(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -91,14 +97,11 @@ __device__ __forceinline__ void px_mma(float c[4], const uint32_t a[4], uint32_t
 __device__ __forceinline__ bool px_slot_ok(long long t0, int n, int P, int Tm) { return t0 - P >= -1 && t0 - P + n <= Tm; }
 __device__ __forceinline__ bool px_nonfinite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
-// A group of one, two or four tiles of 16 query rows against the keys of a piece: a warp has one tile, and where there are fewer than
-// four they share the keys in blocks of 32, each with maximum, sum and output of its own, joined through shared memory at the end.
-// A warp's blocks come through a ring of its own, three blocks of keys and values in 16-byte pieces whose place in the row is turned
-// by the key; two are under way while one is multiplied on mma.m16n8k16.
-constexpr int PX_NS = 3, PX_BLK = 32 * 128;              // stages, bytes of a block's keys (its values lie behind them)
-constexpr int PX_SMEM = 4 * PX_NS * 2 * PX_BLK;
-__device__ __forceinline__ uint32_t px_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void px_copy(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+constexpr int PX_BLK = 32 * 128, PX_STAGE = 2 * PX_BLK;      // a block's keys; keys and values
+constexpr int PX_Q = PX_WARPS * 2 * PX_STAGE, PX_RINGS = PX_Q + PX_WARPS * 16 * 128;      // two blocks a warp, then an item's queries a warp
+static size_t px_smem(int B) { return (size_t)PX_RINGS + 256 + (size_t)(2 * B + 1) * sizeof(int); }
+__device__ __forceinline__ void px_copy(uint32_t dst, const void *src, bool in)      // 16 bytes, zeros where !in
+{ asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); }
 __device__ __forceinline__ void px_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void px_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void px_ldm(uint32_t a, uint32_t v[4])
@@ -106,111 +109,198 @@ __device__ __forceinline__ void px_ldm(uint32_t a, uint32_t v[4])
 __device__ __forceinline__ void px_ldmt(uint32_t a, uint32_t v[4])
 { asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory"); }
 
-__global__ void __launch_bounds__(128, 2) k_px_mma(const __grid_constant__ PxParams p)
+// The blocks of a slot's own keys: from its first visible one, in whole blocks, to the last new token's.
+__device__ __forceinline__ int px_first(const PxParams &p, int t0) { return p.win > 0 ? max(0, t0 - p.win + 1 - p.P) & ~31 : 0; }
+__device__ __forceinline__ int px_blocks(const PxParams &p, long long t0)
 {
-    extern __shared__ __align__(128) uint8_t px_s[];
-    __shared__ float sm[4][16], sl[4][16];
-    float (*so)[16][PX_HD + 4] = reinterpret_cast<float (*)[16][PX_HD + 4]>(px_s);       // at the end, over the rings
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    if (!px_slot_ok(t0, p.n, p.P, p.Tm)) return 0;
+    const int hi = (int)t0 + p.n - 1 - p.P;
+    return hi < 0 ? 0 : (hi - px_first(p, (int)t0)) / 32 + 1;
+}
+// x / d for 0 <= x < 2^24: the quotient of the floats is off by one at most (a division of integers takes ten times as long)
+__device__ __forceinline__ int px_div(int x, int d)
+{
+    int r = __float2int_rz(__fdividef((float)x, (float)d));
+    const int left = x - r * d;
+    return left < 0 ? r - 1 : left >= d ? r + 1 : r;
+}
+// a place in the row of all blocks: item `sub` of slot b (b = B: of the shared keys), the block's first key, the item's last
+struct PxCursor { int b, sub, key, last; };
+
+__global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_constant__ PxParams p)
+{
+    extern __shared__ __align__(1024) uint8_t px_s[];
+    uint64_t *bars = reinterpret_cast<uint64_t *>(px_s + PX_RINGS);                       // a ring's stages are full
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 2 * PX_WARPS);
+    int *plan = const_cast<int *>(abort_flag) + 1;                                        // first key and blocks of a shared item, blocks of a warp
+    int *cum = reinterpret_cast<int *>(px_s + PX_RINGS + 256), *start = cum + p.B + 1;    // blocks of one item of each slot ahead of slot b; its first new position
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    if (smem_u32(px_s) & 1023u) {             // the swizzled blocks need a 1 KiB-aligned base
+        if (tid == 0 && p.errword && atomicCAS(p.errword, 0, 201) == 0) { p.errword[1] = 130; p.errword[2] = (int)blockIdx.x; }
+        pdl_wait();
+        return;
+    }
+    if (tid == 0) {
+        prefetch_map(&p.kc_map); prefetch_map(&p.vc_map);
+        if (!p.Sp && p.P > 0) { prefetch_map(&p.kp_map); prefetch_map(&p.vp_map); }
+        for (int i = 0; i < 2 * PX_WARPS; i++) mbar_init(smem_u32(&bars[i]), 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
     pdl_trigger();
     pdl_wait();
-    const int KD = p.KV * PX_HD, rows_slot = p.n * p.G;
-    const bool own = (int)blockIdx.x < p.own_items;
-    int it = own ? blockIdx.x : blockIdx.x - p.own_items;
-    int b = 0, kvh, rg, piece;
-    const int npiece = own ? p.So : p.Sp, lw = own ? p.lw_own : p.lw_pre;
-    const bf16 *K, *V;
-    if (own) {
-        piece = it % p.So; it /= p.So;
-        rg = it % p.rg_own; it /= p.rg_own;
-        kvh = it % p.KV; b = it / p.KV;
-        K = p.Kc + (size_t)b * p.Tm * KD; V = p.Vc + (size_t)b * p.Tm * KD;
-        if (!px_slot_ok(p.pos[b], p.n, p.P, p.Tm)) {
-            if (threadIdx.x == 0 && kvh == 0 && rg == 0 && piece == 0) report_bad_index(p.errword, 306, b, p.pos[b]);
-            return;
-        }
-    } else {
-        rg = it % p.rg_pre; it /= p.rg_pre;               // groups that read the same keys side by side
-        piece = it % p.Sp; kvh = it / p.Sp;
-        K = p.Kp; V = p.Vp;
-    }
-    K += kvh * PX_HD; V += kvh * PX_HD;
-    const int share = warp >> lw, shares = 4 >> lw, rt = (rg << lw) + (warp & ((1 << lw) - 1));      // the warp's part of the keys, its tile
-    // the keys lo .. hi of the two rows this thread holds, and of the tile; orow: the row's place in O / 64, -1 where there is none
-    int lo[2], hi[2];
-    long long orow[2];
+    const int KT = p.KV * p.t_own;
+    // ---- the slots' block counts, added up by the first warp
+    if (warp == 0) {
+        int carry = 0, first = 0x7fffffff;
+        for (int b0 = 0; b0 < p.B; b0 += 32) {
+            const int b = b0 + lane, t0 = b < p.B ? p.pos[b] : 0, v = b < p.B ? px_blocks(p, t0) : 0;
+            int x = v;
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        const int rr = rt * 16 + g + 8 * e;
-        lo[e] = 0; hi[e] = -1; orow[e] = -1;
-        if (own) {
-            if (rr < rows_slot) {
-                const int i = rr / p.G, t = p.pos[b] + i;
-                orow[e] = ((long long)b * p.n + i) * p.H + kvh * p.G + rr % p.G;
-                hi[e] = t - p.P;
-                if (p.win > 0) lo[e] = max(0, t - p.win + 1 - p.P);
+            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(~0u, x, o); if (lane >= o) x += y; }
+            if (b < p.B) {
+                start[b] = t0;
+                cum[b] = carry + x - v;
+                if (px_slot_ok(t0, p.n, p.P, p.Tm)) first = min(first, t0);
+                else if (blockIdx.x == 0) report_bad_index(p.errword, 306, b, t0);
             }
-        } else if (rr < p.B * rows_slot) {
-            const int token = rr / p.G, t0 = p.pos[token / p.n];
-            if (px_slot_ok(t0, p.n, p.P, p.Tm)) {
-                const int t = t0 + token % p.n;
-                orow[e] = (long long)token * p.H + kvh * p.G + rr % p.G;
-                hi[e] = p.P - 1;
-                if (p.win > 0) lo[e] = max(0, t - p.win + 1);
-            }
+            carry += __shfl_sync(~0u, x, 31);
         }
-        if (lo[e] > hi[e]) { lo[e] = 0x7fffffff; hi[e] = -1; }         // sees nothing here
+        first = __reduce_min_sync(~0u, first);
+        if (lane == 0) {
+            cum[p.B] = carry;
+            // the shared keys that some row sees, the same for every item
+            const int lo = p.win > 0 && first != 0x7fffffff ? max(0, first - p.win + 1) & ~31 : 0;
+            const int n = p.Sp || lo >= p.P || first == 0x7fffffff ? 0 : (p.P - 1 - lo) / 32 + 1;
+            const unsigned total = (unsigned)carry * KT + (unsigned)n * p.KV * p.t_pre;
+            plan[0] = lo; plan[1] = n; plan[2] = (int)max((unsigned)p.least, (total + p.warps - 1) / p.warps);
+        }
     }
-    int tlo = min(lo[0], lo[1]), thi = max(hi[0], hi[1]);
-    int alo = orow[0] < 0 ? -1 : lo[0], ahi = orow[0] < 0 ? 0x7fffffff : hi[0];      // what every row of the tile sees
-    if (orow[1] >= 0) { alo = max(alo, lo[1]); ahi = min(ahi, hi[1]); }
-#pragma unroll
-    for (int o = 16; o >= 4; o >>= 1) {
-        tlo = min(tlo, __shfl_xor_sync(~0u, tlo, o)); thi = max(thi, __shfl_xor_sync(~0u, thi, o));
-        alo = max(alo, __shfl_xor_sync(~0u, alo, o)); ahi = min(ahi, __shfl_xor_sync(~0u, ahi, o));
+    __syncthreads();
+    const int rows_slot = p.n * p.G, lo_pre = plan[0], n_pre = plan[1];
+    const unsigned own = (unsigned)cum[p.B] * KT, total = own + (unsigned)n_pre * p.KV * p.t_pre, per = plan[2];
+    if (blockIdx.x == 0) {
+        for (int b = tid; b <= p.B; b += 32 * PX_WARPS) p.table[b] = cum[b];
+        if (tid == 0) { p.table[p.B + 1] = n_pre; p.table[p.B + 2] = (int)per; }
     }
-    int k0 = 0, k1 = 0;                                                // keys of this piece: whole blocks of 32
-    if (thi >= 0) {
-        tlo &= ~31;
-        const int nblk = (thi - tlo) / 32 + 1, per = (nblk + npiece - 1) / npiece;
-        k0 = tlo + min(piece * per, nblk) * 32; k1 = min(thi + 1, tlo + min((piece + 1) * per, nblk) * 32);
+    const unsigned me = blockIdx.x * PX_WARPS + warp;
+    const unsigned from = me * per;                       // (the warps' number times per is little more than total: no overflow)
+    if (from >= total) return;
+    int count = (int)min(per, total - from);              // blocks of this warp
+    // ---- the first of them
+    const auto open = [&](PxCursor &c, int blk) {         // block blk of item (b, sub)
+        if (c.b < p.B) { const int t0 = start[c.b]; c.key = px_first(p, t0) + 32 * blk; c.last = t0 + p.n - 1 - p.P; }
+        else { c.key = lo_pre + 32 * blk; c.last = p.P - 1; }
+    };
+    PxCursor lc;
+    {
+        int blk;
+        if (from < own) {
+            int lo = 0, hi = p.B - 1;                     // the last slot that starts at or before it
+            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if ((unsigned)cum[mid] * KT <= from) lo = mid; else hi = mid - 1; }
+            const unsigned off = from - (unsigned)cum[lo] * KT, nb = cum[lo + 1] - cum[lo];
+            lc.b = lo; lc.sub = off / nb; blk = off % nb;
+        } else { lc.b = p.B; lc.sub = (from - own) / n_pre; blk = (from - own) % n_pre; }
+        open(lc, blk);
     }
-    const int step = 32 * shares;
-    // a lane's pieces of a block: keys kr + 4 i, 16 bytes kc of the row
+    PxCursor cc = lc;
+    // the next block; true where another item begins
+    const auto step = [&](PxCursor &c) {
+        c.key += 32;
+        if (c.key <= c.last) return false;
+        c.sub++;
+        if (c.b < p.B && c.sub == KT) {
+            c.sub = 0;
+            do c.b++; while (c.b < p.B && cum[c.b + 1] == cum[c.b]);
+        }
+        open(c, 0);
+        return true;
+    };
+    // row r of an item's tile: its place in O / 64 (-1: none) and its position
+    const auto row_of = [&](int b, int sub, int r, int &t) {
+        if (b < p.B) {
+            const int kvh = px_div(sub, p.t_own), rr = (sub - kvh * p.t_own) * 16 + r, i = px_div(rr, p.G);
+            t = start[b] + i;
+            return rr < rows_slot ? (b * p.n + i) * p.H + kvh * p.G + rr - i * p.G : -1;
+        }
+        const int kvh = px_div(sub, p.t_pre), rr = (sub - kvh * p.t_pre) * 16 + r, token = px_div(rr, p.G), s = px_div(token, p.n);
+        if (rr >= p.B * rows_slot || !px_slot_ok(start[s], p.n, p.P, p.Tm)) return -1;
+        t = start[s] + token - s * p.n;
+        return token * p.H + kvh * p.G + rr - token * p.G;
+    };
+    // ---- the ring; of an item's queries a lane has rows kr + 4 i, 16 bytes kc of the row
     const int kr = lane >> 3, kc = lane & 7;
-    const uint32_t ring = px_addr(px_s) + warp * (PX_NS * 2 * PX_BLK);
-    int lb = k0 + 32 * share, ls = 0;                                  // the next block to be requested, and its stage
+    const uint32_t ring = smem_u32(px_s) + warp * (2 * PX_STAGE), sq = smem_u32(px_s) + PX_Q + warp * (16 * 128);
+    const uint64_t *bar = bars + 2 * warp;
+    int ls = 0, to_load = count;
+    bool fresh = true;                                    // the block to be requested is the first of an item here
+    int orow = -1, opos = 0;                              // of the item that was requested last: row lane % 16
     const auto load = [&]() {
-        if (lb < k1) {
-            const uint32_t d = ring + ls * (2 * PX_BLK) + kr * 128;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const size_t o = (size_t)min(lb + kr + 4 * i, k1 - 1) * KD + 8 * kc;      // keys behind the last: the last once more
-                const uint32_t at = d + i * 512 + ((kc ^ ((kr + 4 * i) & 7)) << 4);
-                px_copy(at, K + o);
-                px_copy(at + PX_BLK, V + o);
+        if (to_load > 0) {
+            const bool mine = lc.b < p.B;
+            const uint32_t d = ring + ls * PX_STAGE;
+            if (elect_one()) {
+                const uint32_t full = smem_u32(bar + ls);
+                const int x = px_div(lc.sub, mine ? p.t_own : p.t_pre) * PX_HD, y = mine ? lc.b * p.Tm + lc.key : lc.key;
+                mbar_expect_tx(full, 2 * PX_BLK);
+                tma_load_2d(d, mine ? &p.kc_map : &p.kp_map, full, x, y);
+                tma_load_2d(d + PX_BLK, mine ? &p.vc_map : &p.vp_map, full, x, y);
             }
-            lb += step;
+            __syncwarp();
+            if (fresh) {
+                orow = row_of(lc.b, lc.sub, lane & 15, opos);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int o = __shfl_sync(~0u, orow, kr + 4 * i);
+                    px_copy(sq + (kr + 4 * i) * 128 + ((kc ^ ((kr + 4 * i) & 7)) << 4), p.Q + (size_t)max(o, 0) * PX_HD + 8 * kc, o >= 0);
+                }
+            }
+            if (--to_load > 0) fresh = step(lc);
         }
-        ls = ls + 1 == PX_NS ? 0 : ls + 1;
+        ls ^= 1;
         px_commit();
     };
-    load(); load();
+    load();
+    int lo[2], hi[2], alo = 0, ahi = 0, stage = 0;        // the keys lo .. hi of the thread's two rows; those that every row of the tile sees
+    bool live[2];
     uint32_t qa[4][4];
-#pragma unroll
-    for (int s = 0; s < 4; s++)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) qa[s][2 * h + e] = orow[e] >= 0 ? *reinterpret_cast<const uint32_t *>(p.Q + (size_t)orow[e] * PX_HD + 16 * s + 8 * h + 2 * q) : 0u;
-    float oc[8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    int stage = 0;
-    for (int kb = k0 + 32 * share; kb < k1; kb += step) {
-        px_wait<1>();
+    float oc[8][4], m[2], l[2];
+    bool begin = true;
+    uint32_t phase = 0;
+    for (; count > 0; count--) {
+        px_wait<0>();
+        if (!__all_sync(~0u, at_wait(smem_u32(bar + stage), phase, abort_flag, p.errword, 131))) break;
         __syncwarp();
-        load();                                                        // into the place of the block before this one
-        const uint32_t sk = ring + stage * (2 * PX_BLK), sv = sk + PX_BLK;
-        stage = stage + 1 == PX_NS ? 0 : stage + 1;
+        const uint32_t sk = ring + stage * PX_STAGE, sv = sk + PX_BLK;
+        phase ^= stage;
+        stage ^= 1;
+        const int kb = cc.key, k1 = cc.last + 1;
+        if (begin) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int t = __shfl_sync(~0u, opos, g + 8 * e);
+                live[e] = __shfl_sync(~0u, orow, g + 8 * e) >= 0;
+                lo[e] = 0; hi[e] = -1;
+                if (live[e]) {
+                    hi[e] = cc.b < p.B ? t - p.P : p.P - 1;
+                    if (p.win > 0) lo[e] = max(0, t - p.win + 1 - (cc.b < p.B ? p.P : 0));
+                }
+                if (lo[e] > hi[e]) { lo[e] = 0x7fffffff; hi[e] = -1; }
+                m[e] = -INFINITY; l[e] = 0.0f;
+            }
+            alo = live[0] ? lo[0] : -1; ahi = live[0] ? hi[0] : 0x7fffffff;
+            if (live[1]) { alo = max(alo, lo[1]); ahi = min(ahi, hi[1]); }
+#pragma unroll
+            for (int o = 16; o >= 4; o >>= 1) { alo = max(alo, __shfl_xor_sync(~0u, alo, o)); ahi = min(ahi, __shfl_xor_sync(~0u, ahi, o)); }
+#pragma unroll
+            for (int s = 0; s < 4; s++) px_ldm(sq + (lane & 15) * 128 + (((2 * s + (lane >> 4)) ^ (lane & 7)) << 4), qa[s]);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) oc[j][k] = 0.0f;
+            __syncwarp();                                 // the queries are read
+        }
+        load();                                           // into the place of the block before this one
         float s[4][4] = {};
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -222,55 +312,73 @@ __global__ void __launch_bounds__(128, 2) k_px_mma(const __grid_constant__ PxPar
                 px_mma(s[t], qa[2 * h + 1], w[2], w[3]);
             }
         const bool edge = kb < alo || kb + 31 > ahi || kb + 32 > k1;   // some row does not see some key
-        float mx[2] = {-INFINITY, -INFINITY};
+        if (__builtin_expect(edge, 0)) {
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int e = c >> 1, key = kb + 8 * t + 2 * q + (c & 1);
-                s[t][c] *= p.scale_log2;
-                if (edge && (key < lo[e] || key > hi[e] || key >= k1)) s[t][c] = -INFINITY;
-                mx[e] = fmaxf(mx[e], s[t][c]);
-            }
-        float mu[2];
+                for (int c = 0; c < 4; c++) {
+                    const int key = kb + 8 * t + 2 * q + (c & 1);
+                    if (key < lo[c >> 1] || key > hi[c >> 1] || key >= k1) s[t][c] = -INFINITY;
+                }
+        }
+        float mn[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(~0u, mx[e], 1));
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(~0u, mx[e], 2));
-            const float mn = fmaxf(m[e], mx[e]);
-            mu[e] = mn == -INFINITY ? 0.0f : mn;                       // nothing seen yet: every weight 0
-            const float corr = px_ex2(m[e] - mu[e]);
-            m[e] = mn;
-            l[e] *= corr;
+            float mx = fmaxf(fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1])),
+                             fmaxf(fmaxf(s[2][2 * e], s[2][2 * e + 1]), fmaxf(s[3][2 * e], s[3][2 * e + 1])));
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+            mn[e] = fmaxf(m[e], mx * p.scale_log2);
+        }
+        if (__any_sync(~0u, mn[0] > m[0] || mn[1] > m[1])) {            // a new maximum in some row
 #pragma unroll
-            for (int j = 0; j < 8; j++) { oc[j][2 * e] *= corr; oc[j][2 * e + 1] *= corr; }
+            for (int e = 0; e < 2; e++) {
+                const float corr = ex2(m[e] - (mn[e] == -INFINITY ? 0.0f : mn[e]));
+                m[e] = mn[e];
+                l[e] *= corr;
+#pragma unroll
+                for (int j = 0; j < 8; j++) { oc[j][2 * e] *= corr; oc[j][2 * e + 1] *= corr; }
+            }
         }
         uint32_t pa[2][4];                                             // weights in bf16, as every attention of the library has them
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int e = 0; e < 2; e++) {
+            const float mu = m[e] == -INFINITY ? 0.0f : m[e];          // nothing seen yet: every weight 0
+            float sum[2] = {};
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const float p0 = px_ex2(s[t][2 * e] - mu[e]), p1 = px_ex2(s[t][2 * e + 1] - mu[e]);
-                l[e] += p0 + p1;
+            for (int t = 0; t < 4; t++) {
+                const float p0 = ex2(fmaf(s[t][2 * e], p.scale_log2, -mu)), p1 = ex2(fmaf(s[t][2 * e + 1], p.scale_log2, -mu));
+                sum[t & 1] += p0 + p1;
                 const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
                 pa[t >> 1][2 * (t & 1) + e] = *reinterpret_cast<const uint32_t *>(&h2);
             }
+            l[e] += sum[0] + sum[1];
+        }
         uint32_t vw[2][4][4];                                          // [16 keys][16 dimensions]: two pairs of operands
-        bool odd = false;                                              // an infinity or a NaN that some row must not see
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                px_ldmt(sv + (16 * t + (lane & 15)) * 128 + (((2 * j + (lane >> 4)) ^ (lane & 7)) << 4), vw[t][j]);
-                if (edge) odd |= px_nonfinite(vw[t][j][0]) | px_nonfinite(vw[t][j][1]) | px_nonfinite(vw[t][j][2]) | px_nonfinite(vw[t][j][3]);
-            }
-        if (!edge || !__any_sync(~0u, odd)) {
+            for (int j = 0; j < 4; j++) px_ldmt(sv + (16 * t + (lane & 15)) * 128 + (((2 * j + (lane >> 4)) ^ (lane & 7)) << 4), vw[t][j]);
+        bool odd = false;                                              // an infinity or a NaN that some row must not see
+        if (__builtin_expect(edge, 0)) {                               // keys behind the item's last are nobody's (a register holds keys 2 q and 2 q + 1 of eight)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int key = kb + 16 * t + 8 * (k & 1) + 2 * q;
+                    const uint32_t in = (key < k1 ? 0xffffu : 0u) | (key + 1 < k1 ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) { vw[t][j][k] &= in; odd |= px_nonfinite(vw[t][j][k]); }
+                }
+        }
+        if (__builtin_expect(!edge || !__any_sync(~0u, odd), 1)) {
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) { px_mma(oc[2 * j], pa[t], vw[t][j][0], vw[t][j][1]); px_mma(oc[2 * j + 1], pa[t], vw[t][j][2], vw[t][j][3]); }
         } else {
-            // 0 * inf is not 0: row by row, with the keys the row does not see taken as zeros (a register holds keys 2 q and 2 q + 1 of eight)
+            // 0 * inf is not 0: row by row, with the keys the row does not see taken as zeros
+#pragma unroll 1
             for (int r = 0; r < 16; r++) {
                 const int rlo = __shfl_sync(~0u, r < 8 ? lo[0] : lo[1], (r & 7) * 4), rhi = __shfl_sync(~0u, r < 8 ? hi[0] : hi[1], (r & 7) * 4);
 #pragma unroll
@@ -292,90 +400,83 @@ __global__ void __launch_bounds__(128, 2) k_px_mma(const __grid_constant__ PxPar
             }
         }
         __syncwarp();                                                  // the block is read: the next copies may take its place
+        const PxCursor was = cc;
+        begin = count == 1 || step(cc);
+        if (begin) {                                                   // this warp's segment of the item is whole
+            const size_t seg = (size_t)(was.b < p.B ? (long long)was.b * KT + was.sub : (long long)p.B * KT + was.sub) + me;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                l[e] += __shfl_xor_sync(~0u, l[e], 1);
+                l[e] += __shfl_xor_sync(~0u, l[e], 2);
+                if (!live[e]) continue;
+                const bool none = l[e] == 0.0f;                        // the join does not read such a segment's output
+                if (q == 0) p.seg_l[seg * 16 + g + 8 * e] = none ? -INFINITY : (m[e] == -INFINITY ? 0.0f : m[e]) + __log2f(l[e]);
+                if (none) continue;
+                const float inv = __fdividef(1.0f, l[e]);
+                float *d = p.seg_o + (seg * 16 + g + 8 * e) * PX_HD + 2 * q;
+#pragma unroll
+                for (int j = 0; j < 8; j++) *reinterpret_cast<float2 *>(d + 8 * j) = make_float2(oc[j][2 * e] * inv, oc[j][2 * e + 1] * inv);
+            }
+        }
     }
     px_wait<0>();
-    __syncthreads();
-    // a thread holds columns 8 j + 2 q and the next of its rows
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-        l[e] += __shfl_xor_sync(~0u, l[e], 1);
-        l[e] += __shfl_xor_sync(~0u, l[e], 2);
-        if (q == 0) { sm[warp][g + 8 * e] = m[e]; sl[warp][g + 8 * e] = l[e]; }
-#pragma unroll
-        for (int j = 0; j < 8; j++) *reinterpret_cast<float2 *>(&so[warp][g + 8 * e][8 * j + 2 * q]) = make_float2(oc[j][2 * e], oc[j][2 * e + 1]);
-    }
-    __syncthreads();
-    // the tiles' rows, eight threads each, over the shares
-    for (int tile = 0; tile < 1 << lw; tile++) {
-    const int r = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8, rr = ((rg << lw) + tile) * 16 + r;
-    long long at = -1;
-    if (own) { if (rr < rows_slot) at = ((long long)b * p.n + rr / p.G) * p.H + kvh * p.G + rr % p.G; }
-    else if (rr < p.B * rows_slot && px_slot_ok(p.pos[rr / p.G / p.n], p.n, p.P, p.Tm)) at = (long long)(rr / p.G) * p.H + kvh * p.G + rr % p.G;
-    if (at < 0) continue;
-    float mm = -INFINITY;
-    for (int w = tile; w < 4; w += 1 << lw) mm = fmaxf(mm, sm[w][r]);
-    const float mref = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f, a[8] = {};
-    for (int w = tile; w < 4; w += 1 << lw) {
-        if (sm[w][r] == -INFINITY && sl[w][r] == 0.0f) continue;       // this warp saw nothing (a NaN among the scores leaves a sum of NaN)
-        const float f = px_ex2(sm[w][r] - mref);
-        ll += sl[w][r] * f;
-#pragma unroll
-        for (int k = 0; k < 8; k++) a[k] += so[w][r][c8 + k] * f;
-    }
-    const bool none = ll == 0.0f;
-    const float inv = none ? 0.0f : 1.0f / ll, lg = none ? -INFINITY : mref + log2f(ll);
-    if (p.Sp + p.So == 1) {                                            // the only piece: its output is the row's
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const __nv_bfloat162 h2 = none ? __floats2bfloat162_rn(0.0f, 0.0f) : __floats2bfloat162_rn(a[2 * k] * inv, a[2 * k + 1] * inv);
-            w[k] = *reinterpret_cast<const uint32_t *>(&h2);
-        }
-        *reinterpret_cast<uint4 *>(p.O + (size_t)at * PX_HD + c8) = make_uint4(w[0], w[1], w[2], w[3]);
-        if (p.lse && c8 == 0) p.lse[at] = lg * 0.6931471805599453f;
-        continue;
-    }
-    const size_t po = (size_t)(own ? p.Sp + piece : piece) * ((size_t)p.B * p.n * p.H) + (size_t)at;
-    if (c8 == 0) p.part_l[po] = lg;
-    if (none) continue;                                                // the join does not read it
-    float *d = p.part_o + po * PX_HD + c8;
-    *reinterpret_cast<float4 *>(d) = make_float4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-    *reinterpret_cast<float4 *>(d + 4) = make_float4(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv);
-    }
+    if (*abort_flag)                                      // aborting: the copies under way must land before the CTA gives its shared memory back
+        for (int i = 0; i < 2; i++)
+            for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(bar + i), i < stage ? phase ^ 1u : phase); k++) {}
 }
 
-// A warp per row of O: the pieces' outputs weighted by 2^(their logarithm - the largest), in ascending order.
+// A warp per row of O: its segments and pieces weighted by 2^(their logarithm - the largest), in a fixed order.
 __global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParams p)
 {
     const int lane = threadIdx.x & 31;
     const size_t rows = (size_t)p.B * p.n * p.H, at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     pdl_trigger();
     pdl_wait();
-    if (at >= rows || !px_slot_ok(p.pos[at / ((size_t)p.n * p.H)], p.n, p.P, p.Tm)) return;
-    const int S = p.Sp + p.So;
-    float mx = -INFINITY;
-    for (int s = lane; s < S; s += 32) mx = fmaxf(mx, p.part_l[s * rows + at]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
-    const float mref = mx == -INFINITY ? 0.0f : mx;
-    // half a warp has the 64 columns of a piece, four of its pieces are under way at a time; an empty one's output was not written
+    if (at >= rows) return;
+    const int token = px_div((int)at, p.H), h = (int)at - token * p.H, b = px_div(token, p.n), kvh = px_div(h, p.G), KT = p.KV * p.t_own;
+    const int c0 = p.table[b], nb = p.table[b + 1] - c0, all = p.table[p.B], n_pre = p.table[p.B + 1];
+    const unsigned per = p.table[p.B + 2];
+    if (!px_slot_ok(p.pos[b], p.n, p.P, p.Tm)) return;
+    // the row's segments of its slot's keys, then of the shared ones, then the pieces
+    const int hg = h - kvh * p.G, rr = (token - b * p.n) * p.G + hg, rp = token * p.G + hg, so = kvh * p.t_own + rr / 16, sp = kvh * p.t_pre + rp / 16;
+    const unsigned x0 = (unsigned)c0 * KT + (unsigned)so * nb, x1 = (unsigned)all * KT + (unsigned)sp * n_pre;
+    const int w0 = x0 / per, s0 = nb ? (int)((x0 + nb - 1) / per) - w0 + 1 : 0;
+    const int w1 = x1 / per, s1 = n_pre ? (int)((x1 + n_pre - 1) / per) - w1 + 1 : 0;
+    const size_t g0 = ((size_t)b * KT + so + w0) * 16 + rr % 16, g1 = ((size_t)p.B * KT + sp + w1) * 16 + rp % 16;
+    const int S = s0 + s1 + p.Sp;
+    const auto place = [&](int s) { return s < s0 ? g0 + 16 * (size_t)s : s < s0 + s1 ? g1 + 16 * (size_t)(s - s0) : (size_t)(s - s0 - s1) * rows + at; };
+    // half a warp has the 64 columns of a segment, eight are under way at a time, the first of them while the largest logarithm is
+    // found; an empty one's output was not written
     const int half = lane >> 4, c4 = 4 * (lane & 15);
-    float sum = 0.0f, x[4] = {};
-    for (int s0 = 0; s0 < S; s0 += 32) {
-        const float w = s0 + lane < S ? px_ex2(p.part_l[(s0 + lane) * rows + at] - mref) : 0.0f;
-        for (int k0 = 0; k0 < 32 && s0 + k0 < S; k0 += 8) {
-            float wk[4];
-            float4 o[4];
+    float lg[4], mx = -INFINITY;
+    float4 o[4];
+    const auto fetch = [&](int k0) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int s = k0 + 2 * k + half;
-                wk[k] = __shfl_sync(~0u, w, s);
-                o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (wk[k] != 0.0f) o[k] = *reinterpret_cast<const float4 *>(p.part_o + ((s0 + s) * rows + at) * PX_HD + c4);
+        for (int k = 0; k < 4; k++) {
+            const int s = k0 + 2 * k + half;
+            lg[k] = -INFINITY;
+            o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (s < S) {
+                const size_t pl = place(s);
+                const bool seg = s < s0 + s1;
+                lg[k] = (seg ? p.seg_l : p.part_l)[pl];
+                o[k] = *reinterpret_cast<const float4 *>((seg ? p.seg_o : p.part_o) + pl * PX_HD + c4);
             }
+        }
+    };
+    fetch(0);
+    for (int s = lane; s < S; s += 32) mx = fmaxf(mx, (s < s0 + s1 ? p.seg_l : p.part_l)[place(s)]);
 #pragma unroll
-            for (int k = 0; k < 4; k++) { sum += wk[k]; x[0] += wk[k] * o[k].x; x[1] += wk[k] * o[k].y; x[2] += wk[k] * o[k].z; x[3] += wk[k] * o[k].w; }
+    for (int i = 16; i; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, i));
+    const float mref = mx == -INFINITY ? 0.0f : mx;
+    float sum = 0.0f, x[4] = {};
+    for (int k0 = 0; k0 < S; k0 += 8) {
+        if (k0) fetch(k0);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float w = ex2(lg[k] - mref);
+            if (w == 0.0f) continue;
+            sum += w; x[0] += w * o[k].x; x[1] += w * o[k].y; x[2] += w * o[k].z; x[3] += w * o[k].w;
         }
     }
     sum += __shfl_xor_sync(~0u, sum, 16);
@@ -383,47 +484,46 @@ __global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParam
     for (int k = 0; k < 4; k++) x[k] += __shfl_xor_sync(~0u, x[k], 16);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (half == 0) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0] * inv, x[1] * inv), b = __floats2bfloat162_rn(x[2] * inv, x[3] * inv);
-        *reinterpret_cast<uint2 *>(p.O + at * PX_HD + c4) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0] * inv, x[1] * inv), c = __floats2bfloat162_rn(x[2] * inv, x[3] * inv);
+        *reinterpret_cast<uint2 *>(p.O + at * PX_HD + c4) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&c));
     }
     if (p.lse && lane == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mref + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Pieces of a call.
-struct PxPlan { int Sp, So, rg_own, rg_pre, lw_own, lw_pre, tc, per; };
+// What a call needs: tiles, items, warps, pieces of k_attn_fwd (Sp of `per` tiles of keys), bytes of the workspace's parts.
+struct PxPlan { int t_own, t_pre, warps, Sp, per; size_t seg_o, seg_l, part_o, part_l, table, bytes; };
 static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
 {
     PxPlan pl = {};
     const long long rows = (long long)B * n * (H / KV);
-    const auto tiles = [](long long rows, int *lw, int *rg) {
-        const long long t = (rows + 15) / 16;
-        *lw = t <= 1 ? 0 : t <= 2 ? 1 : 2;
-        *rg = (int)((t + (1 << *lw) - 1) >> *lw);
-    };
-    tiles((long long)n * (H / KV), &pl.lw_own, &pl.rg_own);
-    tiles(rows, &pl.lw_pre, &pl.rg_pre);
-    const auto pieces = [](long long want, long long items, long long keys) {
-        const long long most = (keys + 127) / 128, s = want / items;
-        return (int)(s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s);
-    };
-    int w1 = 3, w2 = 3, lim = 64;
-    { const char *e = getenv("PX_W1"); if (e) w1 = atoi(e); e = getenv("PX_W2"); if (e) w2 = atoi(e); e = getenv("PX_LIM"); if (e) lim = atoi(e); }
-    pl.So = pieces((long long)w1 * sm_count(), (long long)B * KV * pl.rg_own, Tm);
-    if (P > 0) {
-        pl.tc = rows > lim && win <= 0;
-        if (pl.tc) {
-            const int t = (P + 127) / 128, s = pieces(2LL * sm_count(), KV * ((rows + 127) / 128), P);
-            pl.per = (t + s - 1) / s;
-            pl.Sp = (t + pl.per - 1) / pl.per;
-        } else
-            pl.Sp = pieces((long long)w2 * sm_count(), (long long)KV * pl.rg_pre, P);
+    int lim = 64;
+    { const char *e = getenv("PX_LIM"); if (e) lim = atoi(e); }
+    const bool tc = P > 0 && rows > lim && win <= 0;
+    pl.t_own = (n * (H / KV) + 15) / 16;
+    pl.t_pre = P > 0 && !tc ? (int)((rows + 15) / 16) : 0;
+    pl.warps = sm_count() * PX_WARPS;
+    if (tc) {
+        const long long t = (P + 127) / 128, ctas = KV * ((rows + 127) / 128);
+        long long s = 2LL * sm_count() / ctas;
+        s = s < 1 ? 1 : s > t ? t : s;
+        pl.per = (int)((t + s - 1) / s);
+        pl.Sp = (int)((t + pl.per - 1) / pl.per);
     }
+    const size_t segs = (size_t)B * KV * pl.t_own + (size_t)KV * pl.t_pre + pl.warps, all = (size_t)B * n * H;
+    pl.seg_o = segs * 16 * PX_HD * sizeof(float);
+    pl.seg_l = segs * 16 * sizeof(float);
+    pl.part_o = (size_t)pl.Sp * all * PX_HD * sizeof(float);
+    pl.part_l = ((size_t)pl.Sp * all * sizeof(float) + 15) / 16 * 16;
+    pl.table = (size_t)(B + 3) * sizeof(int);
+    pl.bytes = pl.seg_o + pl.seg_l + pl.part_o + pl.part_l + pl.table;
     return pl;
 }
 static bool px_shape_ok(int B, int n, int P, int Tm, int H, int KV)
 {
-    return B > 0 && n > 0 && n <= 64 && P >= 0 && Tm > 0 && H > 0 && KV > 0 && H % KV == 0 && (long long)P + Tm < (1LL << 30) &&
-           (long long)B * n * H < (1LL << 24) && (long long)H * 64 < (1LL << 20);
+    return B > 0 && B <= PX_MAXB && n > 0 && n <= 64 && P >= 0 && Tm > 0 && H > 0 && KV > 0 && H % KV == 0 && (long long)P + Tm < (1LL << 30) &&
+           (long long)B * n * H < (1LL << 24) && (long long)H * 64 < (1LL << 20) &&
+           (long long)B * Tm < (1LL << 31) - 64 &&                     // rows of the caches and blocks are counted in 32 bits
+           (long long)B * KV * ((n * (H / KV) + 15) / 16) * (Tm / 32 + 2) + (long long)KV * (((long long)B * n * (H / KV) + 15) / 16) * (P / 32 + 2) < (1LL << 31);
 }
 
 }  // namespace qlmb
@@ -449,9 +549,8 @@ extern "C" int qlmb_dec_rope_kv(void *Qo, void *Kc, void *Vc, const void *q, con
 extern "C" size_t qlmb_dec_attn_prefix_bytes(int B, int n, int P, int Tm, int H, int KV)
 {
     if (!px_shape_ok(B, n, P, Tm, H, KV)) return 0;
-    const PxPlan pl = px_plan(B, n, P, Tm, H, KV, 0), pw = px_plan(B, n, P, Tm, H, KV, 1);
-    const size_t S = (size_t)pl.So + (pl.Sp > pw.Sp ? pl.Sp : pw.Sp);
-    return S * (size_t)B * n * H * (PX_HD + 1) * sizeof(float) + 16;
+    const size_t a = px_plan(B, n, P, Tm, H, KV, 0).bytes, b = px_plan(B, n, P, Tm, H, KV, 1).bytes;
+    return a > b ? a : b;
 }
 
 extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const void *Kp, const void *Vp, const void *Kc, const void *Vc, const int *pos,
@@ -460,27 +559,36 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     QLMB_REQUIRE(O && Q && Kc && Vc && pos && ws && (P == 0 || (Kp && Vp)), "qlmb_dec_attn_prefix: NULL argument");
     QLMB_REQUIRE(hd == PX_HD, "qlmb_dec_attn_prefix: head dimension %d (only 64 is built)", hd);
     if (B <= 0) return QLMB_OK;
-    QLMB_REQUIRE(px_shape_ok(B, n, P, Tm, H, KV), "qlmb_dec_attn_prefix: bad shape B %d n %d P %d Tm %d H %d KV %d", B, n, P, Tm, H, KV);
+    QLMB_REQUIRE(px_shape_ok(B, n, P, Tm, H, KV), "qlmb_dec_attn_prefix: bad shape B %d (up to %d) n %d P %d Tm %d H %d KV %d", B, PX_MAXB, n, P, Tm, H, KV);
     QLMB_REQUIRE((((uintptr_t)O | (uintptr_t)Q | (uintptr_t)Kp | (uintptr_t)Vp | (uintptr_t)Kc | (uintptr_t)Vc | (uintptr_t)ws) & 15) == 0,
                  "qlmb_dec_attn_prefix: rows, caches and workspace must be 16-byte aligned");
-    const size_t need = qlmb_dec_attn_prefix_bytes(B, n, P, Tm, H, KV);
-    QLMB_REQUIRE(ws_bytes >= need, "qlmb_dec_attn_prefix: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
     const PxPlan pl = px_plan(B, n, P, Tm, H, KV, win);
-    PxParams p = {};
+    QLMB_REQUIRE(ws_bytes >= pl.bytes, "qlmb_dec_attn_prefix: a workspace of %zu bytes, %zu are needed", ws_bytes, pl.bytes);
+    PxParams p;
+    memset(&p, 0, sizeof p);
     const size_t rows = (size_t)B * n * H;
-    p.O = (bf16 *)O; p.lse = lse; p.Q = (const bf16 *)Q;
-    p.Kp = (const bf16 *)Kp; p.Vp = (const bf16 *)Vp; p.Kc = (const bf16 *)Kc; p.Vc = (const bf16 *)Vc; p.pos = pos;
-    p.part_o = (float *)ws; p.part_l = p.part_o + (size_t)(pl.Sp + pl.So) * rows * PX_HD;
+    char *w = (char *)ws;
+    const unsigned long long width = (unsigned long long)KV * PX_HD;
+    const struct { CUtensorMap *m; const void *base; unsigned long long rows; } maps[4] = {
+        {&p.kc_map, Kc, (unsigned long long)B * Tm}, {&p.vc_map, Vc, (unsigned long long)B * Tm}, {&p.kp_map, Kp, (unsigned long long)P}, {&p.vp_map, Vp, (unsigned long long)P}};
+    for (int i = 0; i < (P > 0 && !pl.Sp ? 4 : 2); i++) {
+        const int rc = make_map(maps[i].m, maps[i].base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, width, maps[i].rows, width * 2, PX_HD, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc) return rc;
+    }
+    p.O = (bf16 *)O; p.lse = lse; p.Q = (const bf16 *)Q; p.pos = pos;
+    p.seg_o = (float *)w; w += pl.seg_o;
+    p.seg_l = (float *)w; w += pl.seg_l;
+    p.part_o = (float *)w; w += pl.part_o;
+    p.part_l = (float *)w; w += pl.part_l;
+    p.table = (int *)w;
     p.B = B; p.n = n; p.P = P; p.Tm = Tm; p.H = H; p.KV = KV; p.G = H / KV;
     p.win = win < (1 << 30) ? win : 0;                                 // such a window hides nothing
-    p.Sp = pl.Sp; p.So = pl.So; p.rg_own = pl.rg_own; p.rg_pre = pl.rg_pre; p.lw_own = pl.lw_own; p.lw_pre = pl.lw_pre;
-    const long long own_items = (long long)B * KV * pl.rg_own * pl.So, items = own_items + (pl.tc ? 0 : (long long)KV * pl.rg_pre * pl.Sp);
-    QLMB_REQUIRE(items < (1LL << 31), "qlmb_dec_attn_prefix: %lld pieces are too many", items);
-    p.own_items = (int)own_items;
+    p.Sp = pl.Sp; p.t_own = pl.t_own; p.t_pre = pl.t_pre > 0 ? pl.t_pre : 1; p.warps = pl.warps; p.least = 2;
+    { const char *e = getenv("PX_LEAST"); if (e) p.least = atoi(e); }
     p.scale_log2 = 1.4426950408889634f * 0.125f;
     p.errword = device_error_word();
     cudaStream_t st = as_stream(stream);
-    if (pl.tc) {
+    if (pl.Sp) {
         const PrefixAttn px = {p.Q, p.part_o, p.part_l, rows, (int)(rows / KV), pl.Sp, pl.per};
         const int rc = attn_prefix_launch(px, Kp, Vp, P, H, KV, st);
         if (rc) return rc;
@@ -490,14 +598,12 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     QLMB_CUDA(cudaGetDevice(&dev));
     QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
     if (!configured_dev[dev]) {
-        QLMB_CUDA(cudaFuncSetAttribute(k_px_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, PX_SMEM));
+        QLMB_CUDA(cudaFuncSetAttribute(k_px_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)px_smem(PX_MAXB)));
         configured_dev[dev] = true;
     }
-    QLMB_CUDA(pdl_launch_small(k_px_mma, dim3((unsigned)items), dim3(128), PX_SMEM, st, p));
+    QLMB_CUDA(pdl_launch_small(k_px_mma, dim3((unsigned)(pl.warps / PX_WARPS)), dim3(32 * PX_WARPS), px_smem(B), st, p));
     QLMB_LAUNCH_CHECK("k_px_mma");
-    if (pl.Sp + pl.So > 1) {
-        QLMB_CUDA(pdl_launch(true, k_px_join, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p));
-        QLMB_LAUNCH_CHECK("k_px_join");
-    }
+    QLMB_CUDA(pdl_launch(true, k_px_join, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p));
+    QLMB_LAUNCH_CHECK("k_px_join");
     return QLMB_OK;
 }

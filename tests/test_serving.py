@@ -45,9 +45,9 @@ def test_refusals_of_the_entry_points():
         (lambda: attn(nbytes=ctypes.c_size_t(16)), b"workspace of 16 bytes"),
         (lambda: verify(out=None), b"NULL"), (lambda: verify(draft=None), b"NULL"), (lambda: verify(dt=2), b"type"), (lambda: verify(n=-1), b"n -1"),
         (lambda: verify(n=64), b"n 64"), (lambda: verify(V=0), b"V 0"), (lambda: verify(ld=15), b"rows of 15"), (lambda: verify(ldq=15), b"and 15"),
-        (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None), b"workspace"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
+        (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None, K=8192), b"workspace"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
         (lambda: lora(K=60), b"multiples of 8"), (lambda: lora(N=63), b"multiples of 8"), (lambda: lora(R=12), b"rank 12"), (lambda: lora(R=264), b"rank 264"),
-        (lambda: lora(R=0), b"rank 0"), (lambda: lora(X=odd), b"aligned"), (lambda: lora(nbytes=ctypes.c_size_t(4)), b"workspace of 4 bytes"),
+        (lambda: lora(R=0), b"rank 0"), (lambda: lora(X=odd), b"aligned"), (lambda: lora(K=8192, nbytes=ctypes.c_size_t(4)), b"workspace of 4 bytes"),
     ]
     for i, (call, needle) in enumerate(cases):
         assert call() == 1, i
@@ -57,12 +57,12 @@ def test_refusals_of_the_entry_points():
     assert attn(B=0) == 0 and lora(M=0) == 0
     assert L.qlmb_dec_verify(one, one, one, one, 0, 16, one, 16, one, None, one, one, 0, 2, 16, None) == 0
     # workspaces: 0 where the shape is not supported
-    for bad in ((0, 1, 8, 8, 2, 2), (1, 65, 8, 8, 2, 2), (1, 1, -1, 8, 2, 2), (1, 1, 8, 8, 3, 2), (1, 1, 1 << 30, 8, 2, 2), (1 << 23, 2, 8, 8, 2, 2)):
+    for bad in ((0, 1, 8, 8, 2, 2), (1, 65, 8, 8, 2, 2), (1, 1, -1, 8, 2, 2), (1, 1, 8, 8, 3, 2), (1, 1, 1 << 30, 8, 2, 2), (1025, 2, 8, 8, 2, 2), (1024, 1, 8, 1 << 22, 2, 2)):
         assert L.qlmb_dec_attn_prefix_bytes(*bad) == 0, bad
     assert L.qlmb_dec_attn_prefix_bytes(2, 3, 100, 50, 4, 2) > 0
     for bad in ((0, 64, 64, 8), (4, 60, 64, 8), (4, 64, 64, 4), (4, 64, 64, 300)):
         assert L.qlmb_lora_bytes(*bad) == 0, bad
-    assert L.qlmb_lora_bytes(5, 64, 128, 16) >= 5 * 16 * 4
+    assert L.qlmb_lora_bytes(5, 64, 128, 16) == 16 and L.qlmb_lora_bytes(5, 4096, 128, 16) >= 5 * 16 * 4
 
 
 def test_refusals_of_the_mirrors():
