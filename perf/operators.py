@@ -281,7 +281,9 @@ def _verify(s):
 def _lora(s):
     if own:
         from cudalm_c_b200 import linear
-        return linear.lora_add(s["x"], s["base"], s["a"], s["b"], s["scale"], s["adapter"], order=s["order"])
+        # fp32 rows are added to where they are, as below, where float() makes no copy of them
+        out = s["base"] if s["base"].dtype == torch.float32 else None
+        return linear.lora_add(s["x"], s["base"], s["a"], s["b"], s["scale"], s["adapter"], order=s["order"], out=out)
     y = s["base"].float()
     for i, rows in s["groups"]:
         t = torch.matmul(s["x"][rows].float(), s["a"][i].float().t())
