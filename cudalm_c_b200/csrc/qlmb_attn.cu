@@ -41,7 +41,6 @@ struct AttnFwdParams {
     int B, T, H, KV, win, nqt;
     float scale_log2;                         // log2(e) / sqrt(hd)
     int *errword;
-    PrefixAttn px;                            // k_attn_fwd<true>
 };
 
 template <int M> struct AtMode { static constexpr int value = M; };     // which masks a tile needs
@@ -83,18 +82,6 @@ __device__ __forceinline__ void attn_store_rot(bf16 *dst, uint32_t taddr, bool l
         }
     }
 }
-// two floats in one 64-bit register: sm_100's two-wide multiply-add and add
-__device__ __forceinline__ uint64_t f2_packu(uint32_t a, uint32_t b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) { return f2_packu(__float_as_uint(a), __float_as_uint(b)); }
-__device__ __forceinline__ void f2_unpack(uint64_t v, float &a, float &b)
-{
-    uint32_t x, y;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(v));
-    a = __uint_as_float(x); b = __uint_as_float(y);
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-
 // 32 fp32 TMEM columns of this thread's lane, times mul -> 64 bytes of bf16 in global memory
 // (tcgen05.ld is warp-collective: every lane runs it, only live lanes store)
 __device__ __forceinline__ void attn_store_row32(bf16 *dst, uint32_t taddr, bool live, float mul)
@@ -119,10 +106,7 @@ __device__ __forceinline__ void attn_store_row64(bf16 *dst, uint32_t taddr, bool
     attn_store_row32(dst + 32, taddr + 32, live, mul);
 }
 
-// PX: the queries of a decode step against the rows that its slots share (qlmb_dec_attn_prefix).  A tile is 128 of the rows of one
-// kv head, the G = H / KV heads of a token side by side, then the next token's; every row sees every key, and a CTA takes a piece of
-// them: it leaves the piece's output in fp32, normalised, and the logarithm (base 2) of its sum.
-template <bool PX> __global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_fwd(const __grid_constant__ AttnFwdParams p)
+__global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_fwd(const __grid_constant__ AttnFwdParams p)
 {
     extern __shared__ __align__(1024) uint8_t at_smem[];
     constexpr int NS = AT_FWD_NS;
@@ -139,10 +123,9 @@ template <bool PX> __global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_f
         pdl_wait();
         return;
     }
-    // uniform over the CTA; PX: a slot that was reported (code 201) leaves the others' rows to be made
-    if (__syncthreads_or(threadIdx.x == 0 && (PX ? p.errword && *reinterpret_cast<const volatile int *>(p.errword) == 200 : at_error_seen(p.errword)))) { pdl_wait(); return; }
+    if (__syncthreads_or(threadIdx.x == 0 && at_error_seen(p.errword))) { pdl_wait(); return; }   // uniform over the CTA
     if (threadIdx.x == 0) {
-        mbar_init(smem_u32(q_full), PX ? 4 : 1);
+        mbar_init(smem_u32(q_full), 1);
         for (int i = 0; i < NS; i++) { mbar_init(smem_u32(&kv_full[i]), 1); mbar_init(smem_u32(&kv_empty[i]), 1); }
         mbar_init(smem_u32(s_full), 1);
         mbar_init(smem_u32(s_free), 4);
@@ -161,24 +144,21 @@ template <bool PX> __global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_f
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tS = tmem_base, tO = tmem_base + 128, tP = tmem_base + 192;
 
-    // heaviest query tiles first (PX: the row tiles of a piece, which read the same keys, side by side)
+    // heaviest query tiles first
     const int BH = p.B * p.H;
-    const int qt = PX ? (int)blockIdx.x % p.nqt : p.nqt - 1 - (int)blockIdx.x / BH, bh = (int)blockIdx.x % BH;
-    const int b = PX ? 0 : bh / p.H, h = bh % p.H, piece = PX ? (int)blockIdx.x / p.nqt % p.px.pieces : 0;
-    const int kvh = PX ? (int)blockIdx.x / p.nqt / p.px.pieces : h / (p.H / p.KV);
+    const int qt = p.nqt - 1 - (int)blockIdx.x / BH, bh = (int)blockIdx.x % BH;
+    const int b = bh / p.H, h = bh % p.H, kvh = h / (p.H / p.KV);
     const int q0 = qt * AT_BM;
-    int kt_lo = 0, kt_hi = (q0 + AT_BM - 1 < p.T ? q0 + AT_BM - 1 : p.T - 1) / AT_BN;     // inclusive
-    if (PX) {
-        kt_lo = piece * p.px.per;
-        kt_hi = min(kt_lo + p.px.per, (p.T + AT_BN - 1) / AT_BN) - 1;
-    } else if (p.win > 0) { int lo = q0 - p.win + 1; kt_lo = lo > 0 ? lo / AT_BN : 0; }
+    int kt_lo = 0;
+    if (p.win > 0) { int lo = q0 - p.win + 1; kt_lo = lo > 0 ? lo / AT_BN : 0; }
+    const int kt_hi = (q0 + AT_BM - 1 < p.T ? q0 + AT_BM - 1 : p.T - 1) / AT_BN;     // inclusive
     const int nt = kt_hi - kt_lo + 1;
 
     if (warp == 0) {
         // =============================== TMA producer ===============================
         bool ok = true;
         int issued = 0;
-        if (!PX && elect_one()) {
+        if (elect_one()) {
             mbar_expect_tx(smem_u32(q_full), AT_TILE);
             tma_load_2d(smem_u32(sQ), &p.q_map, smem_u32(q_full), h * AT_HD, b * p.T + q0);
         }
@@ -198,7 +178,7 @@ template <bool PX> __global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_f
         }
         if (*abort_flag) {
             // aborting: the copies this warp started must land before the CTA gives its shared memory back
-            for (uint32_t i = 0; !PX && i < AT_WAIT_LIMIT && !mbar_try(smem_u32(q_full), 0); i++) {}
+            for (uint32_t i = 0; i < AT_WAIT_LIMIT && !mbar_try(smem_u32(q_full), 0); i++) {}
             for (int t = issued > NS ? issued - NS : 0; t < issued; t++)
                 for (uint32_t i = 0; i < AT_WAIT_LIMIT && !mbar_try(smem_u32(&kv_full[t % NS]), (uint32_t)(t / NS) & 1u); i++) {}
         }
@@ -255,42 +235,13 @@ template <bool PX> __global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_f
         const int q = warp & 3, r = q * 32 + lane, i = q0 + r;
         const uint32_t lane_base = (uint32_t)(q * 32) << 16;
         const int iw = q0 + q * 32;                                     // the warp's first query
-        const int G = PX ? p.H / p.KV : 1;
-        const bool warp_live = !PX || iw < p.px.rows;                   // PX: rows behind the last are neither computed nor stored
-        // PX: the row's place in O / 64 (its token and head); a row of the Q tile a thread, 16-byte chunks in the 128-byte swizzle
-        size_t at = 0;
-        if (PX) {
-            uint4 x[8];
-            const bool live = i < p.px.rows;
-            if (live) {
-                at = (size_t)(i / G) * p.H + (size_t)kvh * G + i % G;
-                const uint4 *src = reinterpret_cast<const uint4 *>(p.px.Q + at * AT_HD);
-#pragma unroll
-                for (int c = 0; c < 8; c++) x[c] = src[c];
-            }
-            if (warp_live) {
-#pragma unroll
-                for (int c = 0; c < 8; c++) *reinterpret_cast<uint4 *>(sQ + r * 128 + ((c ^ (r & 7)) << 4)) = live ? x[c] : make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(q_full));
-        }
         const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
-        float m = PX ? -3e38f : -1e30f, l = 0.0f;
+        float m = -1e30f, l = 0.0f;
         bool ok = true;
         for (int t = 0; ok && t < nt; t++) {
             const int k0 = (kt_lo + t) * AT_BN;
             ok = at_wait(smem_u32(s_full), (uint32_t)t & 1u, abort_flag, p.errword, 120);
             if (!ok) break;
-            if (PX && !warp_live) {                                     // its rows of P are whatever TMEM holds: no row reads another's
-                if (lane == 0) mbar_arrive(smem_u32(s_free));
-                if (t > 0) ok = at_wait(smem_u32(o_full), (uint32_t)(t - 1) & 1u, abort_flag, p.errword, 121);   // p_full counts its steps one by one
-                if (!ok) break;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(p_full));
-                continue;
-            }
             tc_fence_after();
             uint32_t v[2][64];
 #pragma unroll
@@ -301,14 +252,14 @@ template <bool PX> __global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_f
             if (lane == 0) mbar_arrive(smem_u32(s_free));
             // Halves of 64 keys: all of them visible to the warp's 32 queries, some, or none.  A key that a query does not
             // see becomes -inf and gets the weight 0.
-            auto none = [&](int c) { return PX ? k0 + c * 64 >= p.T : k0 + c * 64 > iw + 31 || (p.win > 0 && k0 + c * 64 + 63 <= iw - p.win); };
-            float mx = PX ? -3e38f : -1e30f;
+            auto none = [&](int c) { return k0 + c * 64 > iw + 31 || (p.win > 0 && k0 + c * 64 + 63 <= iw - p.win); };
+            float mx = -1e30f;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int kc = k0 + c * 64;
                 if (none(c)) continue;
-                if (PX ? kc + 63 >= p.T : kc + 63 > iw || (p.win > 0 && kc <= iw + 31 - p.win)) {
-                    const int hi = PX ? p.T - 1 - kc : i - kc, lo = !PX && p.win > 0 ? hi - p.win : -1;
+                if (kc + 63 > iw || (p.win > 0 && kc <= iw + 31 - p.win)) {
+                    const int hi = i - kc, lo = p.win > 0 ? hi - p.win : -1;
 #pragma unroll
                     for (int j = 0; j < 64; j++) v[c][j] = j <= hi && j > lo ? v[c][j] : 0xff800000u;
                 }
@@ -381,26 +332,7 @@ template <bool PX> __global__ void __launch_bounds__(AT_FWD_THREADS, 2) k_attn_f
             if (lane == 0) mbar_arrive(smem_u32(p_full));
         }
         if (ok) ok = at_wait(smem_u32(o_full), (uint32_t)(nt - 1) & 1u, abort_flag, p.errword, 122);
-        if (PX && ok && warp_live) {
-            tc_fence_after();
-            const bool some = i < p.px.rows && l != 0.0f;               // l = 0: every score -inf; the join does not read such a piece
-            const size_t po = (size_t)piece * p.px.all_rows + at;
-            const float inv = 1.0f / l;
-            float *dst = p.px.part_o + po * AT_HD;
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                uint32_t o[32];
-                tmem_ld32(tO + lane_base + c * 32, o);
-                tmem_ld_wait();
-                if (some)
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4 *>(dst + c * 32 + j) = make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
-                                                                                   __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
-            }
-            if (i < p.px.rows) p.px.part_l[po] = some ? m + log2f(l) : -INFINITY;
-        }
-        if (!PX && ok) {
+        if (ok) {
             tc_fence_after();
             const float inv = 1.0f / l;
             attn_store_row64(p.O + ((size_t)b * p.T + i) * ((size_t)p.H * AT_HD) + (size_t)h * AT_HD, tO + lane_base, i < p.T, inv);
@@ -995,37 +927,10 @@ extern "C" int qlmb_attn_fwd(void *O, float *lse, const void *Q, const void *K, 
     QLMB_CUDA(cudaGetDevice(&dev_));
     QLMB_REQUIRE(dev_ >= 0 && dev_ < 64, "device index %d", dev_);
     if (!configured_dev[dev_]) {
-        QLMB_CUDA(cudaFuncSetAttribute(k_attn_fwd<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_FWD_SMEM));
+        QLMB_CUDA(cudaFuncSetAttribute(k_attn_fwd, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_FWD_SMEM));
         configured_dev[dev_] = true;
     }
-    QLMB_CUDA(pdl_launch_small(k_attn_fwd<false>, dim3((unsigned)(p.nqt * B * H)), dim3(AT_FWD_THREADS), AT_FWD_SMEM, as_stream(stream), p));
-    QLMB_LAUNCH_CHECK("k_attn_fwd");
-    return QLMB_OK;
-}
-
-int qlmb::attn_prefix_launch(const PrefixAttn &px, const void *Kp, const void *Vp, int P, int H, int KV, cudaStream_t st)
-{
-    AttnFwdParams p;
-    memset(&p, 0, sizeof p);
-    const unsigned long long w = (unsigned long long)KV * AT_HD;
-    int rc = make_map(&p.k_map, Kp, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, w, (unsigned long long)P, w * 2, AT_HD, AT_BN, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-    rc = make_map(&p.v_map, Vp, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, w, (unsigned long long)P, w * 2, AT_HD, AT_BN, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-    p.px = px;
-    p.B = 1; p.T = P; p.H = H; p.KV = KV;
-    p.nqt = (px.rows + AT_BM - 1) / AT_BM;
-    p.scale_log2 = 1.4426950408889634f / sqrtf((float)AT_HD);
-    p.errword = device_error_word();
-    static bool configured_dev[64];
-    int dev_ = 0;
-    QLMB_CUDA(cudaGetDevice(&dev_));
-    QLMB_REQUIRE(dev_ >= 0 && dev_ < 64, "device index %d", dev_);
-    if (!configured_dev[dev_]) {
-        QLMB_CUDA(cudaFuncSetAttribute(k_attn_fwd<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_FWD_SMEM));
-        configured_dev[dev_] = true;
-    }
-    QLMB_CUDA(pdl_launch_small(k_attn_fwd<true>, dim3((unsigned)(p.nqt * px.pieces * KV)), dim3(AT_FWD_THREADS), AT_FWD_SMEM, st, p));
+    QLMB_CUDA(pdl_launch_small(k_attn_fwd, dim3((unsigned)(p.nqt * B * H)), dim3(AT_FWD_THREADS), AT_FWD_SMEM, as_stream(stream), p));
     QLMB_LAUNCH_CHECK("k_attn_fwd");
     return QLMB_OK;
 }

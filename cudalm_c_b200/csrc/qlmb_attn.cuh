@@ -1,4 +1,4 @@
-// Shared by the attention kernels (qlmb_attn.cu, qlmb_prefix.cu): their bounded wait and 2^x.
+// Shared by the attention kernels (qlmb_attn.cu, qlmb_prefix.cu): their bounded wait, 2^x, two-wide fp32.
 #pragma once
 #include "qlmb_tc.cuh"
 
@@ -51,5 +51,16 @@ __device__ __forceinline__ float ex2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two floats in one 64-bit register: sm_100's two-wide multiply-add and add
+__device__ __forceinline__ uint64_t f2_packu(uint32_t a, uint32_t b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) { return f2_packu(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void f2_unpack(uint64_t v, float &a, float &b)
+{
+    uint32_t x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(v));
+    a = __uint_as_float(x); b = __uint_as_float(y);
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
 }  // namespace qlmb

@@ -70,15 +70,6 @@ int count_assign(int *counts, const int *assign, int KN, int E, cudaStream_t st)
 // fp32 <-> bf16 row conversion helpers
 int convert_f32_to_bf16(bf16 *dst, const float *src, size_t n, cudaStream_t st);
 
-// ---- attention of a decode step over the rows its slots share (qlmb_attn.cu, from qlmb_prefix.cu) ----
-struct PrefixAttn {
-    const bf16 *Q;                            // rows of 64: [B*n][H]
-    float *part_o, *part_l;                   // [pieces][all_rows][64], [pieces][all_rows]; all_rows = B*n*H
-    size_t all_rows;
-    int rows, pieces, per;                    // rows of a kv head (B*n*H/KV); pieces of `per` tiles of 128 keys, none of them empty
-};
-int attn_prefix_launch(const PrefixAttn &px, const void *Kp, const void *Vp, int P, int H, int KV, cudaStream_t st);
-
 // ---- tensor-core GEMMs (qlmb_gemm.cu) ----
 struct GemmProblem;   // see qlmb_gemm.cuh
 

@@ -7,7 +7,6 @@
 #include <cuda_bf16.h>
 #include <math.h>
 #include <string.h>
-#include <stdlib.h>
 #include "qlmb_common.cuh"
 #include "qlmb_gemm.cuh"
 #include "qlmb_attn.cuh"
@@ -70,8 +69,15 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 // items' borders, and leaves of each item that it meets a segment: output in fp32, normalised, and the logarithm (base 2) of its
 // sum.  Segment number = item + warp, which no two share.  k_px_join adds the segments of a row up.
 //
-// With many rows a kv head the shared keys are k_attn_fwd's (qlmb_attn.cu: 128 rows a tile on tcgen05), in pieces of their own.
+// Many blocks of shared keys go through k_px_tc instead, in pieces (128 rows a tile, tcgen05), and only the slots' own through
+// k_px_mma: see px_plan.
+//
+// Measured (12 heads, 12 kv heads unless stated; graph of calls, all launches): 1 slot after 512 keys 9.2 us, 8 slots of 4 tokens after
+// 2048 10.9 us (both the length of three small launches), 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
+// 16 heads of 4 kv heads after 32768 95 us.  In the last k_px_tc has 75 us, 43 G scores at 0.57 T/s: without exponentials 60 us,
+// without any softmax 41 us, which is what its MMAs of 64 columns take by themselves.
 constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
+constexpr uint32_t PX_TRIES = 1u << 20;                   // a wait gives up after so many tries
 constexpr int PX_MAXB = 1024;                             // slots: every CTA keeps their positions and block counts
 struct PxParams {
     alignas(64) CUtensorMap kc_map, vc_map, kp_map, vp_map;
@@ -80,10 +86,10 @@ struct PxParams {
     const bf16 *Q;
     const int *pos;
     float *seg_o, *seg_l;                     // [items + warps][16][64] and [items + warps][16]
-    float *part_o, *part_l;                   // the shared keys' pieces of k_attn_fwd: [Sp][B*n*H][64] and [Sp][B*n*H]
+    float *part_o, *part_l;                   // the shared keys' pieces of k_px_tc: [Sp][B*n*H][64] and [Sp][B*n*H]
     int *table;                               // for the join: blocks ahead of each slot's items [B + 1], then of a shared item, then a warp's
     int B, n, P, Tm, H, KV, G, win;
-    int Sp, t_own, t_pre, warps, least;       // least: blocks of a warp at least; pieces of k_attn_fwd (0: the shared keys are items); tiles a (slot, kv head) / a kv head
+    int Sp, t_own, t_pre, warps, least;       // pieces of k_px_tc (0: the shared keys are items); tiles a (slot, kv head) / a kv head; blocks of a warp at least
     float scale_log2;                         // log2(e) / sqrt(64)
     int *errword;
 };
@@ -116,6 +122,22 @@ __device__ __forceinline__ int px_blocks(const PxParams &p, long long t0)
     if (!px_slot_ok(t0, p.n, p.P, p.Tm)) return 0;
     const int hi = (int)t0 + p.n - 1 - p.P;
     return hi < 0 ? 0 : (hi - px_first(p, (int)t0)) / 32 + 1;
+}
+// A warp's wait: all of its lanes go on (0), or none (the site).  Bounded like the library's other waits.  try_wait lets the hardware
+// hold the warp until the phase ends or a time of its own is over: a loop of test_wait instead keeps the queue busy that the
+// exponentials go through, too.
+__device__ __forceinline__ int px_all_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int site)
+{
+#pragma unroll 1
+    for (uint32_t i = 0; !__all_sync(~0u, mbar_try(bar, parity)); i++)
+        if ((i & 255u) == 255u && (*abort_flag || i > PX_TRIES)) return site;
+    return 0;
+}
+__device__ __forceinline__ void px_give_up(int site, volatile int *abort_flag, int *errword)
+{
+    if (!site || *abort_flag) return;
+    *abort_flag = 1;
+    if (errword && atomicCAS(errword, 0, 200) == 0) { errword[1] = site; errword[2] = (int)blockIdx.x; }
 }
 // x / d for 0 <= x < 2^24: the quotient of the floats is off by one at most (a division of integers takes ten times as long)
 __device__ __forceinline__ int px_div(int x, int d)
@@ -266,10 +288,11 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
     uint32_t qa[4][4];
     float oc[8][4], m[2], l[2];
     bool begin = true;
+    int bad = 0;
     uint32_t phase = 0;
     for (; count > 0; count--) {
         px_wait<0>();
-        if (!__all_sync(~0u, at_wait(smem_u32(bar + stage), phase, abort_flag, p.errword, 131))) break;
+        if ((bad = px_all_wait(smem_u32(bar + stage), phase, abort_flag, 131))) break;
         __syncwarp();
         const uint32_t sk = ring + stage * PX_STAGE, sv = sk + PX_BLK;
         phase ^= stage;
@@ -420,16 +443,244 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
         }
     }
     px_wait<0>();
+    px_give_up(bad, abort_flag, p.errword);
     if (*abort_flag)                                      // aborting: the copies under way must land before the CTA gives its shared memory back
         for (int i = 0; i < 2; i++)
             for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(bar + i), i < stage ? phase ^ 1u : phase); k++) {}
 }
 
-// A warp per row of O: its segments and pieces weighted by 2^(their logarithm - the largest), in a fixed order.
-__global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParams p)
+// ------------------------------------------------------------------ the shared keys of many rows
+// One CTA of 160 threads per (kv head, 128 rows, piece of the keys), three on an SM:
+//
+//   warp 0      one thread: K and V in steps of 64 keys through a three-stage TMA ring, S = Q K^T (128 x 64 x 64) and O += P V
+//               (128 x 64 x 64) with tcgen05.mma
+//   warps 1-4   softmax: a thread per row holds the 64 scores in registers, running maximum and sum in the exp2 domain, P as bf16
+//               over the scores in tensor memory, O rescaled there when a row of the warp has a new maximum
+//
+// Every row sees every key, so there is no mask but at the end.  Scores and O take 128 columns of tensor memory and 64 scores
+// 64 registers, so three CTAs share an SM: their phases wait on one another strictly (scores, weights, O), and the other two
+// have the tensor core and the special-function unit meanwhile.  64 slots of 5 tokens, 16 heads, 4 kv heads, 32768 keys: 75.1 us; two
+// CTAs an SM with the scores twice in tensor memory, so that a CTA's own phases overlap: 75.1 us; one CTA with two such tiles that
+// take turns: 84.2 us.
+constexpr int PT_M = 128, PT_N = 64, PT_NS = 3, PT_T = 160;
+constexpr int PT_Q = PT_M * 128, PT_KV = PT_N * 128;      // bytes of the queries and of a step's keys (its values follow)
+constexpr int PT_SMEM = PT_Q + PT_NS * 2 * PT_KV + 128;
+struct PxTcParams {
+    alignas(64) CUtensorMap k_map, v_map;
+    const bf16 *Q;
+    float *part_o, *part_l;                   // [pieces][B*n*H][64], [pieces][B*n*H]
+    size_t all_rows;
+    int rows, pieces, per, tiles, P, H, G;    // rows of a kv head; pieces of `per` steps, none of them empty; tiles of rows
+    float scale_log2;
+    int *errword;
+};
+
+__global__ void __launch_bounds__(PT_T, 3) k_px_tc(const __grid_constant__ PxTcParams p)
 {
-    const int lane = threadIdx.x & 31;
-    const size_t rows = (size_t)p.B * p.n * p.H, at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    extern __shared__ __align__(1024) uint8_t pt_s[];
+    uint8_t *sQ = pt_s, *sKV = pt_s + PT_Q;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sKV + PT_NS * 2 * PT_KV);
+    uint64_t *q_full = bars, *s_full = bars + 1, *p_full = bars + 2, *o_full = bars + 3, *spare = bars + 4, *kv_full = bars + 5;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(kv_full + PT_NS);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (smem_u32(pt_s) & 1023u) {             // the swizzled tiles need a 1 KiB-aligned base
+        if (threadIdx.x == 0 && p.errword && atomicCAS(p.errword, 0, 201) == 0) { p.errword[1] = 140; p.errword[2] = (int)blockIdx.x; }
+        pdl_wait();
+        return;
+    }
+    if (threadIdx.x == 0) {
+        prefetch_map(&p.k_map); prefetch_map(&p.v_map);
+        mbar_init(smem_u32(q_full), 4);
+        mbar_init(smem_u32(s_full), 1);
+        mbar_init(smem_u32(p_full), 4);
+        mbar_init(smem_u32(o_full), 1);
+        mbar_init(smem_u32(spare), 1);
+        for (int i = 0; i < PT_NS; i++) mbar_init(smem_u32(&kv_full[i]), 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), 128); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_wait();                               // barriers and TMEM above are this kernel's own; its inputs come below
+    pdl_trigger();
+    const uint32_t tS = *tmem_slot, tO = tS + 64;
+
+    // the row tiles of a piece, which read the same keys, side by side
+    const int tile = (int)blockIdx.x % p.tiles, piece = (int)blockIdx.x / p.tiles % p.pieces, kvh = (int)blockIdx.x / p.tiles / p.pieces;
+    const int t0 = piece * p.per, nt = min(p.per, (p.P + PT_N - 1) / PT_N - t0);
+
+    if (warp == 0) {
+        constexpr uint32_t IDESC_S = make_idesc(PT_M, PT_N, 0, 0), IDESC_PV = make_idesc(PT_M, PX_HD, 0, 1);
+        int issued = 0;
+        const auto load = [&](int t) {
+            if (t < nt) {
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&kv_full[t % PT_NS]), d = smem_u32(sKV + (t % PT_NS) * 2 * PT_KV);
+                    mbar_expect_tx(bar, 2 * PT_KV);
+                    tma_load_2d(d, &p.k_map, bar, kvh * PX_HD, (t0 + t) * PT_N);
+                    tma_load_2d(d + PT_KV, &p.v_map, bar, kvh * PX_HD, (t0 + t) * PT_N);
+                }
+                __syncwarp();
+                issued = t + 1;
+            }
+        };
+        for (int t = 0; t < PT_NS; t++) load(t);
+        // descriptors: an address is in their low bits, in units of 16 bytes
+        const uint64_t q0 = make_desc(smem_u32(sQ), 16, 1024), k00 = make_desc(smem_u32(sKV), 16, 1024), v00 = make_desc(smem_u32(sKV) + PT_KV, 8192, 1024);
+        int st = 0, bad = px_all_wait(smem_u32(q_full), 0, abort_flag, 141);
+        uint32_t kv_phase = 0;
+        for (int t = 0; !bad && t < nt; t++) {
+            if ((bad = px_all_wait(smem_u32(&kv_full[st]), kv_phase, abort_flag, 142))) break;
+            // P V of the last step has read the weights, over which the scores go, and its stage
+            if (t > 0 && (bad = px_all_wait(smem_u32(o_full), (uint32_t)(t - 1) & 1u, abort_flag, 143))) break;
+            tc_fence_after();
+            const uint64_t k0 = k00 + (uint64_t)(st * (2 * PT_KV / 16)), v0 = v00 + (uint64_t)(st * (2 * PT_KV / 16));
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < PX_HD / 16; k++) tc_mma_bf16(tS, q0 + 2 * k, k0 + 2 * k, IDESC_S, k > 0);
+                tc_commit(smem_u32(s_full));
+            }
+            __syncwarp();
+            if (++st == PT_NS) { st = 0; kv_phase ^= 1; }
+            if (t > 0) load(t - 1 + PT_NS);
+            if ((bad = px_all_wait(smem_u32(p_full), (uint32_t)t & 1u, abort_flag, 144))) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < PT_N / 16; k++)
+                    tc_mma_bf16_ta(tO, tS + k * 8, v0 + 128 * k, IDESC_PV, (t > 0 || k > 0) ? 1u : 0u);
+                tc_commit(smem_u32(o_full));
+            }
+            __syncwarp();
+        }
+        px_give_up(bad, abort_flag, p.errword);
+        if (*abort_flag) {                    // copies and MMAs under way end (bounded) before memory is given back
+            for (int i = issued > PT_NS ? issued - PT_NS : 0; i < issued; i++)
+                for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(&kv_full[i % PT_NS]), (uint32_t)(i / PT_NS) & 1u); k++) {}
+            if (elect_one()) tc_commit(smem_u32(spare));
+            __syncwarp();
+            for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(spare), 0); k++) {}
+        }
+    } else {
+        // a warp reaches the 32 lanes of tensor memory that its place in the warpgroup gives it
+        const int q = warp & 3, r = q * 32 + lane, i = tile * PT_M + r;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const bool live = i < p.rows, warp_live = tile * PT_M + q * 32 < p.rows;       // rows behind the last are neither computed nor stored
+        const int token = px_div(min(i, p.rows - 1), p.G);
+        const size_t at = (size_t)token * p.H + (size_t)kvh * p.G + (min(i, p.rows - 1) - token * p.G);       // the row's place in O / 64
+        if (warp_live) {
+            // the row into the 128-byte swizzle
+            const uint4 *src = reinterpret_cast<const uint4 *>(p.Q + at * PX_HD);
+            uint4 x[8];
+#pragma unroll
+            for (int c = 0; c < 8; c++) x[c] = src[c];
+#pragma unroll
+            for (int c = 0; c < 8; c++) *reinterpret_cast<uint4 *>(sQ + r * 128 + ((c ^ (r & 7)) << 4)) = live ? x[c] : make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(q_full));
+        const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+        float m = -3e38f, l = 0.0f;
+        int bad = 0;
+        for (int t = 0; t < nt; t++) {
+            if ((bad = px_all_wait(smem_u32(s_full), (uint32_t)t & 1u, abort_flag, 145))) break;
+            if (warp_live) {
+                tc_fence_after();
+                uint32_t v[64];
+                tmem_ld32(tS + lanes, v);
+                tmem_ld32(tS + lanes + 32, v + 32);
+                tmem_ld_wait();
+                const int left = p.P - (t0 + t) * PT_N;
+                if (left < PT_N) {
+#pragma unroll
+                    for (int j = 0; j < PT_N; j++) v[j] = j < left ? v[j] : 0xff800000u;
+                }
+                float mm[8];                            // eight chains: a step of one takes its instruction's latency
+#pragma unroll
+                for (int j = 0; j < 8; j++) mm[j] = fmaxf(__uint_as_float(v[j]), __uint_as_float(v[j + 8]));
+#pragma unroll
+                for (int j = 16; j < PT_N; j += 16)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) mm[e] = fmaxf(fmaxf(mm[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 8 + e]));
+                mm[0] = fmaxf(fmaxf(mm[0], mm[1]), mm[2]); mm[3] = fmaxf(fmaxf(mm[3], mm[4]), mm[5]);
+                const float mx = fmaxf(fmaxf(mm[0], mm[3]), fmaxf(mm[6], mm[7])) * p.scale_log2;
+                // A maximum that has grown by more than 2^8: O, to which nothing is being added now, is rescaled.  (Below that the weights
+                // stay under 2^8, their rounding to bf16 is as large a part of them, and sums stay far from fp32's limits.)
+                if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
+                    const float mn = fmaxf(m, mx), corr = ex2(m - mn);
+                    m = mn;
+                    l *= corr;
+                    if (t > 0) {
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            uint32_t o[16];
+                            tmem_ld16(tO + lanes + c * 16, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                            tmem_st16(tO + lanes + c * 16, o);
+                        }
+                    }
+                }
+                const uint64_t negm2 = f2_pack(-m, -m);
+                uint64_t rs[4] = {0, 0, 0, 0};          // pairs of 0.0f
+                uint32_t pk[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    float x0, x1;
+                    f2_unpack(f2_fma(f2_packu(v[2 * j], v[2 * j + 1]), scale2, negm2), x0, x1);
+                    const float p0 = ex2(x0), p1 = ex2(x1);
+                    rs[j & 3] = f2_add(rs[j & 3], f2_pack(p0, p1));
+                    const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
+                    pk[j] = *reinterpret_cast<const uint32_t *>(&h2);
+                }
+                tmem_st32(tS + lanes, pk);
+                float r0, r1;
+                f2_unpack(f2_add(f2_add(rs[0], rs[1]), f2_add(rs[2], rs[3])), r0, r1);
+                l += r0 + r1;
+                tmem_st_wait();
+                tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(p_full));
+        }
+        if (!bad) bad = px_all_wait(smem_u32(o_full), (uint32_t)(nt - 1) & 1u, abort_flag, 146);
+        px_give_up(bad, abort_flag, p.errword);
+        if (!bad && warp_live) {
+            tc_fence_after();
+            const bool some = live && l != 0.0f;        // l = 0: every score -inf; the join does not read such a piece
+            const size_t po = (size_t)piece * p.all_rows + at;
+            const float inv = 1.0f / l;
+            float *dst = p.part_o + po * PX_HD;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t o[32];
+                tmem_ld32(tO + lanes + c * 32, o);
+                tmem_ld_wait();
+                if (some)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4 *>(dst + c * 32 + j) = make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
+                                                                                   __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
+            }
+            if (live) p.part_l[po] = some ? m + log2f(l) : -INFINITY;
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 0) { tc_fence_after(); tmem_dealloc(tS, 128); }
+}
+
+// NW warps per row of O: its segments and pieces weighted by 2^(their logarithm - the largest), in a fixed order.
+template <int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 32 * NW) k_px_join(const __grid_constant__ PxParams p)
+{
+    __shared__ float xs[NW == 1 ? 1 : NW][PX_HD + 1];
+    const int lane = threadIdx.x & 31, part = NW == 1 ? 0 : threadIdx.x >> 5;
+    const size_t rows = (size_t)p.B * p.n * p.H, at = NW == 1 ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     pdl_trigger();
     pdl_wait();
     if (at >= rows) return;
@@ -464,14 +715,14 @@ __global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParam
             }
         }
     };
-    fetch(0);
+    fetch(8 * part);
     for (int s = lane; s < S; s += 32) mx = fmaxf(mx, (s < s0 + s1 ? p.seg_l : p.part_l)[place(s)]);
 #pragma unroll
     for (int i = 16; i; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, i));
     const float mref = mx == -INFINITY ? 0.0f : mx;
     float sum = 0.0f, x[4] = {};
-    for (int k0 = 0; k0 < S; k0 += 8) {
-        if (k0) fetch(k0);
+    for (int k0 = 8 * part; k0 < S; k0 += 8 * NW) {
+        if (k0 != 8 * part) fetch(k0);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const float w = ex2(lg[k] - mref);
@@ -482,6 +733,21 @@ __global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParam
     sum += __shfl_xor_sync(~0u, sum, 16);
 #pragma unroll
     for (int k = 0; k < 4; k++) x[k] += __shfl_xor_sync(~0u, x[k], 16);
+    if (NW > 1) {
+        if (half == 0) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) xs[part][c4 + k] = x[k];
+            if (lane == 0) xs[part][PX_HD] = sum;
+        }
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int w = 1; w < NW; w++) {
+            sum += xs[w][PX_HD];
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] += xs[w][c4 + k];
+        }
+    }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (half == 0) {
         const __nv_bfloat162 a = __floats2bfloat162_rn(x[0] * inv, x[1] * inv), c = __floats2bfloat162_rn(x[2] * inv, x[3] * inv);
@@ -490,21 +756,23 @@ __global__ void __launch_bounds__(128) k_px_join(const __grid_constant__ PxParam
     if (p.lse && lane == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mref + log2f(sum)) * 0.6931471805599453f;
 }
 
-// What a call needs: tiles, items, warps, pieces of k_attn_fwd (Sp of `per` tiles of keys), bytes of the workspace's parts.
+// What a call needs: tiles, items, warps, pieces of k_px_tc (Sp of `per` steps of keys), bytes of the workspace's parts.
 struct PxPlan { int t_own, t_pre, warps, Sp, per; size_t seg_o, seg_l, part_o, part_l, table, bytes; };
 static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
 {
     PxPlan pl = {};
     const long long rows = (long long)B * n * (H / KV);
-    int lim = 64;
-    { const char *e = getenv("PX_LIM"); if (e) lim = atoi(e); }
-    const bool tc = P > 0 && rows > lim && win <= 0;
+    // k_px_tc is a launch more, and as long for 16 rows as for 128; k_px_mma's warps take a block of 16 rows and 32 keys at a time.
+    // Whole calls, k_px_mma alone and with k_px_tc, by blocks: 6144 (64 rows, 12 kv heads) 20.0 and 22.7 us, 10240 (320 rows, 4) 22.6
+    // and 26.8, 12800 (1280 rows, 4) 24.5 and 24.3, 12288 (64 rows, 12) 26.0 and 27.7, 20480 (320, 4) 35 and 29, 24576 (16 rows, 12) 58
+    // and 47, (32 rows, 12) 45 and 33, 49152 (one row, 12) 100 and 73.  k_px_tc has no window.
+    const bool tc = P > 0 && win <= 0 && KV * ((rows + 15) / 16) * ((P + 31) / 32) > 12288;
     pl.t_own = (n * (H / KV) + 15) / 16;
     pl.t_pre = P > 0 && !tc ? (int)((rows + 15) / 16) : 0;
     pl.warps = sm_count() * PX_WARPS;
     if (tc) {
-        const long long t = (P + 127) / 128, ctas = KV * ((rows + 127) / 128);
-        long long s = 2LL * sm_count() / ctas;
+        const long long t = (P + PT_N - 1) / PT_N, ctas = KV * ((rows + PT_M - 1) / PT_M);
+        long long s = 3LL * sm_count() / ctas;
         s = s < 1 ? 1 : s > t ? t : s;
         pl.per = (int)((t + s - 1) / s);
         pl.Sp = (int)((t + pl.per - 1) / pl.per);
@@ -562,6 +830,7 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     QLMB_REQUIRE(px_shape_ok(B, n, P, Tm, H, KV), "qlmb_dec_attn_prefix: bad shape B %d (up to %d) n %d P %d Tm %d H %d KV %d", B, PX_MAXB, n, P, Tm, H, KV);
     QLMB_REQUIRE((((uintptr_t)O | (uintptr_t)Q | (uintptr_t)Kp | (uintptr_t)Vp | (uintptr_t)Kc | (uintptr_t)Vc | (uintptr_t)ws) & 15) == 0,
                  "qlmb_dec_attn_prefix: rows, caches and workspace must be 16-byte aligned");
+    if (win >= P + Tm) win = 0;                                        // hides nothing
     const PxPlan pl = px_plan(B, n, P, Tm, H, KV, win);
     QLMB_REQUIRE(ws_bytes >= pl.bytes, "qlmb_dec_attn_prefix: a workspace of %zu bytes, %zu are needed", ws_bytes, pl.bytes);
     PxParams p;
@@ -582,28 +851,38 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     p.part_l = (float *)w; w += pl.part_l;
     p.table = (int *)w;
     p.B = B; p.n = n; p.P = P; p.Tm = Tm; p.H = H; p.KV = KV; p.G = H / KV;
-    p.win = win < (1 << 30) ? win : 0;                                 // such a window hides nothing
+    p.win = win;
     p.Sp = pl.Sp; p.t_own = pl.t_own; p.t_pre = pl.t_pre > 0 ? pl.t_pre : 1; p.warps = pl.warps; p.least = 2;
-    { const char *e = getenv("PX_LEAST"); if (e) p.least = atoi(e); }
     p.scale_log2 = 1.4426950408889634f * 0.125f;
     p.errword = device_error_word();
     cudaStream_t st = as_stream(stream);
-    if (pl.Sp) {
-        const PrefixAttn px = {p.Q, p.part_o, p.part_l, rows, (int)(rows / KV), pl.Sp, pl.per};
-        const int rc = attn_prefix_launch(px, Kp, Vp, P, H, KV, st);
-        if (rc) return rc;
-    }
     static bool configured_dev[64];                                    // the attribute belongs to a device's copy of the kernel
     int dev = 0;
     QLMB_CUDA(cudaGetDevice(&dev));
     QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
     if (!configured_dev[dev]) {
         QLMB_CUDA(cudaFuncSetAttribute(k_px_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)px_smem(PX_MAXB)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_px_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM));
         configured_dev[dev] = true;
+    }
+    if (pl.Sp) {
+        PxTcParams t;
+        memset(&t, 0, sizeof t);
+        int rc = make_map(&t.k_map, Kp, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, width, (unsigned long long)P, width * 2, PX_HD, PT_N, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (!rc) rc = make_map(&t.v_map, Vp, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, width, (unsigned long long)P, width * 2, PX_HD, PT_N, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc) return rc;
+        t.Q = p.Q; t.part_o = p.part_o; t.part_l = p.part_l; t.all_rows = rows;
+        t.rows = (int)(rows / KV); t.pieces = pl.Sp; t.per = pl.per; t.tiles = (t.rows + PT_M - 1) / PT_M;
+        t.P = P; t.H = H; t.G = p.G; t.scale_log2 = p.scale_log2; t.errword = p.errword;
+        QLMB_CUDA(pdl_launch(true, k_px_tc, dim3((unsigned)(t.tiles * t.pieces * KV)), dim3(PT_T), PT_SMEM, st, t));
+        QLMB_LAUNCH_CHECK("k_px_tc");
     }
     QLMB_CUDA(pdl_launch_small(k_px_mma, dim3((unsigned)(pl.warps / PX_WARPS)), dim3(32 * PX_WARPS), px_smem(B), st, p));
     QLMB_LAUNCH_CHECK("k_px_mma");
-    QLMB_CUDA(pdl_launch(true, k_px_join, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p));
+    // Eight warps a row where rows are few: one of a long prefix has a hundred segments.  Whole calls with one warp a row and with eight:
+    // 384 rows 16.6 and 11.0 us, 768 rows 33.4 and 31.8, 5120 rows 96 and 114.
+    if (rows <= 1024) QLMB_CUDA(pdl_launch(true, k_px_join<8>, dim3((unsigned)rows), dim3(256), 0, st, p));
+    else QLMB_CUDA(pdl_launch(true, k_px_join<1>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p));
     QLMB_LAUNCH_CHECK("k_px_join");
     return QLMB_OK;
 }

@@ -207,6 +207,9 @@ SHAPES = [
     (1, 1, 1, 1, 0, 1, 0), (1, 1, 1, 1, 1, 1, 0), (1, 1, 12, 12, 512, 64, 0), (2, 1, 4, 4, 31, 33, 0), (3, 1, 4, 2, 32, 32, 0), (5, 2, 6, 2, 127, 65, 0),
     (8, 4, 12, 12, 300, 200, 0), (2, 3, 8, 1, 129, 40, 0), (7, 5, 16, 4, 1000, 130, 0), (64, 1, 12, 12, 640, 96, 0), (33, 5, 8, 2, 515, 64, 0), (1, 64, 8, 2, 257, 80, 0),
     (2, 16, 32, 2, 60, 100, 0), (4, 1, 2, 2, 4097, 20, 0), (1, 1, 2, 2, 3, 5000, 0), (16, 8, 8, 8, 0, 300, 0), (70, 3, 4, 4, 200, 30, 0), (1, 5, 1, 1, 20000, 9, 0),
+    # shared keys of many rows (or very many of one) have a kernel of their own, joins of many rows and windows theirs
+    (16, 5, 16, 4, 5003, 40, 0), (13, 5, 8, 8, 9857, 20, 0), (1, 1, 12, 12, 33003, 20, 0), (3, 64, 8, 2, 16448, 80, 0), (64, 5, 16, 4, 1217, 50, 0), (16, 5, 16, 4, 5003, 40, 4000),
+    (300, 2, 4, 2, 40, 9, 0), (1024, 1, 2, 2, 40, 6, 0), (1024, 1, 1, 1, 13000, 3, 0),
     (3, 2, 4, 2, 100, 50, 1), (3, 4, 4, 2, 100, 50, 20), (6, 3, 2, 2, 400, 300, 128), (20, 5, 8, 2, 300, 64, 100), (2, 1, 2, 1, 64, 64, 2 ** 31 - 1), (9, 7, 3, 3, 5, 70, 33),
 ]
 
@@ -297,6 +300,39 @@ def test_attention_reports_a_slot_past_its_cache(cuda, bad):
     ok()
     for b in (0, 2):
         assert torch.equal(o[b * n:b * n + n], O[b * n:b * n + n]) and torch.equal(l[b * n:b * n + n], lse[b * n:b * n + n])
+
+
+@pytest.mark.gpu
+def test_attention_of_many_rows_at_its_borders(cuda):
+    """Long shared keys of many rows: a slot past its cache is left as it is, scores of some 10^3 with the largest in the last key or
+    the first, a shared value that is no number (seen by every row), a slot that sees nothing of its own."""
+    from cudalm_c_b200 import attn
+    from cudalm_c_b200._lib import calls, lib, stream_ptr
+    B, n, H, KV, P, Tm = 16, 5, 16, 4, 5003, 12
+    q, kp, vp, kc, vc = make_attn(B, n, H, KV, P, Tm, 18, cuda, spread=6.0)
+    kp[0] *= 2
+    kp[P - 1] *= 2
+    q[:n] = 0
+    pos = P + torch.arange(B, device=cuda, dtype=torch.int32) % (Tm - n) - 1
+    pos[3] = P + Tm - n + 1
+    O, lse = torch.full_like(q, 7.0), torch.full((B * n, H), 7.0, device=cuda)
+    nb = lib().qlmb_dec_attn_prefix_bytes(B, n, P, Tm, H, KV)
+    ws = torch.full((nb,), 255, dtype=torch.uint8, device=cuda)
+    run = lambda: calls.dec_attn_prefix(O, lse, q, kp, vp, kc, vc, pos, 0, B, n, P, Tm, H, KV, 64, ws, nb, stream_ptr())
+    run()
+    assert b"error code 201 (site 306" in ok(4)
+    assert bool((O[3 * n:4 * n] == 7).all()) and bool((lse[3 * n:4 * n] == 7).all())
+    pos[3] = P
+    run()
+    ok()
+    check_attn(O, lse, attn64(q, kp, vp, kc, vc, pos, H, 0))
+    vp[77, 5] = math.inf                                   # kv head 0, dimension 5
+    run()
+    ok()
+    o = O.float().view(B * n, KV, H // KV, HD)
+    assert not bool(torch.isfinite(o[:n, 0, :, 5]).any())  # (queries of 0: every weight is the same)
+    o[:, 0, :, 5] = 0                                      # elsewhere 0 * inf where the weight has gone to 0: no number, either
+    assert bool(torch.isfinite(o).all())
 
 
 @pytest.mark.gpu
@@ -546,6 +582,7 @@ LORA = [
     # M, K, N, R, adapters
     (1, 8, 8, 8, 1), (1, 768, 768, 8, 4), (3, 72, 136, 16, 2), (16, 64, 64, 64, 1), (17, 256, 512, 24, 5), (64, 768, 1536, 16, 64), (64, 1000, 200, 72, 7), (130, 512, 768, 256, 3),
     (333, 384, 264, 32, 10), (1000, 768, 768, 8, 40), (2, 4096, 16384, 16, 2), (70, 40, 1032, 40, 3),
+    (2049, 72, 136, 8, 3), (2500, 768, 264, 64, 9), (2300, 256, 520, 136, 5), (4097, 512, 768, 16, 200), (257, 1024, 128, 64, 3),
 ]
 
 
