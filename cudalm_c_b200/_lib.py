@@ -240,15 +240,6 @@ def need(name, t, dtype, *shape):
     return t
 
 
-def alike(dev, dtype, *tensors):
-    """Whether all of them are contiguous, of that type and on that CUDA device: a mirror's quick look at its arguments (need() takes
-    1.5 us each, this 0.2), with need() for the message where it fails."""
-    for t in tensors:
-        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
-            return False
-    return True
-
-
 class _Calls:
     """The hot entry points without their qlmb_ prefix as native calls (csrc/pycalls.c): tensors, addresses or None for
     pointers, a QlmbError for a status other than 0."""

@@ -2,7 +2,7 @@
 attention part of gpu_backward, cudalm.cu:5918-5960) over the C ABI."""
 import torch
 
-from ._lib import alike, calls, check, device_index, lib, need, ptr, stream_ptr
+from ._lib import calls, check, device_index, lib, need, ptr, stream_ptr
 
 
 def attn_fwd(Q, K, V, B, T, H, KV, win=0):
@@ -45,22 +45,16 @@ def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
     bf16, pos [B] int32 = absolute position of each slot's first new token (its cache row is pos - P).  Returns O [B*n, H*64] bf16 and
     the scores' log-sum-exp [B*n, H] fp32."""
     dev = device_index()
-    try:
-        B, Tm, KD = Kc.shape
-        rows, width = Q.shape
-        P, kd = Kp.shape
-        good = (alike(dev, torch.bfloat16, Q, Kp, Vp, Kc, Vc) and alike(dev, torch.int32, pos) and pos.shape == (B,) and Vc.shape == Kc.shape and
-                Vp.shape == Kp.shape and kd == KD and width == H * 64 and KD % 64 == 0 and B > 0 and rows % B == 0 and rows > 0)
-    except (AttributeError, ValueError):
-        good = False
-    if not good:
+    got = calls.sizes(dev, torch.bfloat16, Q, "rw", Kc, "btk", Vc, "btk", Kp, "pk", Vp, "pk", torch.int32, pos, "b")
+    if got is None or not (got[1] == H * 64 and got[4] % 64 == 0 and got[2] > 0 and got[0] > 0 and got[0] % got[2] == 0):
         _dec_attn_prefix_args(Q, Kp, Vp, Kc, Vc, pos, H)
+    rows, _, B, Tm, KD, P = got
     shape = (B, rows // B, P, Tm, H, KD // 64)
     nbytes = _prefix_ws.get((dev, shape))
     if nbytes is None:
         nbytes = _prefix_ws[(dev, shape)] = lib().qlmb_dec_attn_prefix_bytes(*shape)
     O = torch.empty_like(Q)
     lse = torch.empty((rows, H), dtype=torch.float32, device=Q.device)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device) if nbytes else None
+    ws = Q.new_empty(nbytes + 1 >> 1) if nbytes else None
     calls.dec_attn_prefix(O, lse, Q, Kp, Vp, Kc, Vc, pos, win, *shape, 64, ws, nbytes, stream_ptr())
     return O, lse

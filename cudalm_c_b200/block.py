@@ -2,7 +2,7 @@
 k_embed, k_embed_bwd, k_softmax_ce; cudalm.cu:3630-3645, 5740, 5838, 6000) over the C ABI."""
 import torch
 
-from ._lib import BF16, F32, alike, calls, check, device_index, lib, need, ptr, stream_ptr
+from ._lib import BF16, F32, calls, check, device_index, lib, need, ptr, stream_ptr
 
 
 def _dt(t):
@@ -151,19 +151,12 @@ def dec_rope_kv(q, k, v, Kc, Vc, cosb, sinb, pos, H, P=0, out=None):
     [B*n, KD], caches [B, Tm, KD] bf16 (row j is position P + j), tables [Tr, 32], pos [B] int32 = absolute position of each slot's
     first new token.  Returns the rotated q (out may be q)."""
     dev = device_index()
-    try:
-        B, Tm, KD = Kc.shape
-        rows, width = q.shape
-        Tr, half = cosb.shape
-        if out is None:
-            out = torch.empty_like(q)
-        good = (alike(dev, torch.bfloat16, q, k, v, Kc, Vc, out) and alike(dev, torch.float32, cosb, sinb) and alike(dev, torch.int32, pos) and
-                pos.shape == (B,) and Vc.shape == Kc.shape and k.shape == v.shape == (rows, KD) and out.shape == q.shape and
-                sinb.shape == cosb.shape and half == 32 and width == H * 64 and KD % 64 == 0 and B > 0 and rows % B == 0 and rows > 0)
-    except (AttributeError, ValueError, TypeError):
-        good = False
-    if not good:
+    if out is None and isinstance(q, torch.Tensor):
+        out = torch.empty_like(q)
+    got = calls.sizes(dev, torch.bfloat16, q, "rw", out, "rw", Kc, "btk", Vc, "btk", k, "rk", v, "rk", torch.float32, cosb, "x5", sinb, "x5", torch.int32, pos, "b")
+    if got is None or not (got[1] == H * 64 and got[4] % 64 == 0 and got[2] > 0 and got[0] > 0 and got[0] % got[2] == 0):
         _dec_rope_kv_args(q, k, v, Kc, Vc, cosb, sinb, pos, H, out)
+    rows, _, B, Tm, KD, Tr = got
     calls.dec_rope_kv(out, Kc, Vc, q, k, v, cosb, sinb, pos, B, rows // B, P, Tm, H, KD // 64, 64, Tr, stream_ptr())
     return out
 
@@ -186,24 +179,14 @@ def dec_verify(logits, draft, u, temp, q=None, nd=None, V=None):
     [B, n+1] uniform numbers, temp [B] (0: greedy), q [B, n, ldq] the probabilities the drafts were drawn from (None: certain), nd [B] int32
     drafts per slot (None: n).  Returns (tokens [B, n+1], -1 behind the last; how many [B]; log-probabilities [B, n+1])."""
     dev = device_index()
-    try:
-        B, n1, ld = logits.shape
-        n = n1 - 1
-        dt = logits.dtype
-        good = (B > 0 and (dt is torch.float32 or dt is torch.bfloat16) and alike(dev, dt, logits) and alike(dev, torch.float32, u, temp) and
-                alike(dev, torch.int32, draft) and draft.shape == (B, n) and u.shape == (B, n1) and temp.shape == (B,))
-        ldq = 0
-        if good and q is not None:
-            ldq = q.shape[2]
-            good = alike(dev, torch.float32, q) and q.shape == (B, n, ldq)
-        if good and nd is not None:
-            good = alike(dev, torch.int32, nd) and nd.shape == (B,)
-    except (AttributeError, ValueError, IndexError):
-        good = False
-    if not good:
+    dt = torch.bfloat16 if getattr(logits, "dtype", None) is torch.bfloat16 else torch.float32
+    got = calls.sizes(dev, dt, logits, "bml", torch.float32, u, "bm", temp, "b", torch.int32, draft, "bn", nd, "?b", torch.float32, q, "?bnq")
+    if got is None or not (got[0] > 0 and got[3] == got[1] - 1):
         _dec_verify_args(logits, draft, u, temp, q, nd, V)
-    out = torch.empty((B, n1), dtype=torch.int32, device=logits.device)
-    count = torch.empty_like(temp, dtype=torch.int32)
+    B, n1, ld, n = got[:4]
+    ldq = got[4] if q is not None else 0
+    out = draft.new_empty((B, n1))
+    count = draft.new_empty(B)
     lp = torch.empty_like(u)
     calls.dec_verify(out, count, lp, logits, F32 if dt is torch.float32 else BF16, ld, q if n else None, ldq, draft if n else None, nd, u, temp,
                      B, n, ld if V is None else V, stream_ptr())

@@ -6,7 +6,7 @@
 #include <Python.h>
 #include "../../include/qlm_b200.h"
 
-static PyObject *error_class, *name_data_ptr;
+static PyObject *error_class, *name_data_ptr, *name_dtype, *name_get_device, *name_is_contiguous, *name_shape;
 
 /* The converters run in the order of the arguments.  After the first that failed the others do nothing: no Python code
  * may run with an exception set, and the caller is to see that one. */
@@ -103,6 +103,69 @@ CALL(dec_verify, 16, ARG_P(0); ARG_P(1); ARG_P(2); ARG_P(3); ARG_I(4); ARG_U(5);
 CALL(lora_add, 17, ARG_P(0); ARG_P(1); ARG_P(2); ARG_I(3); ARG_P(4); ARG_P(5); ARG_P(6); ARG_I(7); ARG_P(8); ARG_P(9); ARG_I(10); ARG_I(11);
      ARG_I(12); ARG_I(13); ARG_P(14); ARG_U(15); ARG_P(16), p0, p1, p2, i3, p4, p5, p6, i7, p8, p9, i10, i11, i12, i13, p14, (size_t)u15, p16)
 
+/* A mirror's look at its arguments: sizes(device, dtype, tensor, "bn", tensor, "bk", dtype, tensor, "k", ...).  Each tensor is to be
+ * contiguous, of the dtype named last and on that CUDA device; a letter a dimension, and the same letter is the same size wherever it
+ * stands (a digit d in place of a letter: the size 2^d).  After a '?' the tensor may be None.  Returns the letters' sizes in the order of
+ * their first appearance, or None where the look failed: the mirror's slow checks then find words for it. */
+static PyObject *sizes(PyObject *self, PyObject *const *a, Py_ssize_t n)
+{
+    (void)self;
+    if (n < 1) { PyErr_SetString(PyExc_TypeError, "sizes takes a device first"); return NULL; }
+    const long dev = PyLong_AsLong(a[0]);
+    if (dev == -1 && PyErr_Occurred()) return NULL;
+    PyObject *dtype = NULL;
+    Py_ssize_t value[26];
+    int count = 0, known[26];
+    for (int i = 0; i < 26; i++) known[i] = -1;
+    for (Py_ssize_t i = 1; i < n;) {
+        if (i + 1 >= n || !PyUnicode_Check(a[i + 1])) { dtype = a[i++]; continue; }
+        PyObject *t = a[i];
+        Py_ssize_t dims;
+        const char *spec = PyUnicode_AsUTF8AndSize(a[i + 1], &dims);
+        if (!spec) return NULL;
+        i += 2;
+        if (dims && spec[0] == '?') {
+            if (t == Py_None) continue;
+            spec++; dims--;
+        }
+        PyObject *r = PyObject_GetAttr(t, name_dtype);
+        if (!r) goto failed;
+        const int same = r == dtype;
+        Py_DECREF(r);
+        if (!same) Py_RETURN_NONE;
+        if (!(r = PyObject_CallMethodNoArgs(t, name_get_device))) goto failed;
+        const long d = PyLong_AsLong(r);
+        Py_DECREF(r);
+        if (d != dev) goto failed;
+        if (!(r = PyObject_CallMethodNoArgs(t, name_is_contiguous))) goto failed;
+        const int flat = r == Py_True;
+        Py_DECREF(r);
+        if (!flat) Py_RETURN_NONE;
+        if (!(r = PyObject_GetAttr(t, name_shape))) goto failed;
+        int good = PyTuple_Check(r) && PyTuple_GET_SIZE(r) == dims;
+        for (Py_ssize_t k = 0; good && k < dims; k++) {
+            const Py_ssize_t v = PyLong_AsSsize_t(PyTuple_GET_ITEM(r, k));
+            const int c = spec[k] - 'a';
+            if (c >= 0 && c < 26) {
+                if (known[c] < 0) { known[c] = count; value[count++] = v; }
+                else good = value[known[c]] == v;
+            } else good = spec[k] >= '0' && spec[k] <= '9' && v == (Py_ssize_t)1 << (spec[k] - '0');
+        }
+        Py_DECREF(r);
+        if (!good) goto failed;
+    }
+    PyObject *out = PyTuple_New(count);
+    for (int i = 0; out && i < count; i++) {
+        PyObject *v = PyLong_FromSsize_t(value[i]);
+        if (!v) { Py_DECREF(out); return NULL; }
+        PyTuple_SET_ITEM(out, i, v);
+    }
+    return out;
+failed:
+    PyErr_Clear();                                        /* not a tensor: the slow checks say so */
+    Py_RETURN_NONE;
+}
+
 static PyObject *set_error_class(PyObject *self, PyObject *cls)
 {
     (void)self;
@@ -117,6 +180,7 @@ static PyMethodDef methods[] = {
     ENTRY(rmsnorm_bwd), ENTRY(rope), ENTRY(attn_fwd), ENTRY(attn_bwd), ENTRY(moe_forward), ENTRY(moe_decode), ENTRY(moe_backward), ENTRY(adamw),
     ENTRY(step), ENTRY(gnorm), ENTRY(dec_step), ENTRY(dec_greedy),
     ENTRY(dec_rope_kv), ENTRY(dec_attn_prefix), ENTRY(dec_verify), ENTRY(lora_add),
+    {"sizes", (PyCFunction)(void (*)(void))sizes, METH_FASTCALL, NULL},
     {"set_error_class", set_error_class, METH_O, NULL},
     {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycalls", NULL, -1, methods, NULL, NULL, NULL, NULL};
@@ -124,5 +188,9 @@ static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycalls", NULL, -1,
 PyMODINIT_FUNC PyInit__pycalls(void)
 {
     name_data_ptr = PyUnicode_InternFromString("data_ptr");
-    return name_data_ptr ? PyModule_Create(&module) : NULL;
+    name_dtype = PyUnicode_InternFromString("dtype");
+    name_get_device = PyUnicode_InternFromString("get_device");
+    name_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+    name_shape = PyUnicode_InternFromString("shape");
+    return name_data_ptr && name_dtype && name_get_device && name_is_contiguous && name_shape ? PyModule_Create(&module) : NULL;
 }

@@ -6,7 +6,7 @@ KN = codes of W[K,N] (the reference's own [in,out] storage, applied with g_ab),
 NK = codes of W[N,K] (applied with g_abt)."""
 import torch
 
-from ._lib import BF16, F32, KN, NK, Qkv, alike, calls, check, device_index, lib, need, ptr, stream_ptr  # noqa: F401
+from ._lib import BF16, F32, KN, NK, Qkv, calls, check, device_index, lib, need, ptr, stream_ptr  # noqa: F401
 
 
 def _dt(t):
@@ -100,26 +100,19 @@ def lora_add(X, base, A, Bm, scale, adapter, order=None, out=None):
     """base + scale[a] * (X A[a]^T) Bm[a] row by row, a = adapter[m] (-1: base): X [M, K], base [M, N] (fp32 or bf16), A [n, R, K] and Bm
     [n, R, N] bf16, scale [n] fp32, adapter [M] int32.  out may be base (not X)."""
     dev = device_index()
-    try:
-        dt = X.dtype
-        M, K = X.shape
-        n, R, N = Bm.shape
-        if out is None:
-            out = torch.empty_like(base)
-        good = ((dt is torch.bfloat16 or dt is torch.float32) and alike(dev, dt, X, base, out) and alike(dev, torch.bfloat16, A, Bm) and
-                alike(dev, torch.float32, scale) and alike(dev, torch.int32, adapter) and base.shape == out.shape == (M, N) and
-                A.shape == (n, R, K) and scale.shape == (n,) and adapter.shape == (M,) and
-                (order is None or (alike(dev, torch.int32, order) and order.shape == (M,))))
-    except (AttributeError, ValueError, TypeError):
-        good = False
-    if not good:
+    dt = torch.bfloat16 if getattr(X, "dtype", None) is torch.bfloat16 else torch.float32
+    if out is None and isinstance(base, torch.Tensor):
+        out = torch.empty_like(base)
+    got = calls.sizes(dev, dt, X, "mk", base, "mn", out, "mn", torch.bfloat16, A, "ark", Bm, "arn", torch.float32, scale, "a", torch.int32, adapter, "m", order, "?m")
+    if got is None:
         _lora_add_args(X, base, A, Bm, scale, adapter, order, out)
+    M, K, N, n, R = got
     if M == 0:
         return out
     shape = (M, K, N, R)
     nbytes = _lora_ws.get((dev, shape))
     if nbytes is None:
         nbytes = _lora_ws[(dev, shape)] = lib().qlmb_lora_bytes(*shape)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=X.device) if nbytes > 16 else None
+    ws = Bm.new_empty(nbytes + 1 >> 1) if nbytes > 16 else None
     calls.lora_add(out, X, base, F32 if dt is torch.float32 else BF16, A, Bm, scale, n, adapter, order, M, K, N, R, ws, nbytes, stream_ptr())
     return out

@@ -726,3 +726,19 @@ def test_two_graphs_and_two_streams(cuda):
         eager = _step(fresh)
     ok()
     assert all(torch.equal(a, b) for a, b in zip(outs[0], w)) and all(torch.equal(a, b) for a, b in zip(eager, w))
+
+
+def test_the_mirrors_look_at_their_arguments():
+    """calls.sizes: letters bind sizes, digits are powers of two, '?' may be None; whatever does not hold gives None."""
+    from cudalm_c_b200._lib import calls
+    f, i = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32)
+    look = lambda *a: calls.sizes(-1, torch.float32, *a)
+    assert look(f, "ab", None, "?xy", torch.int32, i, "a") == (4, 8) and look(f, "b3") == (4,) and look(None, "?a") == () and look(f[:0], "ab") == (0, 8)
+    for bad in ((f, "aa"), (f, "a"), (f, "abc"), (f.t(), "ab"), (f, "ab", f[:3], "ab"), (f, "a4"), (f.double(), "ab"), (3, "ab"), ([1.0], "a"), (None, "a"), (f, "a!"),
+                (torch.int32, f, "ab"), (f[:, ::2], "ab")):
+        assert look(*bad) is None, bad
+    assert calls.sizes(0, torch.float32, f, "ab") is None
+    with pytest.raises(TypeError):
+        calls.sizes()
+    with pytest.raises(TypeError):
+        calls.sizes("x", f, "ab")
