@@ -99,7 +99,7 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
     }
     const float temp = p.temp[b];
     const bool greedy = !(temp > 0.0f);
-    const double it = greedy ? 1.4426950408889634 : 1.4426950408889634 / (double)temp;
+    const double it = greedy ? 1.4426950408889634 : 1.4426950408889634 / fmin((double)temp, 1e30);      // an infinite one: every finite logit has the weight 1
     const float cT = (float)fmin(it, 1e38);
     const bool unit = cT == 1.4426950408889634f;          // the two sums are one
     // runs of whole groups of four

@@ -499,6 +499,25 @@ def test_verify_at_its_borders(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 40001])
+def test_verify_at_an_infinite_temperature(cuda, V):
+    """Every token that is not cut has the same probability; a temperature that is no number picks the arg-max, as 0 does."""
+    from cudalm_c_b200 import block
+    B, n = 4, 2
+    lg, x, u, temp, q = make_verify(B, n, V, V, torch.float32, False, 12, cuda)
+    temp[:] = torch.tensor([math.inf, math.inf, math.nan, 3e38], device=cuda)
+    lg[1, :, V // 2:] = -math.inf
+    x[1] = V // 2 + 1
+    x[2] = lg[2, :n].argmax(-1).int()
+    got = block.dec_verify(lg, x, u, temp)
+    ok()
+    assert got[1][1] == 1 and int(got[0][1, 0]) == int(u[1, n].double() * (V // 2)) and got[1][2] == n + 1
+    # finite logits: the oracle's own division by a large number is the same
+    keep = torch.tensor([0, 3], device=cuda)
+    check_verify(tuple(t[keep] for t in got), verify64(lg[keep], x[keep], u[keep], torch.full((2,), 1e30, device=cuda), None, None, V))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what,site", [("nan", 309), ("inf", 309), ("none", 309), ("token", 308), ("negative", 308), ("count", 310)])
 def test_verify_reports_what_it_cannot_use(cuda, what, site):
     from cudalm_c_b200 import block
