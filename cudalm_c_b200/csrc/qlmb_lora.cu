@@ -16,7 +16,7 @@
 namespace qlmb {
 
 constexpr int LR_RT = 64;                     // inner columns made at a time
-constexpr int LR_UP = 512;                    // output columns of a CTA of k_lora_up
+constexpr int LR_UP = 512;                    // output columns of a CTA of k_lora_one
 
 struct LoraParams {
     void *Y;
@@ -44,14 +44,23 @@ template <int TERMS> __device__ __forceinline__ void lr_split(float x, float y, 
         x -= __uint_as_float(t[k] << 16); y -= __uint_as_float(t[k] & 0xffff0000u);
     }
 }
+__device__ __forceinline__ uint32_t lt_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void lt_copy(uint32_t dst, const void *src, bool in)      // 16 bytes, zeros where !in
+{ asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); }
+__device__ __forceinline__ void lt_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void lt_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Loads that stay where they are written and pass by L1: k_lora_up reads ahead of its wait.
+__device__ __forceinline__ int lr_ldcg(const int *p) { int v; asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory"); return v; }
+__device__ __forceinline__ uint4 lr_ldcg(const uint4 *p)
+{ uint4 v; asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory"); return v; }
 // Row of place j (of the tile order) and its adapter; -1, -1 behind the last row or for an index out of range, which is reported.
 __device__ __forceinline__ void lr_row(const LoraParams &p, int j, int &m, int &a, bool report)
 {
     m = a = -1;
     if (j >= p.M) return;
-    m = p.order ? p.order[j] : j;
+    m = p.order ? lr_ldcg(p.order + j) : j;
     if (m < 0 || m >= p.M) { if (report) report_bad_index(p.errword, 307, j, m); m = -1; return; }
-    a = p.adapter[m];
+    a = lr_ldcg(p.adapter + m);
     if (a < -1 || a >= p.adapters) { if (report) report_bad_index(p.errword, 307, m, a); a = -1; }
 }
 
@@ -115,14 +124,17 @@ __device__ __forceinline__ void lr_down(const LoraParams &p, float (&c)[NT][4], 
 }
 
 // Columns n0 .. n0 + 63 of 16 rows: base + T B.  A thread asks for B's rows r0 + 2 q, + 1, + 8, + 9, columns n0 + 8 g .. n0 + 8 g + 7.
-__device__ __forceinline__ void lr_up_b(const LoraParams &p, int cur, int n0, int r0, uint4 (&b)[4])
+template <bool CG> __device__ __forceinline__ void lr_up_b(const LoraParams &p, int cur, int n0, int r0, uint4 (&b)[4])
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         const int r = r0 + 2 * q + (w & 1) + 8 * (w >> 1), n = n0 + 8 * g;
         b[w] = make_uint4(0, 0, 0, 0);
-        if (cur >= 0 && n < p.N && r < p.R) b[w] = *reinterpret_cast<const uint4 *>(p.Bm + ((size_t)cur * p.R + r) * p.N + n);
+        if (cur >= 0 && n < p.N && r < p.R) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(p.Bm + ((size_t)cur * p.R + r) * p.N + n);
+            b[w] = CG ? lr_ldcg(src) : *src;
+        }
     }
 }
 // T as bf16 terms in shared memory: [term][row][ldt] pairs, t0 = the pairs of row g
@@ -193,21 +205,14 @@ template <bool F32> __device__ __forceinline__ void lr_up_store(const LoraParams
         }
     }
 }
-template <bool F32>
-__device__ __forceinline__ void lr_up(const LoraParams &p, const uint32_t *t0, int ldt, int cur, int n0, const int (&mrow)[2], const bool (&keep)[2])
+template <bool F32> __device__ __forceinline__ void lr_up(const LoraParams &p, float (&c)[8][4], const uint32_t *t0, int ldt, int cur, int n0)
 {
-    uint4 base[2][2][F32 ? 2 : 1];
-    lr_up_base<F32>(p, base, n0, mrow, keep);
-    float c[8][4] = {};
-    if (cur >= 0) {
 #pragma unroll 2
-        for (int r0 = 0; r0 < p.R; r0 += 16) {
-            uint4 b[4];
-            lr_up_b(p, cur, n0, r0, b);
-            lr_up_mul<F32>(p, c, b, t0, ldt, r0);
-        }
+    for (int r0 = 0; r0 < p.R; r0 += 16) {
+        uint4 b[4];
+        lr_up_b<false>(p, cur, n0, r0, b);
+        lr_up_mul<F32>(p, c, b, t0, ldt, r0);
     }
-    lr_up_store<F32>(p, c, base, cur, n0, mrow, keep);
 }
 
 // ---- many rows.  A CTA of eight warps (four row groups of 16 times two halves of 32 columns) has 64 rows: the products' operands come
@@ -218,11 +223,6 @@ constexpr int LT_M = 64, LT_NS = 4, LT_W = 64 * 64 * 2;      // rows, stages, by
 template <bool F32> constexpr int lt_x() { return LT_M * 64 * (F32 ? 4 : 2); }
 template <bool F32> static size_t lt_smem(int R) { return (size_t)LT_NS * (lt_x<F32>() + LT_W) + (size_t)(F32 ? 3 : 2) * LT_M * ((R + 15) / 16 * 8 + 4) * sizeof(uint32_t); }
 
-__device__ __forceinline__ uint32_t lt_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void lt_copy(uint32_t dst, const void *src, bool in)      // 16 bytes, zeros where !in
-{ asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); }
-__device__ __forceinline__ void lt_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void lt_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void lt_ldm(uint32_t a, uint32_t v[4])
 { asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory"); }
 __device__ __forceinline__ void lt_ldmt(uint32_t a, uint32_t v[4])
@@ -486,7 +486,13 @@ template <bool F32, int NT, int UK> __global__ void __launch_bounds__(256) k_lor
         __syncthreads();
     }
     const int n1 = min(p.N, ((int)blockIdx.y + 1) * LR_UP);
-    for (int n0 = blockIdx.y * LR_UP + 64 * warp; n0 < n1; n0 += 512) lr_up<F32>(p, ts + g * ldt, ldt, cur, n0, rows, keep);
+    for (int n0 = blockIdx.y * LR_UP + 64 * warp; n0 < n1; n0 += 512) {
+        uint4 base[2][2][F32 ? 2 : 1];
+        lr_up_base<F32>(p, base, n0, rows, keep);
+        float c[8][4] = {};
+        if (cur >= 0) lr_up<F32>(p, c, ts + g * ldt, ldt, cur, n0);
+        lr_up_store<F32>(p, c, base, cur, n0, rows, keep);
+    }
 }
 
 // ---- few rows, large adapters: two launches, CTAs of places again; first the inner numbers in slices of K, then blocks of columns.
@@ -494,11 +500,11 @@ template <bool F32, int NT, int UK> __global__ void __launch_bounds__(128) k_lor
 {
     __shared__ float red[4][16][8 * NT + 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    pdl_wait();                               // ahead of the trigger: what ran before has ended when k_lora_up starts
     pdl_trigger();
-    pdl_wait();
     const int j0 = (int)blockIdx.x / 16 * 16, place = blockIdx.x % 16, r0 = blockIdx.z * (8 * NT), k0 = blockIdx.y * p.kslice, k1 = min(p.K, k0 + p.kslice);
     int m, a;
-    lr_row(p, j0 + (lane & 15), m, a, false);
+    lr_row(p, j0 + (lane & 15), m, a, blockIdx.y == 0 && blockIdx.z == 0 && place == 0 && threadIdx.x < 16);
     const int cur = __shfl_sync(~0u, a, place);
     const unsigned mine = __ballot_sync(~0u, a == cur) & 0xffffu;
     if (cur < 0 || __ffs(mine) - 1 != place) return;
@@ -517,72 +523,225 @@ template <bool F32, int NT, int UK> __global__ void __launch_bounds__(128) k_lor
             p.part[((size_t)blockIdx.y * p.M + j0 + r) * p.R + r0 + col] = (red[0][r][col] + red[1][r][col]) + (red[2][r][col] + red[3][r][col]);
     }
 }
-// AHEAD (R <= 16): a warp's four blocks of 64 columns of B are requested before anything is multiplied.
-template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, AHEAD ? 4 : 3) k_lora_up(const __grid_constant__ LoraParams p)
+// k_lora_up starts while k_lora_down runs and requests what that does not write ahead of its wait: the rows' places, their base and
+// B.  A place with one or two rows is multiplied by plain instructions, a lane having LC neighbouring columns: on tensor cores 14 or
+// 15 rows of 16 would be nobody's, and the instructions around them bound it (64 rows on 64 adapters, K 4096, N 16384, R 16: 14.8 us
+// instead of 16.2).  One with more goes through the tensor cores, the base in shared memory, and (AHEAD, R <= 16) B for all of a warp's
+// blocks of 64 columns requested first.  Now 17.3 us both launches (k_lora_down 8.7, k_lora_up 11.4 by themselves; 46 MB, 2.7 TB/s); a
+// CTA a place and 1024 columns, which was two waves, 20.4; rings of copies a warp or a CTA with tensor cores only 24.7 and 27.3.
+constexpr int LR_FEW = 2;
+template <bool F32, bool AHEAD> constexpr int lr_cols() { return AHEAD && !F32 ? 1024 : 512; }        // columns of a CTA
+template <bool F32, bool AHEAD> constexpr int lr_pitch() { return lr_cols<F32, AHEAD>() * (F32 ? 4 : 2) + 16; }       // bytes of a row of the base
+template <bool F32, bool AHEAD> static size_t lr_smem(int R) { return 16 * (size_t)lr_pitch<F32, AHEAD>() + (size_t)(F32 ? 3 : 2) * 16 * ((R + 15) / 16 * 8 + 4) * sizeof(uint32_t); }
+
+// A lane's LC columns of bf16 (LC = 8 or 4) as they lie, and of the rows
+template <int LC> struct LrVec { uint32_t w[LC / 2]; };
+template <int LC> __device__ __forceinline__ LrVec<LC> lr_ldv(const bf16 *p)
 {
-    constexpr int TT = F32 ? 3 : 2, UP = AHEAD ? 1024 : LR_UP;
-    extern __shared__ __align__(16) uint32_t lr_t[];     // [term][16][ldt] pairs of bf16
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, ldt = (p.R + 15) / 16 * 8 + 4;
-    pdl_trigger();
-    pdl_wait();
-    const int j0 = (int)blockIdx.x / 16 * 16, place = blockIdx.x % 16;
-    int m, a;
-    lr_row(p, j0 + (lane & 15), m, a, blockIdx.y == 0 && place == 0 && threadIdx.x < 16);
-    const int cur = __shfl_sync(~0u, a, place);
-    const unsigned mine = __ballot_sync(~0u, m >= 0 && a == cur) & 0xffffu;
-    if (__ffs(mine) - 1 != place) return;
-    const int rows[2] = {__shfl_sync(~0u, m, g), __shfl_sync(~0u, m, g + 8)};
-    const bool keep[2] = {(mine >> g & 1) != 0, (mine >> (g + 8) & 1) != 0};
-    uint4 b[AHEAD ? 4 : 1][4];
-    if (AHEAD)
+    LrVec<LC> v;
+    if (LC == 8) { const uint4 x = lr_ldcg(reinterpret_cast<const uint4 *>(p)); v.w[0] = x.x; v.w[1] = x.y; v.w[LC / 2 - 2] = x.z; v.w[LC / 2 - 1] = x.w; }
+    else asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(v.w[0]), "=r"(v.w[1]) : "l"(p) : "memory");
+    return v;
+}
+// One or two rows of a place: blocks b0 .. b1 - 1 of 128 LC columns.  Whatever a block or 16 inner indices need next takes the
+// registers' place as soon as they are used.
+template <bool F32, int LC> __device__ __forceinline__ void lr_few(const LoraParams &p, float *tf, int j0, int cur, unsigned mine, int m, int b0, int b1, bool wait)
+{
+    constexpr int BW = F32 ? LC : LC / 2;                 // words of a row's base
+    const bool two = (mine & (mine - 1)) != 0;
+    const int place[2] = {__ffs(mine) - 1, two ? __ffs(mine & (mine - 1)) - 1 : __ffs(mine) - 1};
+    const int row[2] = {__shfl_sync(~0u, m, place[0]), __shfl_sync(~0u, m, place[1])};
+    int n = b0 * (128 * LC) + threadIdx.x * LC;
+    const bf16 *B = p.Bm + (size_t)max(cur, 0) * p.R * p.N + n;
+    LrVec<LC> b[16];
+    uint32_t base[2][BW];
+    // 16 rows of B from `from` on, `have` of them there
+    const auto ask = [&](int r, const bf16 *&from, int have) { if (r < have) b[r] = lr_ldv<LC>(from); from += p.N; };
+    const auto ask_base = [&](int n) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) lr_up_b(p, cur, blockIdx.y * UP + 256 * i + 64 * warp, 0, b[AHEAD ? i : 0]);
+        for (int e = 0; e < 2; e++) {
+            if (n >= p.N || (e && !two)) continue;
+#pragma unroll
+            for (int k = 0; k < BW; k += LC / 2) {
+                const LrVec<LC> v = lr_ldv<LC>(reinterpret_cast<const bf16 *>(reinterpret_cast<const uint32_t *>(p.base) + ((size_t)row[e] * p.N + n) / (F32 ? 1 : 2) + k));
+#pragma unroll
+                for (int i = 0; i < LC / 2; i++) base[e][k + i] = v.w[i];
+            }
+        }
+    };
+#pragma unroll
+    for (int r = 0; r < 16; r++) b[r] = {};
+    {
+        const bf16 *from = B;
+        const int have = cur >= 0 && n < p.N ? p.R : 0;
+#pragma unroll
+        for (int r = 0; r < 16; r++) ask(r, from, have);
+    }
+    ask_base(n);
+    if (wait) pdl_wait();
+    else __syncthreads();                     // the place before this one is done with tf
     if (cur >= 0) {
         const float scale = p.scale[cur];
-        for (int i = threadIdx.x; i < 16 * p.R / 2; i += 128) {
-            const int r = i / (p.R / 2), col = 2 * (i % (p.R / 2));
-            if (!(mine >> r & 1)) continue;
-            float x = 0.0f, y = 0.0f;
-            const float *src = p.part + (size_t)(j0 + r) * p.R + col;
+        for (int i = threadIdx.x; i < (two ? 2 : 1) * p.R; i += 128) {
+            const int e = i >= p.R, r = e ? i - p.R : i;
+            float x = 0.0f;
+            const float *src = p.part + (size_t)(j0 + place[e]) * p.R + r;
 #pragma unroll 8
-            for (int s = 0; s < p.S; s++) { const float2 v = *reinterpret_cast<const float2 *>(src + (size_t)s * p.M * p.R); x += v.x; y += v.y; }
-            uint32_t t[TT];
-            lr_split<TT>(x * scale, y * scale, t);
-#pragma unroll
-            for (int k = 0; k < TT; k++) lr_t[(k * 16 + r) * ldt + col / 2] = t[k];
+            for (int s = 0; s < p.S; s++) x += src[(size_t)s * p.M * p.R];
+            tf[e * 256 + r] = x * scale;
         }
         __syncthreads();
     }
-    if (AHEAD) {
+    for (int blk = b0; blk < b1; blk++, n += 128 * LC) {
+        float c[2][LC] = {};
+        if (cur >= 0)
+            for (int r0 = 0; r0 < p.R; r0 += 16) {
+                const bool end = r0 + 16 >= p.R, half = r0 + 8 >= p.R;
+                if (end) B += 128 * LC;
+                const bf16 *from = end ? B : B + (size_t)(r0 + 16) * p.N;
+                const int have = end ? (blk + 1 < b1 && n + 128 * LC < p.N ? p.R : 0) : n < p.N ? p.R - r0 - 16 : 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int n0 = blockIdx.y * UP + 256 * i + 64 * warp;
-            if (n0 >= p.N) break;
-            uint4 base[2][2][F32 ? 2 : 1];
-            lr_up_base<F32>(p, base, n0, rows, keep);
-            float c[8][4] = {};
-            if (cur >= 0) lr_up_mul<F32>(p, c, b[AHEAD ? i : 0], lr_t + g * ldt, ldt, 0);
-            lr_up_store<F32>(p, c, base, cur, n0, rows, keep);
+                for (int r = 0; r < 16; r++) {
+                    if (r < 8 || !half) {
+                        float f[LC];
+#pragma unroll
+                        for (int k = 0; k < LC / 2; k++) { f[2 * k] = __uint_as_float(b[r].w[k] << 16); f[2 * k + 1] = __uint_as_float(b[r].w[k] & 0xffff0000u); }
+                        const float t0 = tf[r0 + r];
+#pragma unroll
+                        for (int k = 0; k < LC; k++) c[0][k] = fmaf(t0, f[k], c[0][k]);
+                        if (two) {
+                            const float t1 = tf[256 + r0 + r];
+#pragma unroll
+                            for (int k = 0; k < LC; k++) c[1][k] = fmaf(t1, f[k], c[1][k]);
+                        }
+                    }
+                    ask(r, from, have);
+                }
+            }
+        uint32_t w[2][BW];
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int k = 0; k < BW; k++) {
+                if (F32) w[e][k] = __float_as_uint(__uint_as_float(base[e][k]) + c[e][k]);
+                else {
+                    const __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(base[e][k] << 16) + c[e][2 * k], __uint_as_float(base[e][k] & 0xffff0000u) + c[e][2 * k + 1]);
+                    w[e][k] = cur >= 0 ? *reinterpret_cast<const uint32_t *>(&h2) : base[e][k];
+                }
+            }
+        if (blk + 1 < b1) ask_base(n + 128 * LC);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if (n >= p.N || (e && !two)) continue;
+            uint32_t *d = reinterpret_cast<uint32_t *>(p.Y) + ((size_t)row[e] * p.N + n) / (F32 ? 1 : 2);
+#pragma unroll
+            for (int k = 0; k < BW; k += 4) {
+                if (BW >= 4) *reinterpret_cast<uint4 *>(d + k) = make_uint4(w[e][k], w[e][k + 1], w[e][BW >= 4 ? k + 2 : 0], w[e][BW >= 4 ? k + 3 : 0]);
+                else *reinterpret_cast<uint2 *>(d) = make_uint2(w[e][0], w[e][1]);
+            }
         }
-        return;
     }
-    const int n1 = min(p.N, ((int)blockIdx.y + 1) * UP);
-    for (int n0 = blockIdx.y * UP + 64 * warp; n0 < n1; n0 += 256) lr_up<F32>(p, lr_t + g * ldt, ldt, cur, n0, rows, keep);
+}
+template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora_up(const __grid_constant__ LoraParams p)
+{
+    constexpr int TT = F32 ? 3 : 2, EB = F32 ? 4 : 2, UP = lr_cols<F32, AHEAD>(), NB = UP / 256, PITCH = lr_pitch<F32, AHEAD>(), PIECES = UP * EB / 16;
+    extern __shared__ __align__(16) uint8_t lr_s[];
+    uint32_t *ts = reinterpret_cast<uint32_t *>(lr_s + 16 * PITCH);       // [term][16][ldt] pairs of bf16
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, ldt = (p.R + 15) / 16 * 8 + 4;
+    pdl_trigger();
+    const int j0 = (int)blockIdx.x / 16 * 16;
+    int m, a;
+    lr_row(p, j0 + (lane & 15), m, a, false);
+    // The tile's places that have work (the first of each adapter), times blocks of columns, in equal shares to its 16 gridDim.y CTAs
+    const unsigned same = __match_any_sync(~0u, m >= 0 ? a : -2) & 0xffffu;
+    const unsigned work = __ballot_sync(~0u, m >= 0 && __ffs(same) - 1 == lane && !(a < 0 && p.Y == p.base));
+    const int blocks = (p.N + UP - 1) / UP, total = __popc(work) * blocks, shares = 16 * gridDim.y, me = blockIdx.x % 16 * gridDim.y + blockIdx.y;
+    const int u1 = (int)((long long)total * (me + 1) / shares);
+    int u = (int)((long long)total * me / shares);
+    if (u == u1) { pdl_wait(); return; }
+    for (bool wait = true; u < u1; wait = false) {
+        unsigned w = work;
+        for (int k = u / blocks; k; k--) w &= w - 1;
+        const int place = __ffs(w) - 1, b0 = u % blocks, b1 = min(blocks, b0 + u1 - u);
+        u += b1 - b0;                         // this place's part of the share
+        const int cur = __shfl_sync(~0u, a, place);
+        const unsigned mine = __ballot_sync(~0u, m >= 0 && a == cur) & 0xffffu;
+        if (__popc(mine) <= LR_FEW) { lr_few<F32, UP / 128>(p, reinterpret_cast<float *>(lr_s), j0, cur, mine, m, b0, b1, wait); continue; }
+        if (!wait) __syncthreads();               // the place before this one is done with the shared memory
+        uint4 b[AHEAD ? NB : 1][4];
+        const auto ask = [&](int c0) {            // B and the base of the CTA's columns
+            if (AHEAD)
+#pragma unroll
+                for (int i = 0; i < NB; i++) lr_up_b<true>(p, cur, c0 + 256 * i + 64 * warp, 0, b[AHEAD ? i : 0]);
+            for (int i = threadIdx.x; i < 16 * PIECES; i += 128) {
+                const int r = i / PIECES, n = c0 + i % PIECES * (16 / EB), row = __shfl_sync(~0u, m, r);     // r: the warp's
+                if ((mine >> r & 1) && n < p.N) lt_copy(lt_addr(lr_s + r * PITCH + i % PIECES * 16), reinterpret_cast<const uint8_t *>(p.base) + ((size_t)row * p.N + n) * EB, true);
+            }
+            lt_commit();
+        };
+        ask(b0 * UP);
+        if (wait) pdl_wait();
+        const int rows[2] = {__shfl_sync(~0u, m, g), __shfl_sync(~0u, m, g + 8)};
+        const bool keep[2] = {(mine >> g & 1) != 0, (mine >> (g + 8) & 1) != 0};
+        if (cur >= 0) {
+            const float scale = p.scale[cur];
+            for (int i = threadIdx.x; i < 16 * p.R / 2; i += 128) {
+                const int r = i / (p.R / 2), col = 2 * (i % (p.R / 2));
+                if (!(mine >> r & 1)) continue;
+                float x = 0.0f, y = 0.0f;
+                const float *src = p.part + (size_t)(j0 + r) * p.R + col;
+#pragma unroll 8
+                for (int s = 0; s < p.S; s++) { const float2 v = *reinterpret_cast<const float2 *>(src + (size_t)s * p.M * p.R); x += v.x; y += v.y; }
+                uint32_t t[TT];
+                lr_split<TT>(x * scale, y * scale, t);
+#pragma unroll
+                for (int k = 0; k < TT; k++) ts[(k * 16 + r) * ldt + col / 2] = t[k];
+            }
+        }
+        for (int c0 = b0 * UP;;) {
+            lt_wait<0>();
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const int n0 = c0 + 256 * i + 64 * warp;
+                if (n0 >= p.N) break;
+                float c[8][4] = {};
+                if (cur >= 0) {
+                    if (AHEAD) lr_up_mul<F32>(p, c, b[AHEAD ? i : 0], ts + g * ldt, ldt, 0);
+                    else lr_up<F32>(p, c, ts + g * ldt, ldt, cur, n0);
+                }
+                uint4 base[2][2][F32 ? 2 : 1];
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int k = 0; k < (F32 ? 2 : 1); k++) base[e][h][k] = *reinterpret_cast<const uint4 *>(lr_s + (g + 8 * e) * PITCH + (256 * i + 64 * warp + 16 * q + 8 * h) * EB + 16 * k);
+                lr_up_store<F32>(p, c, base, cur, n0, rows, keep);
+            }
+            c0 += UP;
+            if (c0 >= b1 * UP) break;
+            __syncthreads();
+            ask(c0);
+        }
+    }
 }
 
 // Which form, and the slices of K of LORA_TWO.  Us, on both sides of each border (bf16, M rows on so many adapters):
-//   TILE above 2048 rows      K 768, N 1536, R 64: 2048 / 8 rows 19.6 as tiles, 26.9 as places; 8192 / 9 32.7 and 81.6
-//                             K 768, N 768, R 16: 2048 / 8 14.7 and 12.3, 8192 / 9 22.2 and 30.0; K 4096, N 4096, R 32: 1024 / 64
-//                             (runs of 16) 135 and 58, 8192 / 9 84 and 174
-//   ONE up to 256 rows and K R of 32768, where making the inner numbers once per 512 columns costs less than a launch
-//                             K 768, N 768, R 16: 64 rows 3.7 instead of 6.9, 256 / 2 4.7 and 7.0, 512 / 64 10.5 and 9.7
-//                             K 768, N 1536, R 64 (K R 49152): 64 rows 14.2 and 13.3
+//   TILE above 2048 rows      K 768, N 1536, R 64: 2048 / 8 rows 19.6 as tiles, 22.3 as places; 8192 / 9 32.7 and 81.6
+//                             K 768, N 768, R 16: 2048 / 8 14.7 and 13.1, 8192 / 9 22.2 and 30.0; K 4096, N 4096, R 32: 1024 / 64
+//                             (runs of 16) 135 and 52, 8192 / 9 84 and 174
+//   ONE up to 256 rows, K R of 32768 and N of 2048 (or M N of 32768), where making the inner numbers once per 512 columns costs less
+//                             than a launch.  K 768, N 768, R 16: 64 rows 4.8 instead of 6.2, 256 / 64 7.2 and 9.7, 512 / 64 10.5 and
+//                             9.7; K 2048, N 2048, R 16: 64 / 64 7.2 and 8.1; K 768, N 4096, R 16: 8 / 8 4.5 and 5.5, 64 / 64 10.4 and
+//                             7.4; K 768, N 16384, R 16: 1 row 5.7 and 5.5, 64 / 64 30.8 and 15.1
+//                             K 768, N 1536, R 64 (K R 49152): 64 rows 14.2 and 10.3
 enum LoraForm { LORA_ONE, LORA_TWO, LORA_TILE };
-static LoraForm lora_form(int M, int K, int R, int *S, int *kslice)
+static LoraForm lora_form(int M, int K, int N, int R, int *S, int *kslice)
 {
     *kslice = K; *S = 0;
     if (M > 2048) return LORA_TILE;
-    if (M <= 256 && R <= 64 && (long long)K * R <= 32768) return LORA_ONE;
+    if (M <= 256 && R <= 64 && (long long)K * R <= 32768 && (N <= 2048 || (long long)M * N <= 32768)) return LORA_ONE;
     long long s = (4LL * sm_count() + M - 1) / M;
     const long long most = (K + 511) / 512;              // four warps with four steps of 32 each
     if (s > most) s = most;
@@ -603,7 +762,7 @@ extern "C" size_t qlmb_lora_bytes(int M, int K, int N, int R)
 {
     if (!lora_shape_ok(M, K, N, R)) return 0;
     int S, ks;
-    return lora_form(M, K, R, &S, &ks) == LORA_TWO ? (size_t)S * M * R * sizeof(float) : 16;
+    return lora_form(M, K, N, R, &S, &ks) == LORA_TWO ? (size_t)S * M * R * sizeof(float) : 16;
 }
 template <bool F32> static int lora_launch(const LoraParams &p, LoraForm form, cudaStream_t st)
 {
@@ -632,12 +791,24 @@ template <bool F32> static int lora_launch(const LoraParams &p, LoraForm form, c
         return QLMB_OK;
     }
     const bool narrow = p.R <= 16;
+    // blocks of columns, and how many CTAs of k_lora_up there are to each 16 rows: as many as fit the device at once
+    const int cols = narrow ? lr_cols<F32, true>() : lr_cols<F32, false>(), blocks = (p.N + cols - 1) / cols;
+    const int each = (int)(((long long)blocks * p.M + 4 * sm_count() - 1) / (4 * sm_count()));
     const unsigned units = (unsigned)((p.M + 15) / 16 * 16);
-    const dim3 gd(units, (unsigned)p.S, (unsigned)(narrow ? 1 : (p.R + LR_RT - 1) / LR_RT)), gu(units, (unsigned)(narrow ? (p.N + 1023) / 1024 : (p.N + LR_UP - 1) / LR_UP));
+    const dim3 gd(units, (unsigned)p.S, (unsigned)(narrow ? 1 : (p.R + LR_RT - 1) / LR_RT)), gu(units, (unsigned)((blocks + each - 1) / each));
     QLMB_REQUIRE(gd.y < 65536 && gu.y < 65536, "qlmb_lora_add: K %d, N %d", p.K, p.N);
+    static bool configured_dev[64];
+    int dev = 0;
+    QLMB_CUDA(cudaGetDevice(&dev));
+    QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
+    if (!configured_dev[dev]) {
+        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, true>(16)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, false>(256)));
+        configured_dev[dev] = true;
+    }
     QLMB_CUDA(pdl_launch_small(narrow ? k_lora_down<F32, 2, 4> : k_lora_down<F32, LR_RT / 8, 1>, gd, dim3(128), 0, st, p));
     QLMB_LAUNCH_CHECK("k_lora_down");
-    QLMB_CUDA(pdl_launch_small(narrow ? k_lora_up<F32, true> : k_lora_up<F32, false>, gu, dim3(128), (size_t)(F32 ? 3 : 2) * 16 * ((p.R + 15) / 16 * 8 + 4) * sizeof(uint32_t), st, p));
+    QLMB_CUDA(pdl_launch(true, narrow ? k_lora_up<F32, true> : k_lora_up<F32, false>, gu, dim3(128), narrow ? lr_smem<F32, true>(p.R) : lr_smem<F32, false>(p.R), st, p));
     QLMB_LAUNCH_CHECK("k_lora_up");
     return QLMB_OK;
 }
@@ -652,6 +823,6 @@ extern "C" int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype
     const size_t need = qlmb_lora_bytes(M, K, N, R);
     QLMB_REQUIRE(need <= 16 || (ws && ws_bytes >= need), "qlmb_lora_add: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
     LoraParams p = {Y, X, base, (const bf16 *)A, (const bf16 *)Bm, scale, adapter, order, (float *)ws, M, K, N, R, adapters, 0, 0, device_error_word()};
-    const LoraForm form = lora_form(M, K, R, &p.S, &p.kslice);
+    const LoraForm form = lora_form(M, K, N, R, &p.S, &p.kslice);
     return dtype == QLMB_F32 ? lora_launch<true>(p, form, as_stream(stream)) : lora_launch<false>(p, form, as_stream(stream));
 }
