@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 //
 // Measured (12 heads, 12 kv heads unless stated; graph of calls, all launches): 1 slot after 512 keys 9.2 us, 8 slots of 4 tokens after
 // 2048 10.9 us (both the length of three small launches), 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
-// 16 heads of 4 kv heads after 32768 95 us.  In the last k_px_tc has 75 us, 43 G scores at 0.57 T/s: without exponentials 60 us,
-// without any softmax 41 us, which is what its MMAs of 64 columns take by themselves.
+// 16 heads of 4 kv heads after 32768 95 us.  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of
+// the special-function units; without them it takes 60 us, without any softmax 41 us, which is what its MMAs of 64 columns need.
 constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
 constexpr uint32_t PX_TRIES = 1u << 20;                   // a wait gives up after so many tries
 constexpr int PX_MAXB = 1024;                             // slots: every CTA keeps their positions and block counts
