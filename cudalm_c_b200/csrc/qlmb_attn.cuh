@@ -1,4 +1,4 @@
-// Shared by the attention kernels (qlmb_attn.cu, qlmb_prefix.cu): their bounded wait, 2^x, two-wide fp32.
+// Shared by the attention kernels and the adapters' (qlmb_attn.cu, qlmb_prefix.cu, qlmb_lora.cu): bounded waits, 2^x, two-wide fp32.
 #pragma once
 #include "qlmb_tc.cuh"
 
@@ -41,6 +41,23 @@ __device__ __forceinline__ bool at_wait(uint32_t bar, uint32_t parity, volatile 
         if (errword && atomicCAS(errword, 0, 200) == 0) { errword[1] = site; errword[2] = (int)blockIdx.x; errword[3] = (int)parity; }
     }
     return false;
+}
+constexpr uint32_t AT_TRIES = 1u << 20;                     // a warp's wait gives up after so many
+// A warp's wait: all of its lanes go on (0), or none (the site).  Bounded like the library's other waits.  try_wait lets the hardware
+// hold the warp until the phase ends or a time of its own is over: a loop of test_wait instead keeps the queue busy that the
+// exponentials go through, too.
+__device__ __forceinline__ int at_all_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int site)
+{
+#pragma unroll 1
+    for (uint32_t i = 0; !__all_sync(~0u, mbar_try(bar, parity)); i++)
+        if ((i & 255u) == 255u && (*abort_flag || i > AT_TRIES)) return site;
+    return 0;
+}
+__device__ __forceinline__ void at_give_up(int site, volatile int *abort_flag, int *errword)
+{
+    if (!site || *abort_flag) return;
+    *abort_flag = 1;
+    if (errword && atomicCAS(errword, 0, 200) == 0) { errword[1] = site; errword[2] = (int)blockIdx.x; }
 }
 __device__ __forceinline__ bool at_error_seen(const int *errword) { return errword && *reinterpret_cast<const volatile int *>(errword) != 0; }
 

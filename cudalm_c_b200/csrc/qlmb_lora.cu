@@ -9,8 +9,12 @@
 // The R inner numbers of a row are sums in fp32; they enter the second product as two bf16 terms (bf16 rows) or three (fp32 rows), and
 // so does X where it is fp32: 16 and 24 bits.
 //
+#include <cuda.h>
 #include <cuda_bf16.h>
+#include <string.h>
 #include "qlmb_common.cuh"
+#include "qlmb_gemm.cuh"
+#include "qlmb_attn.cuh"
 #include "qlmb_internal.h"
 
 namespace qlmb {
@@ -215,7 +219,7 @@ template <bool F32> __device__ __forceinline__ void lr_up(const LoraParams &p, f
     }
 }
 
-// ---- many rows.  A CTA of eight warps (four row groups of 16 times two halves of 32 columns) has 64 rows: the products' operands come
+// ---- many rows that are fp32, out of order or of another rank.  A CTA of eight warps (four row groups of 16 times two halves of 32 columns) has 64 rows: the products' operands come
 // through a ring of four stages in shared memory, a stage being 64 x 64 elements of X (or of the base) and of A (or B), in 16-byte
 // pieces whose place is turned by the row.  First the inner numbers over K, 64 at a time, kept as bf16 terms; then Y, 64 columns at a
 // time: the base lies in the stage, the sum takes its place there and leaves in whole pieces.
@@ -443,6 +447,333 @@ template <bool F32, bool SMALL> __global__ void __launch_bounds__(256, 2) k_lora
             for (int n = c0 + lane * (16 / EB); n < c1; n += 32 * (16 / EB))
                 *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p.Y) + ((size_t)row * p.N + n) * EB) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p.base) + ((size_t)row * p.N + n) * EB);
         }
+}
+
+// ---- many neighbouring rows in bf16, ranks of whole 16: tcgen05.  A pair is a tile of 128 rows and an adapter that occurs in it (rows without
+// one, where Y is not the base, are such a pair, too); the pairs' blocks of 64 columns are dealt out evenly to the CTAs, one an SM.
+//
+//   warp 0      TMA into a ring of stages of 64 columns: X and A along K, then the base and B along N
+//   warp 1      D = X A^T (128 x R), then for every block T B (128 x 64, T as two bf16 terms in tensor memory)
+//   warps 2-9   D to T; of a block two groups of four warps take turns: a thread has a row, adds the sum to its base in the stage, and
+//               the warp's rows leave by TMA (by plain stores where some are another adapter's)
+//
+// Tensor memory: T in columns 0 and 128, D in 256, which the blocks' sums (four of 64 columns) take over once D is read.
+//
+// 8192 rows on 9 adapters, K 768, N 1536, R 64: 22.6 us (63 MB, 2.8 TB/s; 64-row tiles on mma.sync 32.7).  Of a CTA's 27 k cycles in front of
+// its end: counting adapters 5 k, the first pair's walk and copies 4 k, 12 steps of K 6 k (511 a step of 24 KB, what an SM gets from L2
+// when all ask), D to T 2 k, 12 blocks 10 k.  Rows leaving by plain stores instead of TMA: 23.7; a fence behind those stores, which it
+// then waits for: 26.
+constexpr int LC_T = 320, LC_TILES = 8192, LC_NS = 8;
+struct LcParams { alignas(64) CUtensorMap x_map, a_map, base_map, b_map, y_map; LoraParams l; int stages; };
+static int lc_stage(int R) { return 128 * 128 + R * 128; }
+static size_t lc_smem(int R, int stages) { return (size_t)stages * lc_stage(R) + LC_TILES + 512; }
+static int lc_stages(int R) { const int s = (226 * 1024 - LC_TILES - 512) / lc_stage(R); return s < LC_NS ? s : LC_NS; }
+
+// A warp's way through the pairs: the tile's adapters (row 32 k + lane), those that are still to come
+struct LcWalk { int t, cur, a[4]; unsigned todo[4]; };
+__device__ __forceinline__ void lc_ask(const LoraParams &p, int t, int (&a)[4])
+{
+#pragma unroll
+    for (int k = 0; k < 4; k++) { const int row = 128 * t + 32 * k + (threadIdx.x & 31); a[k] = row < p.M ? p.adapter[row] : -2; }
+}
+__device__ __forceinline__ void lc_open(const LoraParams &p, LcWalk &w, const int (&v)[4], bool report)
+{
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int row = 128 * w.t + 32 * k + (threadIdx.x & 31);
+        w.a[k] = v[k];
+        if (row < p.M && (v[k] < -1 || v[k] >= p.adapters)) { if (report) report_bad_index(p.errword, 307, row, v[k]); w.a[k] = -1; }
+        if (w.a[k] == -1 && p.Y == p.base) w.a[k] = -2;
+        w.todo[k] = __ballot_sync(~0u, w.a[k] != -2);
+    }
+}
+__device__ __forceinline__ bool lc_pick(LcWalk &w)        // the tile's next adapter
+{
+    if (!(w.todo[0] | w.todo[1] | w.todo[2] | w.todo[3])) return false;
+    const unsigned t = w.todo[0] ? w.todo[0] : w.todo[1] ? w.todo[1] : w.todo[2] ? w.todo[2] : w.todo[3];
+    const int v = w.todo[0] ? w.a[0] : w.todo[1] ? w.a[1] : w.todo[2] ? w.a[2] : w.a[3];
+    w.cur = __shfl_sync(~0u, v, __ffs(t) - 1);
+#pragma unroll
+    for (int k = 0; k < 4; k++) w.todo[k] &= ~__ballot_sync(~0u, w.a[k] == w.cur);
+    return true;
+}
+
+__global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcParams cp)
+{
+    extern __shared__ __align__(1024) uint8_t lc_s[];
+    const LoraParams &p = cp.l;
+    const int NS = cp.stages, STAGE = 128 * 128 + p.R * 128;
+    uint8_t *cnt = lc_s + (size_t)NS * STAGE;             // adapters of a tile
+    uint64_t *bars = reinterpret_cast<uint64_t *>(cnt + LC_TILES);
+    uint64_t *full = bars, *empty = bars + LC_NS, *d2_full = empty + LC_NS, *d2_empty = d2_full + 4, *d1_full = d2_empty + 4, *t_full = d1_full + 1, *spare = t_full + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(spare + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    int *sum = const_cast<int *>(abort_flag) + 1, *begin = sum + 1;                  // pairs; the CTA's first tile, and pairs of it before the first
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(lc_s) & 1023u) {             // the swizzled tiles need a 1 KiB-aligned base
+        if (tid == 0 && p.errword && atomicCAS(p.errword, 0, 201) == 0) { p.errword[1] = 160; p.errword[2] = (int)blockIdx.x; }
+        pdl_wait();
+        return;
+    }
+    if (tid == 0) {
+        prefetch_map(&cp.x_map); prefetch_map(&cp.a_map); prefetch_map(&cp.base_map); prefetch_map(&cp.b_map);
+        for (int i = 0; i < NS; i++) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 4); }
+        for (int i = 0; i < 4; i++) { mbar_init(smem_u32(&d2_full[i]), 1); mbar_init(smem_u32(&d2_empty[i]), 4); }
+        mbar_init(smem_u32(d1_full), 1);
+        mbar_init(smem_u32(t_full), 8);
+        mbar_init(smem_u32(spare), 1);
+        *abort_flag = 0;
+        *sum = 0; begin[0] = begin[1] = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_wait();                               // barriers and TMEM above are this kernel's own; its inputs come below
+    pdl_trigger();
+    // ---- the tiles' adapters are counted, and the CTA's share found
+    const int tiles = (p.M + 127) / 128, blocks = (p.N + 63) / 64;
+    LcWalk w;
+    {
+        int mine = 0;
+        for (int t = warp; t < tiles; t += 4 * (LC_T / 32)) {             // four tiles a warp at a time
+            int v[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) lc_ask(p, t + i * (LC_T / 32), v[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                w.t = t + i * (LC_T / 32);
+                if (w.t >= tiles) break;
+                int n = 1;
+                const int one = __shfl_sync(~0u, v[i][0], 0);             // mostly there is one adapter
+                if (!__all_sync(~0u, v[i][0] == one && v[i][1] == one && v[i][2] == one && v[i][3] == one) || one < 0 || one >= p.adapters) {
+                    lc_open(p, w, v[i], blockIdx.x == 0);
+                    for (n = 0; lc_pick(w);) n++;
+                }
+                if (lane == 0) cnt[w.t] = (uint8_t)n;
+                mine += n;
+            }
+        }
+        if (lane == 0 && mine) atomicAdd(sum, mine);
+    }
+    __syncthreads();
+    // (below 2^31, and in 32 bits: divisions in 64 took 1.2 us)
+    const int units = *sum * blocks, share = units / (int)gridDim.x, over = units - share * (int)gridDim.x, me = blockIdx.x;
+    const int u0 = share * me + min(me, over), u1 = u0 + share + (me < over), pair0 = u0 / blocks;
+    if (warp == 0 && u0 < u1) {
+        int before = 0;
+        for (int t0 = 0; t0 < tiles; t0 += 32) {
+            const int n = t0 + lane < tiles ? cnt[t0 + lane] : 0;
+            int x = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(~0u, x, o); if (lane >= o) x += y; }
+            const int at = before + x - n;
+            if (at <= pair0 && pair0 < at + n) { begin[0] = t0 + lane; begin[1] = pair0 - at; }
+            before += __shfl_sync(~0u, x, 31);
+            if (before > pair0) break;
+        }
+    }
+    __syncthreads();
+    const uint32_t tT = *tmem_slot, tD = tT + 256;
+    // the next pair, and its blocks b0 .. b1 - 1
+    int u = u0, b0 = 0, b1 = 0, bad = 0, ask[4];
+    const auto next = [&]() {
+        if (u >= u1) return false;
+        if (u == u0) {
+            w.t = begin[0];
+            lc_ask(p, w.t, ask);
+            lc_open(p, w, ask, false);
+            for (int i = begin[1]; i >= 0; i--) lc_pick(w);
+            b0 = u0 - pair0 * blocks;
+        } else {
+            b0 = 0;
+            if (!lc_pick(w)) {
+                do w.t++; while (w.t + 1 < tiles && cnt[w.t] == 0);
+                lc_ask(p, w.t, ask);
+                lc_open(p, w, ask, false);
+                lc_pick(w);
+            }
+        }
+        b1 = min(blocks, b0 + u1 - u);
+        u += b1 - b0;
+        return true;
+    };
+    const int steps = (p.K + 63) / 64;
+    int s = 0;                                // the stage, and how often the ring was gone through
+    uint32_t phase = 0;
+    const auto advance = [&](int n) { for (s += n; s >= NS; s -= NS) phase ^= 1; };
+
+    if (warp == 0) {
+        int issued = 0;
+        while (!bad && next()) {
+            const int n = (w.cur >= 0 ? steps : 0) + b1 - b0;
+            for (int i = 0; i < n; i++) {
+                if ((bad = at_all_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, 161))) break;
+                const bool inner = w.cur >= 0 && i < steps;
+                const int x = 64 * (inner ? i : b0 + i - (w.cur >= 0 ? steps : 0));
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&full[s]), d = smem_u32(lc_s + s * STAGE);
+                    mbar_expect_tx(bar, w.cur >= 0 ? STAGE : 128 * 128);
+                    tma_load_2d(d, inner ? &cp.x_map : &cp.base_map, bar, x, 128 * w.t);
+                    if (w.cur >= 0) tma_load_2d(d + 128 * 128, inner ? &cp.a_map : &cp.b_map, bar, x, w.cur * p.R);
+                }
+                __syncwarp();
+                issued++;
+                advance(1);
+            }
+        }
+        at_give_up(bad, abort_flag, p.errword);
+        if (*abort_flag)                      // copies under way end (bounded) before memory is given back
+            for (int i = issued > NS ? issued - NS : 0; i < issued; i++)
+                for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(&full[i % NS]), (uint32_t)(i / NS) & 1u); k++) {}
+    } else if (warp == 1) {
+        const uint32_t IDESC_D = make_idesc(128, p.R, 0, 0);
+        constexpr uint32_t IDESC_Y = make_idesc(128, 64, 0, 1);
+        const uint64_t x00 = make_desc(smem_u32(lc_s), 16, 1024), a00 = make_desc(smem_u32(lc_s) + 128 * 128, 16, 1024), b00 = make_desc(smem_u32(lc_s) + 128 * 128, 8192, 1024);
+        int nb = 0, np = 0;                   // blocks, pairs with an adapter
+        while (!bad && next()) {
+            if (w.cur < 0) { advance(b1 - b0); continue; }
+            for (int k = 0; k < 4 && !bad; k++) {         // D takes the place of the last pair's sums
+                const int uses = (nb - k + 3) / 4;
+                if (uses > 0) bad = at_all_wait(smem_u32(&d2_empty[k]), (uint32_t)(uses - 1) & 1u, abort_flag, 162);
+            }
+            for (int i = 0; i < steps && !bad; i++) {
+                if ((bad = at_all_wait(smem_u32(&full[s]), phase, abort_flag, 163))) break;
+                tc_fence_after();
+                const uint64_t o = (uint64_t)(s * (STAGE / 16));
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tc_mma_bf16(tD, x00 + o + 2 * k, a00 + o + 2 * k, IDESC_D, i > 0 || k > 0);
+                    for (int k = 0; k < 3; k++) mbar_arrive(smem_u32(&empty[s]));    // (a block's stage is given back by four warps)
+                    tc_commit(smem_u32(&empty[s]));
+                    if (i + 1 == steps) tc_commit(smem_u32(d1_full));
+                }
+                __syncwarp();
+                advance(1);
+            }
+            if (bad || (bad = at_all_wait(smem_u32(t_full), (uint32_t)np & 1u, abort_flag, 164))) break;
+            np++;
+            for (int b = b0; b < b1; b++, nb++) {
+                const int buf = nb & 3;
+                if ((bad = at_all_wait(smem_u32(&full[s]), phase, abort_flag, 165))) break;
+                if (nb >= 4 && (bad = at_all_wait(smem_u32(&d2_empty[buf]), (uint32_t)(nb / 4 - 1) & 1u, abort_flag, 166))) break;
+                tc_fence_after();
+                const uint64_t o = (uint64_t)(s * (STAGE / 16));
+                if (elect_one()) {
+                    for (int k = 0; k < p.R / 16; k++) {
+                        tc_mma_bf16_ta(tD + 64 * buf, tT + k * 8, b00 + o + 128 * k, IDESC_Y, k > 0);
+                        tc_mma_bf16_ta(tD + 64 * buf, tT + 128 + k * 8, b00 + o + 128 * k, IDESC_Y, 1);
+                    }
+                    tc_commit(smem_u32(&d2_full[buf]));
+                }
+                __syncwarp();
+                advance(1);
+            }
+        }
+        at_give_up(bad, abort_flag, p.errword);
+        if (*abort_flag) {                    // MMAs under way end (bounded) before memory is given back
+            if (elect_one()) tc_commit(smem_u32(spare));
+            __syncwarp();
+            for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(spare), 0); k++) {}
+        }
+    } else {
+        // a warp reaches the 32 lanes of tensor memory that its place in the warpgroup gives it
+        const int quarter = warp & 3, group = (warp - 2) >> 2, r = 32 * quarter + lane;
+        const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+        int nb = 0, np = 0, turn = 0;         // turn: blocks of all pairs
+        while (!bad && next()) {
+            const bool adapted = w.cur >= 0;
+            const int own = quarter == 0 ? w.a[0] : quarter == 1 ? w.a[1] : quarter == 2 ? w.a[2] : w.a[3];
+            const unsigned keep = __ballot_sync(~0u, own == w.cur);
+            const bool whole = keep == __ballot_sync(~0u, 128 * w.t + r < p.M);      // (rows behind the last are not stored)
+            if (adapted) {
+                const float scale = p.scale[w.cur];
+                if ((bad = at_all_wait(smem_u32(d1_full), (uint32_t)np & 1u, abort_flag, 167))) break;
+                np++;
+                tc_fence_after();
+                for (int c = 32 * group; c < p.R; c += 64) {             // (columns from R on are read and written, not used)
+                    uint32_t v[32], hi[16], lo[16];
+                    tmem_ld32(tD + lanes + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        uint32_t t[2];
+                        lr_split<2>(__uint_as_float(v[2 * k]) * scale, __uint_as_float(v[2 * k + 1]) * scale, t);
+                        hi[k] = t[0]; lo[k] = t[1];
+                    }
+                    tmem_st16(tT + lanes + c / 2, hi);
+                    tmem_st16(tT + 128 + lanes + c / 2, lo);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(t_full));
+                advance(steps);
+            }
+            for (int b = b0; b < b1; b++, turn++) {
+                const int buf = nb & 3, at = nb;
+                if (adapted) nb++;
+                if ((turn & 1) != group) { advance(1); continue; }
+                if ((bad = at_all_wait(smem_u32(&full[s]), phase, abort_flag, 168))) break;
+                if (adapted && (bad = at_all_wait(smem_u32(&d2_full[buf]), (uint32_t)(at / 4) & 1u, abort_flag, 169))) break;
+                uint8_t *tile = lc_s + s * STAGE;
+                if (adapted && keep) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t v[32];
+                        tmem_ld32(tD + 64 * buf + lanes + 32 * h, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            uint4 *d = reinterpret_cast<uint4 *>(tile + r * 128 + (((4 * h + c) ^ (r & 7)) << 4));
+                            uint4 x = *d;
+                            uint32_t *e = &x.x;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(e[k] << 16) + __uint_as_float(v[8 * c + 2 * k]),
+                                                                                __uint_as_float(e[k] & 0xffff0000u) + __uint_as_float(v[8 * c + 2 * k + 1]));
+                                e[k] = *reinterpret_cast<const uint32_t *>(&h2);
+                            }
+                            *d = x;
+                        }
+                    }
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (adapted && lane == 0) mbar_arrive(smem_u32(&d2_empty[buf]));
+                if (whole) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (keep && elect_one()) {
+                        tma_store_2d(&cp.y_map, smem_u32(tile + 32 * quarter * 128), 64 * b, 128 * w.t + 32 * quarter);
+                        bulk_commit();
+                        bulk_wait_read();
+                    }
+                } else {
+                    uint4 out[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) { const int rr = 32 * quarter + 4 * i + (lane >> 3); out[i] = *reinterpret_cast<const uint4 *>(tile + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)); }
+                    fence_proxy_async();                  // the next copy comes after these reads and writes (the fence waits for stores to Y, too)
+                    bf16 *y = reinterpret_cast<bf16 *>(p.Y) + (size_t)(128 * w.t + 32 * quarter + (lane >> 3)) * p.N + 64 * b + 8 * (lane & 7);
+                    if (64 * b + 8 * (lane & 7) < p.N)
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (keep >> (4 * i + (lane >> 3)) & 1) *reinterpret_cast<uint4 *>(y + (size_t)(4 * i) * p.N) = out[i];
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+                advance(1);
+            }
+        }
+        if (elect_one()) bulk_wait_all();
+        __syncwarp();
+        at_give_up(bad, abort_flag, p.errword);
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 0) { tc_fence_after(); tmem_dealloc(tT, 512); }
 }
 
 // ---- few rows, small adapters: one launch.  blockIdx.x = 16 tile + place: the CTA of a place that is the first of its adapter in the
@@ -728,7 +1059,8 @@ template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora
 }
 
 // Which form, and the slices of K of LORA_TWO.  Us, on both sides of each border (bf16, M rows on so many adapters):
-//   TILE above 2048 rows      K 768, N 1536, R 64: 2048 / 8 rows 19.6 as tiles, 22.3 as places; 8192 / 9 32.7 and 81.6
+//   TILE (what TC does not take) above 2048 rows
+//                             K 768, N 1536, R 64: 2048 / 8 rows 19.6 as tiles, 22.3 as places; 8192 / 9 32.7 and 81.6
 //                             K 768, N 768, R 16: 2048 / 8 14.7 and 13.1, 8192 / 9 22.2 and 30.0; K 4096, N 4096, R 32: 1024 / 64
 //                             (runs of 16) 135 and 52, 8192 / 9 84 and 174
 //   ONE up to 256 rows, K R of 32768 and N of 2048 (or M N of 32768), where making the inner numbers once per 512 columns costs less
@@ -736,7 +1068,7 @@ template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora
 //                             9.7; K 2048, N 2048, R 16: 64 / 64 7.2 and 8.1; K 768, N 4096, R 16: 8 / 8 4.5 and 5.5, 64 / 64 10.4 and
 //                             7.4; K 768, N 16384, R 16: 1 row 5.7 and 5.5, 64 / 64 30.8 and 15.1
 //                             K 768, N 1536, R 64 (K R 49152): 64 rows 14.2 and 10.3
-enum LoraForm { LORA_ONE, LORA_TWO, LORA_TILE };
+enum LoraForm { LORA_ONE, LORA_TWO, LORA_TILE, LORA_TC };
 static LoraForm lora_form(int M, int K, int N, int R, int *S, int *kslice)
 {
     *kslice = K; *S = 0;
@@ -749,6 +1081,17 @@ static LoraForm lora_form(int M, int K, int N, int R, int *S, int *kslice)
     *kslice = (int)(((K + s - 1) / s + 127) / 128 * 128);
     *S = (K + *kslice - 1) / *kslice;
     return LORA_TWO;
+}
+
+// TC: bf16 rows that stand in their order, ranks of whole 16 (a tile of D and of B has no rows of the next adapter then), counts that fit
+// 32 bits.  Us with it and without (M / adapters): K 768, N 1536, R 64: 512 / 8 11.0 and 14.8, 1024 / 4 9.9 and 17.8, 2048 / 8 12.0 and 22.1,
+// 8192 / 9 22.6 and 32.7, 32768 / 9 57.7 and 91.7; R 256: 8192 / 3 29 and 127; K 768, N 768, R 16: 512 / 1 8.2 and 7.9, 1024 / 8 9.2 and 10.3,
+// 8192 / 9 14.4 and 21.2.  Every CTA makes the inner numbers of its pairs for itself, which few rows do not pay for where K is large:
+// K 4096, N 4096: R 16 512 / 4 39 and 15, R 32 1024 / 64 57 and 53, 8192 / 9 61 and 91.
+static bool lora_tc_ok(int M, int K, int N, int R, int adapters)
+{
+    return R % 16 == 0 && (M > 2048 || (M >= 512 && K <= 1024)) && (M + 127) / 128 <= LC_TILES && (long long)M * ((N + 63) / 64) < (1LL << 31) &&
+           (long long)adapters * R < (1LL << 31);
 }
 
 }  // namespace qlmb
@@ -764,8 +1107,35 @@ extern "C" size_t qlmb_lora_bytes(int M, int K, int N, int R)
     int S, ks;
     return lora_form(M, K, N, R, &S, &ks) == LORA_TWO ? (size_t)S * M * R * sizeof(float) : 16;
 }
+static int lora_tc_launch(const LoraParams &p, cudaStream_t st)
+{
+    static bool configured_dev[64];                      // the attribute belongs to a device's copy of the kernel
+    int dev = 0;
+    QLMB_CUDA(cudaGetDevice(&dev));
+    QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
+    if (!configured_dev[dev]) {
+        QLMB_CUDA(cudaFuncSetAttribute(k_lora_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        configured_dev[dev] = true;
+    }
+    LcParams c;
+    memset(&c, 0, sizeof c);
+    c.l = p;
+    c.stages = lc_stages(p.R);
+    const unsigned long long M = p.M, K = p.K, N = p.N, AR = (unsigned long long)p.adapters * p.R;
+    const struct { CUtensorMap *m; const void *base; unsigned long long inner, rows; unsigned box; } maps[5] = {{&c.x_map, p.X, K, M, 128}, {&c.a_map, p.A, K, AR, (unsigned)p.R}, {&c.base_map, p.base, N, M, 128}, {&c.b_map, p.Bm, N, AR, (unsigned)p.R},
+                                                                                                                      {&c.y_map, p.Y, N, M, 32}};
+    for (int i = 0; i < 5; i++) {
+        const int rc = make_map(maps[i].m, maps[i].base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, maps[i].inner, maps[i].rows, maps[i].inner * 2, 64, maps[i].box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc) return rc;
+    }
+    const long long most = (long long)((p.M + 127) / 128) * ((p.N + 63) / 64);
+    QLMB_CUDA(pdl_launch(true, k_lora_tc, dim3((unsigned)(most < sm_count() ? most : sm_count())), dim3(LC_T), lc_smem(p.R, c.stages), st, c));
+    QLMB_LAUNCH_CHECK("k_lora_tc");
+    return QLMB_OK;
+}
 template <bool F32> static int lora_launch(const LoraParams &p, LoraForm form, cudaStream_t st)
 {
+    if (form == LORA_TC) return lora_tc_launch(p, st);
     if (form == LORA_TILE) {
         static bool configured_dev[64];                  // the attribute belongs to a device's copy of the kernel
         int dev = 0;
@@ -823,6 +1193,7 @@ extern "C" int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype
     const size_t need = qlmb_lora_bytes(M, K, N, R);
     QLMB_REQUIRE(need <= 16 || (ws && ws_bytes >= need), "qlmb_lora_add: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
     LoraParams p = {Y, X, base, (const bf16 *)A, (const bf16 *)Bm, scale, adapter, order, (float *)ws, M, K, N, R, adapters, 0, 0, device_error_word()};
-    const LoraForm form = lora_form(M, K, N, R, &p.S, &p.kslice);
+    LoraForm form = lora_form(M, K, N, R, &p.S, &p.kslice);
+    if (dtype == QLMB_BF16 && !order && lora_tc_ok(M, K, N, R, adapters)) form = LORA_TC;
     return dtype == QLMB_F32 ? lora_launch<true>(p, form, as_stream(stream)) : lora_launch<false>(p, form, as_stream(stream));
 }

@@ -77,7 +77,6 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 // 16 heads of 4 kv heads after 32768 95 us.  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of
 // the special-function units; without them it takes 60 us, without any softmax 41 us, which is what its MMAs of 64 columns need.
 constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
-constexpr uint32_t PX_TRIES = 1u << 20;                   // a wait gives up after so many tries
 constexpr int PX_MAXB = 1024;                             // slots: every CTA keeps their positions and block counts
 struct PxParams {
     alignas(64) CUtensorMap kc_map, vc_map, kp_map, vp_map;
@@ -122,22 +121,6 @@ __device__ __forceinline__ int px_blocks(const PxParams &p, long long t0)
     if (!px_slot_ok(t0, p.n, p.P, p.Tm)) return 0;
     const int hi = (int)t0 + p.n - 1 - p.P;
     return hi < 0 ? 0 : (hi - px_first(p, (int)t0)) / 32 + 1;
-}
-// A warp's wait: all of its lanes go on (0), or none (the site).  Bounded like the library's other waits.  try_wait lets the hardware
-// hold the warp until the phase ends or a time of its own is over: a loop of test_wait instead keeps the queue busy that the
-// exponentials go through, too.
-__device__ __forceinline__ int px_all_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int site)
-{
-#pragma unroll 1
-    for (uint32_t i = 0; !__all_sync(~0u, mbar_try(bar, parity)); i++)
-        if ((i & 255u) == 255u && (*abort_flag || i > PX_TRIES)) return site;
-    return 0;
-}
-__device__ __forceinline__ void px_give_up(int site, volatile int *abort_flag, int *errword)
-{
-    if (!site || *abort_flag) return;
-    *abort_flag = 1;
-    if (errword && atomicCAS(errword, 0, 200) == 0) { errword[1] = site; errword[2] = (int)blockIdx.x; }
 }
 // x / d for 0 <= x < 2^24: the quotient of the floats is off by one at most (a division of integers takes ten times as long)
 __device__ __forceinline__ int px_div(int x, int d)
@@ -292,7 +275,7 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
     uint32_t phase = 0;
     for (; count > 0; count--) {
         px_wait<0>();
-        if ((bad = px_all_wait(smem_u32(bar + stage), phase, abort_flag, 131))) break;
+        if ((bad = at_all_wait(smem_u32(bar + stage), phase, abort_flag, 131))) break;
         __syncwarp();
         const uint32_t sk = ring + stage * PX_STAGE, sv = sk + PX_BLK;
         phase ^= stage;
@@ -443,7 +426,7 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
         }
     }
     px_wait<0>();
-    px_give_up(bad, abort_flag, p.errword);
+    at_give_up(bad, abort_flag, p.errword);
     if (*abort_flag)                                      // aborting: the copies under way must land before the CTA gives its shared memory back
         for (int i = 0; i < 2; i++)
             for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(bar + i), i < stage ? phase ^ 1u : phase); k++) {}
@@ -530,12 +513,12 @@ __global__ void __launch_bounds__(PT_T, 3) k_px_tc(const __grid_constant__ PxTcP
         for (int t = 0; t < PT_NS; t++) load(t);
         // descriptors: an address is in their low bits, in units of 16 bytes
         const uint64_t q0 = make_desc(smem_u32(sQ), 16, 1024), k00 = make_desc(smem_u32(sKV), 16, 1024), v00 = make_desc(smem_u32(sKV) + PT_KV, 8192, 1024);
-        int st = 0, bad = px_all_wait(smem_u32(q_full), 0, abort_flag, 141);
+        int st = 0, bad = at_all_wait(smem_u32(q_full), 0, abort_flag, 141);
         uint32_t kv_phase = 0;
         for (int t = 0; !bad && t < nt; t++) {
-            if ((bad = px_all_wait(smem_u32(&kv_full[st]), kv_phase, abort_flag, 142))) break;
+            if ((bad = at_all_wait(smem_u32(&kv_full[st]), kv_phase, abort_flag, 142))) break;
             // P V of the last step has read the weights, over which the scores go, and its stage
-            if (t > 0 && (bad = px_all_wait(smem_u32(o_full), (uint32_t)(t - 1) & 1u, abort_flag, 143))) break;
+            if (t > 0 && (bad = at_all_wait(smem_u32(o_full), (uint32_t)(t - 1) & 1u, abort_flag, 143))) break;
             tc_fence_after();
             const uint64_t k0 = k00 + (uint64_t)(st * (2 * PT_KV / 16)), v0 = v00 + (uint64_t)(st * (2 * PT_KV / 16));
             if (elect_one()) {
@@ -546,7 +529,7 @@ __global__ void __launch_bounds__(PT_T, 3) k_px_tc(const __grid_constant__ PxTcP
             __syncwarp();
             if (++st == PT_NS) { st = 0; kv_phase ^= 1; }
             if (t > 0) load(t - 1 + PT_NS);
-            if ((bad = px_all_wait(smem_u32(p_full), (uint32_t)t & 1u, abort_flag, 144))) break;
+            if ((bad = at_all_wait(smem_u32(p_full), (uint32_t)t & 1u, abort_flag, 144))) break;
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
@@ -556,7 +539,7 @@ __global__ void __launch_bounds__(PT_T, 3) k_px_tc(const __grid_constant__ PxTcP
             }
             __syncwarp();
         }
-        px_give_up(bad, abort_flag, p.errword);
+        at_give_up(bad, abort_flag, p.errword);
         if (*abort_flag) {                    // copies and MMAs under way end (bounded) before memory is given back
             for (int i = issued > PT_NS ? issued - PT_NS : 0; i < issued; i++)
                 for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(&kv_full[i % PT_NS]), (uint32_t)(i / PT_NS) & 1u); k++) {}
@@ -587,7 +570,7 @@ __global__ void __launch_bounds__(PT_T, 3) k_px_tc(const __grid_constant__ PxTcP
         float m = -3e38f, l = 0.0f;
         int bad = 0;
         for (int t = 0; t < nt; t++) {
-            if ((bad = px_all_wait(smem_u32(s_full), (uint32_t)t & 1u, abort_flag, 145))) break;
+            if ((bad = at_all_wait(smem_u32(s_full), (uint32_t)t & 1u, abort_flag, 145))) break;
             if (warp_live) {
                 tc_fence_after();
                 uint32_t v[64];
@@ -648,8 +631,8 @@ __global__ void __launch_bounds__(PT_T, 3) k_px_tc(const __grid_constant__ PxTcP
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(p_full));
         }
-        if (!bad) bad = px_all_wait(smem_u32(o_full), (uint32_t)(nt - 1) & 1u, abort_flag, 146);
-        px_give_up(bad, abort_flag, p.errword);
+        if (!bad) bad = at_all_wait(smem_u32(o_full), (uint32_t)(nt - 1) & 1u, abort_flag, 146);
+        at_give_up(bad, abort_flag, p.errword);
         if (!bad && warp_live) {
             tc_fence_after();
             const bool some = live && l != 0.0f;        // l = 0: every score -inf; the join does not read such a piece

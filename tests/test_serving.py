@@ -602,6 +602,7 @@ LORA = [
     (1, 8, 8, 8, 1), (1, 768, 768, 8, 4), (3, 72, 136, 16, 2), (16, 64, 64, 64, 1), (17, 256, 512, 24, 5), (64, 768, 1536, 16, 64), (64, 1000, 200, 72, 7), (130, 512, 768, 256, 3),
     (333, 384, 264, 32, 10), (1000, 768, 768, 8, 40), (2, 4096, 16384, 16, 2), (70, 40, 1032, 40, 3),
     (2049, 72, 136, 8, 3), (2500, 768, 264, 64, 9), (2300, 256, 520, 136, 5), (4097, 512, 768, 16, 200), (257, 1024, 128, 64, 3),
+    (600, 72, 136, 16, 3), (2304, 768, 520, 256, 4), (700, 64, 64, 32, 2), (5000, 136, 72, 48, 20), (512, 1024, 1544, 112, 1), (2180, 4104, 8, 16, 2),
 ]
 
 
@@ -644,6 +645,34 @@ def test_lora_keeps_one_adapters_infinities_from_other_rows(cuda):
     assert bool(torch.isfinite(y[clean].float()).all()) and not bool(torch.isfinite(y[adapter == 2].float()).any())
     fixed = torch.where(clean, adapter, torch.full_like(adapter, -1))
     check_lora(torch.where(clean[:, None], y, base), X, base, A, Bm, scale, fixed)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("place", ["new", "in place"])
+def test_lora_of_many_rows_keeps_adapters_apart(cuda, place):
+    """Tiles with several adapters, with rows without one and with an adapter out of range: an adapter's infinities stay with its rows,
+    a row whose adapter is no adapter keeps its base and is reported."""
+    from cudalm_c_b200 import linear
+    X, base, A, Bm, scale = make_lora(1300, 256, 320, 32, 5, torch.bfloat16, 4, cuda)
+    adapter = torch.full((1300,), 3, device=cuda, dtype=torch.int32)
+    adapter[100:300] = 1
+    adapter[300:310] = torch.arange(10, device=cuda, dtype=torch.int32) % 5
+    adapter[310:700] = -1
+    adapter[900:1000] = 0
+    adapter[1000:1024] = 2
+    adapter[1030], adapter[1299] = 5, -2
+    A[2, 3], Bm[2, 5], X[120] = math.nan, math.inf, math.inf
+    out = base.clone() if place == "in place" else None
+    b = out if out is not None else base
+    y = linear.lora_add(X, b, A, Bm, scale, adapter, out=out)
+    assert b"error code 201 (site 307" in ok(4)
+    fixed = adapter.clone()
+    fixed[1030], fixed[1299] = -1, -1
+    odd = adapter == 2
+    odd[120] = True
+    assert not bool(torch.isfinite(y[odd].float()).any()) and bool(torch.isfinite(y[~odd].float()).all())
+    fixed[odd] = -1
+    check_lora(torch.where(odd[:, None], base, y), X, base, A, Bm, scale, fixed)
 
 
 @pytest.mark.gpu
