@@ -42,15 +42,20 @@ __device__ __forceinline__ bool at_wait(uint32_t bar, uint32_t parity, volatile 
     }
     return false;
 }
-constexpr uint32_t AT_TRIES = 1u << 20;                     // a warp's wait gives up after so many
-// A warp's wait: all of its lanes go on (0), or none (the site).  Bounded like the library's other waits.  try_wait lets the hardware
-// hold the warp until the phase ends or a time of its own is over: a loop of test_wait instead keeps the queue busy that the
-// exponentials go through, too.
+// A warp's wait: all of its lanes go on (0), or none (the site).  Bounded like at_wait, by a second of the clock's lower half.  try_wait lets
+// the hardware hold the warp until the phase ends or a time of its own is over: a loop of test_wait instead keeps the queue busy that
+// the exponentials go through, too.
+__device__ __forceinline__ uint32_t at_now_lo() { uint32_t t; asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t)); return t; }
 __device__ __forceinline__ int at_all_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int site)
 {
+    uint32_t t0 = 0;
 #pragma unroll 1
     for (uint32_t i = 0; !__all_sync(~0u, mbar_try(bar, parity)); i++)
-        if ((i & 255u) == 255u && (*abort_flag || i > AT_TRIES)) return site;
+        if ((i & 63u) == 63u) {
+            const uint32_t now = __shfl_sync(~0u, at_now_lo(), 0);
+            if (i == 63u) t0 = now;
+            if (__any_sync(~0u, *abort_flag) || now - t0 > (uint32_t)AT_WAIT_NS) return site;
+        }
     return 0;
 }
 __device__ __forceinline__ void at_give_up(int site, volatile int *abort_flag, int *errword)

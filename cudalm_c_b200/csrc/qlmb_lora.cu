@@ -1084,13 +1084,17 @@ static LoraForm lora_form(int M, int K, int N, int R, int *S, int *kslice)
 }
 
 // TC: bf16 rows that stand in their order, ranks of whole 16 (a tile of D and of B has no rows of the next adapter then), counts that fit
-// 32 bits.  Us with it and without (M / adapters): K 768, N 1536, R 64: 512 / 8 11.0 and 14.8, 1024 / 4 9.9 and 17.8, 2048 / 8 12.0 and 22.1,
-// 8192 / 9 22.6 and 32.7, 32768 / 9 57.7 and 91.7; R 256: 8192 / 3 29 and 127; K 768, N 768, R 16: 512 / 1 8.2 and 7.9, 1024 / 8 9.2 and 10.3,
-// 8192 / 9 14.4 and 21.2.  Every CTA makes the inner numbers of its pairs for itself, which few rows do not pay for where K is large:
-// K 4096, N 4096: R 16 512 / 4 39 and 15, R 32 1024 / 64 57 and 53, 8192 / 9 61 and 91.
+// 32 bits.  Us with it and without, rows in runs (M / adapters): K 768, N 1536, R 64: 512 / 8 11.0 and 14.8, 1024 / 4 9.9 and 17.8, 2048 / 8
+// 12.0 and 22.1, 8192 / 9 22.6 and 32.7, 32768 / 9 57.7 and 91.7; R 256: 8192 / 3 29 and 127; K 768, N 768, R 16: 512 / 1 8.2 and 7.9, 1024 / 8
+// 9.2 and 10.3, 8192 / 9 14.4 and 21.2.  Up to 2048 rows LORA_TWO's tiles of 16 are the better ones
+//   where K is large, since every CTA makes the inner numbers of its pairs for itself: K 4096, N 4096: R 16 512 / 4 39 and 15, R 32 1024 / 64
+//   57 and 53 (8192 / 9 61 and 91);
+//   where rows come in no order with many adapters, or a small rank: K 768, N 1536, R 64: 512 / 8 14.6 and 21.6, 1024 / 16 28.9 and 39.4,
+//   1024 / 32 47.9 and 44.7; K 768, N 768, R 16: 512 / 16 22.9 and 9.6, 512 / 64 67 and 9.3 (above 2048 the tiles of 64 are no better: K 768,
+//   N 1536, R 64: 4096 / 64 255 and 581).
 static bool lora_tc_ok(int M, int K, int N, int R, int adapters)
 {
-    return R % 16 == 0 && (M > 2048 || (M >= 512 && K <= 1024)) && (M + 127) / 128 <= LC_TILES && (long long)M * ((N + 63) / 64) < (1LL << 31) &&
+    return R % 16 == 0 && (M > 2048 || (M >= 512 && K <= 1024 && R >= 32 && adapters <= 16)) && (M + 127) / 128 <= LC_TILES && (long long)M * ((N + 63) / 64) < (1LL << 31) &&
            (long long)adapters * R < (1LL << 31);
 }
 
@@ -1189,6 +1193,7 @@ extern "C" int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype
     QLMB_REQUIRE(dtype == QLMB_F32 || dtype == QLMB_BF16, "qlmb_lora_add: rows of type %d", dtype);
     if (M <= 0) return QLMB_OK;
     QLMB_REQUIRE(lora_shape_ok(M, K, N, R) && adapters > 0, "qlmb_lora_add: M %d, K %d and N %d (multiples of 8), rank %d (a multiple of 8 up to 256), %d adapters", M, K, N, R, adapters);
+    QLMB_REQUIRE(Y != X, "qlmb_lora_add: Y is X (it may be the base)");
     QLMB_REQUIRE((((uintptr_t)Y | (uintptr_t)X | (uintptr_t)base | (uintptr_t)A | (uintptr_t)Bm | (uintptr_t)ws) & 15) == 0, "qlmb_lora_add: rows, adapters and workspace must be 16-byte aligned");
     const size_t need = qlmb_lora_bytes(M, K, N, R);
     QLMB_REQUIRE(need <= 16 || (ws && ws_bytes >= need), "qlmb_lora_add: a workspace of %zu bytes, %zu are needed", ws_bytes, need);

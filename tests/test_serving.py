@@ -33,7 +33,7 @@ def test_refusals_of_the_entry_points():
     def verify(out=one, dt=0, ld=16, q=one, ldq=16, draft=one, n=2, V=16):
         return L.qlmb_dec_verify(out, one, one, one, dt, ld, q, ldq, draft, None, one, one, 1, n, V, None)
 
-    def lora(Y=one, X=one, dt=1, n=2, M=4, K=64, N=64, R=8, ws=one, nbytes=big):
+    def lora(Y=ctypes.c_void_p(8192), X=one, dt=1, n=2, M=4, K=64, N=64, R=8, ws=one, nbytes=big):
         return L.qlmb_lora_add(Y, X, one, dt, one, one, one, n, one, None, M, K, N, R, ws, nbytes, None)
 
     cases = [
@@ -47,7 +47,7 @@ def test_refusals_of_the_entry_points():
         (lambda: verify(n=64), b"n 64"), (lambda: verify(V=0), b"V 0"), (lambda: verify(ld=15), b"rows of 15"), (lambda: verify(ldq=15), b"and 15"),
         (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None, K=8192), b"workspace"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
         (lambda: lora(K=60), b"multiples of 8"), (lambda: lora(N=63), b"multiples of 8"), (lambda: lora(R=12), b"rank 12"), (lambda: lora(R=264), b"rank 264"),
-        (lambda: lora(R=0), b"rank 0"), (lambda: lora(X=odd), b"aligned"), (lambda: lora(K=8192, nbytes=ctypes.c_size_t(4)), b"workspace of 4 bytes"),
+        (lambda: lora(R=0), b"rank 0"), (lambda: lora(Y=ctypes.c_void_p(8192), X=ctypes.c_void_p(8192)), b"Y is X"), (lambda: lora(Y=ctypes.c_void_p(8192), X=odd), b"aligned"), (lambda: lora(K=8192, nbytes=ctypes.c_size_t(4)), b"workspace of 4 bytes"),
     ]
     for i, (call, needle) in enumerate(cases):
         assert call() == 1, i
@@ -333,6 +333,20 @@ def test_attention_of_many_rows_at_its_borders(cuda):
     assert not bool(torch.isfinite(o[:n, 0, :, 5]).any())  # (queries of 0: every weight is the same)
     o[:, 0, :, 5] = 0                                      # elsewhere 0 * inf where the weight has gone to 0: no number, either
     assert bool(torch.isfinite(o).all())
+
+
+@pytest.mark.gpu
+def test_attention_of_slots_that_see_nothing(cuda):
+    """No prefix and pos = -1: the first token sees nothing at all (zeros, -inf), the next one only itself."""
+    from cudalm_c_b200 import attn
+    for n in (1, 2):
+        q, kp, vp, kc, vc = make_attn(3, n, 4, 2, 0, 9, 3, cuda)
+        pos = torch.tensor([-1, 2, -1], dtype=torch.int32, device=cuda)
+        for win in (0, 2):
+            o, lse = attn.dec_attn_prefix(q, kp, vp, kc, vc, pos, 4, win=win)
+            ok()
+            check_attn(o, lse, attn64(q, kp, vp, kc, vc, pos, 4, win))
+            assert bool((o[0] == 0).all()) and bool((lse[0] == -math.inf).all()) and bool(torch.isfinite(lse[n:2 * n]).all())
 
 
 @pytest.mark.gpu
