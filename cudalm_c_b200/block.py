@@ -185,7 +185,7 @@ def dec_verify(logits, draft, u, temp, q=None, nd=None, V=None):
         _dec_verify_args(logits, draft, u, temp, q, nd, V)
     B, n1, ld, n = got[:4]
     ldq = got[4] if q is not None else 0
-    out = draft.new_empty((B, n1))
+    out = torch.empty_like(u, dtype=torch.int32)
     count = draft.new_empty(B)
     lp = torch.empty_like(u)
     calls.dec_verify(out, count, lp, logits, F32 if dt is torch.float32 else BF16, ld, q if n else None, ldq, draft if n else None, nd, u, temp,

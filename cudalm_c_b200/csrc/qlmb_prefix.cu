@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 //
 // Measured (12 heads, 12 kv heads unless stated; graph of calls, all launches): 1 slot after 512 keys 9.2 us, 8 slots of 4 tokens after
 // 2048 10.9 us (both the length of three small launches), 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
-// 16 heads of 4 kv heads after 32768 95 us.  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of
+// 16 heads of 4 kv heads after 32768 91 us (96 where k_px_mma waits for k_px_tc's end).  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of
 // the special-function units; without them it takes 60 us, without any softmax 41 us, which is what its MMAs of 64 columns need.
 constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
 constexpr int PX_MAXB = 1024;                             // slots: every CTA keeps their positions and block counts
@@ -131,6 +131,7 @@ __device__ __forceinline__ int px_div(int x, int d)
 }
 // a place in the row of all blocks: item `sub` of slot b (b = B: of the shared keys), the block's first key, the item's last
 struct PxCursor { int b, sub, key, last; };
+__device__ __forceinline__ int px_ldcg(const int *p) { int v; asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory"); return v; }
 
 __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_constant__ PxParams p)
 {
@@ -153,13 +154,15 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
         fence_barrier_init();
     }
     pdl_trigger();
-    pdl_wait();
+    // Behind k_px_tc, which has waited before it let this kernel start and writes nothing that is read here, the wait comes last: SMs that
+    // have no CTA of k_px_tc left begin with the slots' own keys.  (Reads pass by L1: copies, and the positions.)
+    if (!p.Sp) pdl_wait();
     const int KT = p.KV * p.t_own;
     // ---- the slots' block counts, added up by the first warp
     if (warp == 0) {
         int carry = 0, first = 0x7fffffff;
         for (int b0 = 0; b0 < p.B; b0 += 32) {
-            const int b = b0 + lane, t0 = b < p.B ? p.pos[b] : 0, v = b < p.B ? px_blocks(p, t0) : 0;
+            const int b = b0 + lane, t0 = b < p.B ? px_ldcg(p.pos + b) : 0, v = b < p.B ? px_blocks(p, t0) : 0;
             int x = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(~0u, x, o); if (lane >= o) x += y; }
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
     }
     const unsigned me = blockIdx.x * PX_WARPS + warp;
     const unsigned from = me * per;                       // (the warps' number times per is little more than total: no overflow)
-    if (from >= total) return;
+    if (from >= total) { if (p.Sp) pdl_wait(); return; }
     int count = (int)min(per, total - from);              // blocks of this warp
     // ---- the first of them
     const auto open = [&](PxCursor &c, int blk) {         // block blk of item (b, sub)
@@ -430,6 +433,7 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
     if (*abort_flag)                                      // aborting: the copies under way must land before the CTA gives its shared memory back
         for (int i = 0; i < 2; i++)
             for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(bar + i), i < stage ? phase ^ 1u : phase); k++) {}
+    if (p.Sp) pdl_wait();
 }
 
 // ------------------------------------------------------------------ the shared keys of many rows
@@ -746,9 +750,10 @@ static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
     PxPlan pl = {};
     const long long rows = (long long)B * n * (H / KV);
     // k_px_tc is a launch more, and as long for 16 rows as for 128; k_px_mma's warps take a block of 16 rows and 32 keys at a time.
-    // Whole calls, k_px_mma alone and with k_px_tc, by blocks: 6144 (64 rows, 12 kv heads) 20.0 and 22.7 us, 10240 (320 rows, 4) 22.6
-    // and 26.8, 12800 (1280 rows, 4) 24.5 and 24.3, 12288 (64 rows, 12) 26.0 and 27.7, 20480 (320, 4) 35 and 29, 24576 (16 rows, 12) 58
-    // and 47, (32 rows, 12) 45 and 33, 49152 (one row, 12) 100 and 73.  k_px_tc has no window.
+    // Whole calls, k_px_mma alone and with k_px_tc, by blocks, slots with 64 keys of their own: 6144 (64 rows, 12 kv heads) 20.2 and 21.4 us,
+    // 10240 (320 rows, 4) 22.9 and 22.7, 12288 (64 rows, 12) 26.1 and 25.1, 12800 (1280 rows, 4) 24.8 and 22.9, 15360 (320, 4) 29.6 and 23.7,
+    // 24576 (16 rows, 12) 58 and 47, 49152 (one row, 12) 100 and 73; with 1000, which k_px_mma takes along: 10240 (320, 4) 21.6 and 27.8,
+    // 12288 (64, 12) 47.8 and 50.7, 15360 (320, 4) 25.5 and 29.1, 16384 (128, 4) 24.4 and 27.0.  k_px_tc has no window.
     const bool tc = P > 0 && win <= 0 && KV * ((rows + 15) / 16) * ((P + 31) / 32) > 12288;
     pl.t_own = (n * (H / KV) + 15) / 16;
     pl.t_pre = P > 0 && !tc ? (int)((rows + 15) / 16) : 0;
