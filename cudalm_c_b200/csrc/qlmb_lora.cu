@@ -1059,10 +1059,10 @@ template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora
 }
 
 // Which form, and the slices of K of LORA_TWO.  Us, on both sides of each border (bf16, M rows on so many adapters):
-//   TILE (what TC does not take) above 2048 rows
-//                             K 768, N 1536, R 64: 2048 / 8 rows 19.6 as tiles, 22.3 as places; 8192 / 9 32.7 and 81.6
-//                             K 768, N 768, R 16: 2048 / 8 14.7 and 13.1, 8192 / 9 22.2 and 30.0; K 4096, N 4096, R 32: 1024 / 64
-//                             (runs of 16) 135 and 52, 8192 / 9 84 and 174
+//   TILE (what TC does not take) above 2048 rows, of ranks up to 16 above 8192.  R 64: K 768, N 1536, rows in no order on 9 4096 24.0 as tiles
+//                             and 41.2 as places, on 64 8192 52.3 and 82.8; K 2048, N 2048 on 64 4096 72.6 and 77.2; fp32, K 520, N 3664, 2660 / 8
+//                             55.7 and 52.6.  fp32, R 16: K 3328, N 848, 2256 / 2 97.2 and 20.3; K 1024, N 1024, 8192 / 9 44.0 and 41.5;
+//                             K 4096, N 4096 8192 / 9 162 and 101; K 2048, N 2048, 16384 / 9 109 and 126
 //   ONE up to 256 rows, K R of 32768 and N of 2048 (or M N of 32768), where making the inner numbers once per 512 columns costs less
 //                             than a launch.  K 768, N 768, R 16: 64 rows 4.8 instead of 6.2, 256 / 64 7.2 and 9.7, 512 / 64 10.5 and
 //                             9.7; K 2048, N 2048, R 16: 64 / 64 7.2 and 8.1; K 768, N 4096, R 16: 8 / 8 4.5 and 5.5, 64 / 64 10.4 and
@@ -1072,7 +1072,7 @@ enum LoraForm { LORA_ONE, LORA_TWO, LORA_TILE, LORA_TC };
 static LoraForm lora_form(int M, int K, int N, int R, int *S, int *kslice)
 {
     *kslice = K; *S = 0;
-    if (M > 2048) return LORA_TILE;
+    if (M > 8192 || (M > 2048 && R > 16)) return LORA_TILE;
     if (M <= 256 && R <= 64 && (long long)K * R <= 32768 && (N <= 2048 || (long long)M * N <= 32768)) return LORA_ONE;
     long long s = (4LL * sm_count() + M - 1) / M;
     const long long most = (K + 511) / 512;              // four warps with four steps of 32 each

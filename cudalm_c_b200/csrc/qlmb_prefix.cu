@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 // k_px_mma: see px_plan.
 //
 // Measured (12 heads, 12 kv heads unless stated; graph of calls, all launches): 1 slot after 512 keys 9.2 us, 8 slots of 4 tokens after
-// 2048 10.9 us (both the length of three small launches), 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
+// 2048 10.9 us (both the length of two small launches), 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
 // 16 heads of 4 kv heads after 32768 91 us (96 where k_px_mma waits for k_px_tc's end).  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of
 // the special-function units; without them it takes 60 us, without any softmax 41 us, which is what its MMAs of 64 columns need.
 constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
@@ -753,9 +753,11 @@ static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
     // Whole calls, k_px_mma alone and with k_px_tc, by blocks, slots with 64 keys of their own: 6144 (64 rows, 12 kv heads) 20.2 and 21.4 us,
     // 10240 (320 rows, 4) 22.9 and 22.7, 12288 (64 rows, 12) 26.1 and 25.1, 12800 (1280 rows, 4) 24.8 and 22.9, 15360 (320, 4) 29.6 and 23.7,
     // 24576 (16 rows, 12) 58 and 47, 49152 (one row, 12) 100 and 73; with 1000, which k_px_mma takes along: 10240 (320, 4) 21.6 and 27.8,
-    // 12288 (64, 12) 47.8 and 50.7, 15360 (320, 4) 25.5 and 29.1, 16384 (128, 4) 24.4 and 27.0.  k_px_tc has no window.
-    const bool tc = P > 0 && win <= 0 && KV * ((rows + 15) / 16) * ((P + 31) / 32) > 12288;
+    // 12288 (64, 12) 47.8 and 50.7, 15360 (320, 4) 25.5 and 29.1, 16384 (128, 4) 24.4 and 27.0.  So the border moves with what the slots' caches
+    // can hold (10560 blocks, 480 rows, 2 kv heads, caches of 36 rows: 27.5 and 22.6).  k_px_tc has no window.
     pl.t_own = (n * (H / KV) + 15) / 16;
+    const long long most_own = (long long)B * KV * pl.t_own * (Tm / 32 + 1);         // if the slots' caches are full
+    const bool tc = P > 0 && win <= 0 && KV * ((rows + 15) / 16) * ((P + 31) / 32) > 8704 + (most_own < 4096 ? most_own : 4096);
     pl.t_pre = P > 0 && !tc ? (int)((rows + 15) / 16) : 0;
     pl.warps = sm_count() * PX_WARPS;
     if (tc) {

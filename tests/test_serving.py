@@ -208,7 +208,7 @@ SHAPES = [
     (8, 4, 12, 12, 300, 200, 0), (2, 3, 8, 1, 129, 40, 0), (7, 5, 16, 4, 1000, 130, 0), (64, 1, 12, 12, 640, 96, 0), (33, 5, 8, 2, 515, 64, 0), (1, 64, 8, 2, 257, 80, 0),
     (2, 16, 32, 2, 60, 100, 0), (4, 1, 2, 2, 4097, 20, 0), (1, 1, 2, 2, 3, 5000, 0), (16, 8, 8, 8, 0, 300, 0), (70, 3, 4, 4, 200, 30, 0), (1, 5, 1, 1, 20000, 9, 0),
     # shared keys of many rows (or very many of one) have a kernel of their own, joins of many rows and windows theirs
-    (16, 5, 16, 4, 5003, 40, 0), (13, 5, 8, 8, 9857, 20, 0), (1, 1, 12, 12, 33003, 20, 0), (3, 64, 8, 2, 16448, 80, 0), (64, 5, 16, 4, 1217, 50, 0), (16, 5, 16, 4, 5003, 40, 4000),
+    (16, 5, 16, 4, 5003, 40, 0), (13, 5, 8, 8, 9857, 20, 0), (1, 1, 12, 12, 33003, 20, 0), (3, 64, 8, 2, 16448, 80, 0), (12, 5, 16, 2, 4800, 36, 0), (64, 5, 16, 4, 1217, 50, 0), (16, 5, 16, 4, 5003, 40, 4000),
     (300, 2, 4, 2, 40, 9, 0), (1024, 1, 2, 2, 40, 6, 0), (1024, 1, 1, 1, 13000, 3, 0),
     (3, 2, 4, 2, 100, 50, 1), (3, 4, 4, 2, 100, 50, 20), (6, 3, 2, 2, 400, 300, 128), (20, 5, 8, 2, 300, 64, 100), (2, 1, 2, 1, 64, 64, 2 ** 31 - 1), (9, 7, 3, 3, 5, 70, 33),
 ]
@@ -616,7 +616,7 @@ LORA = [
     (1, 8, 8, 8, 1), (1, 768, 768, 8, 4), (3, 72, 136, 16, 2), (16, 64, 64, 64, 1), (17, 256, 512, 24, 5), (64, 768, 1536, 16, 64), (64, 1000, 200, 72, 7), (130, 512, 768, 256, 3),
     (333, 384, 264, 32, 10), (1000, 768, 768, 8, 40), (2, 4096, 16384, 16, 2), (70, 40, 1032, 40, 3),
     (2049, 72, 136, 8, 3), (2500, 768, 264, 64, 9), (2300, 256, 520, 136, 5), (4097, 512, 768, 16, 200), (257, 1024, 128, 64, 3),
-    (600, 72, 136, 16, 3), (2304, 768, 520, 256, 4), (700, 64, 64, 32, 2), (5000, 136, 72, 48, 20), (512, 1024, 1544, 112, 1), (2180, 4104, 8, 16, 2),
+    (2049, 72, 136, 24, 3), (8200, 40, 136, 8, 3), (2100, 1032, 72, 16, 5), (600, 72, 136, 16, 3), (2304, 768, 520, 256, 4), (700, 64, 64, 32, 2), (5000, 136, 72, 48, 20), (512, 1024, 1544, 112, 1), (2180, 4104, 8, 16, 2),
 ]
 
 
