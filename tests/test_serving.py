@@ -804,3 +804,47 @@ def test_the_mirrors_look_at_their_arguments():
         calls.sizes()
     with pytest.raises(TypeError):
         calls.sizes("x", f, "ab")
+
+
+@pytest.mark.gpu
+def test_the_large_forms_on_two_streams(cuda):
+    """The tensor-core kernels (512 columns of tensor memory a CTA, 128 a CTA three times an SM), clusters and rings beside one another on two
+    streams, eager and captured: results bit for bit those of calls one after the other."""
+    from cudalm_c_b200 import attn, block, linear
+    at = make_attn(16, 5, 16, 4, 5003, 40, 51, cuda)
+    pos = positions(16, 5, 5003, 40, 52, cuda)
+    big = make_lora(2500, 768, 264, 16, 5, torch.bfloat16, 53, cuda)
+    wide = make_lora(2300, 256, 520, 128, 3, torch.float32, 54, cuda)
+    few = make_lora(40, 4096, 2048, 16, 40, torch.bfloat16, 55, cuda)
+    a_big = (torch.arange(2500, device=cuda, dtype=torch.int32) // 300) % 6 - 1
+    a_wide = (torch.arange(2300, device=cuda, dtype=torch.int32) // 37) % 3
+    a_few = torch.arange(40, device=cuda, dtype=torch.int32)
+    lg, x, u, temp, q = make_verify(3, 4, 40001, 40001, torch.float32, True, 56, cuda)
+    ops = [lambda: attn.dec_attn_prefix(at[0], at[1], at[2], at[3], at[4], pos, 16), lambda: (linear.lora_add(*big, a_big),), lambda: (linear.lora_add(*wide, a_wide),),
+           lambda: (linear.lora_add(*few, a_few),), lambda: block.dec_verify(lg, x, u, temp, q=q)]
+    want = [f() for f in ops]
+    ok()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append([f() for f in (ops if k == 0 else ops[::-1])])
+    ok()
+    for k in range(2):
+        for step in got[k]:
+            for a, b in zip(step if k == 0 else step[::-1], want):
+                assert all(torch.equal(p, r) for p, r in zip(a, b))
+    graphs = []
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got[k] = [f() for f in (ops if k == 0 else ops[::-1])]
+        graphs.append(g)
+    for _ in range(6):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    ok()
+    for k in range(2):
+        for a, b in zip(got[k] if k == 0 else got[k][::-1], want):
+            assert all(torch.equal(p, r) for p, r in zip(a, b))
