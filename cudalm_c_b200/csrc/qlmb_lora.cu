@@ -857,13 +857,13 @@ template <bool F32, int NT, int UK> __global__ void __launch_bounds__(128) k_lor
 // k_lora_up starts while k_lora_down runs and requests what that does not write ahead of its wait: the rows' places, their base and
 // B.  A place with one or two rows is multiplied by plain instructions, a lane having LC neighbouring columns: on tensor cores 14 or
 // 15 rows of 16 would be nobody's, and the instructions around them bound it (64 rows on 64 adapters, K 4096, N 16384, R 16: 14.8 us
-// instead of 16.2).  One with more goes through the tensor cores, the base in shared memory, and (AHEAD, R <= 16) B for all of a warp's
+// instead of 16.2).  One with more goes through the tensor cores, the base in shared memory, and (NARROW, R <= 16) B for all of a warp's
 // blocks of 64 columns requested first.  Now 17.3 us both launches (k_lora_down 8.7, k_lora_up 11.4 by themselves; 46 MB, 2.7 TB/s); a
 // CTA a place and 1024 columns, which was two waves, 20.4; rings of copies a warp or a CTA with tensor cores only 24.7 and 27.3.
 constexpr int LR_FEW = 2;
-template <bool F32, bool AHEAD> constexpr int lr_cols() { return AHEAD && !F32 ? 1024 : 512; }        // columns of a CTA
-template <bool F32, bool AHEAD> constexpr int lr_pitch() { return lr_cols<F32, AHEAD>() * (F32 ? 4 : 2) + 16; }       // bytes of a row of the base
-template <bool F32, bool AHEAD> static size_t lr_smem(int R) { return 16 * (size_t)lr_pitch<F32, AHEAD>() + (size_t)(F32 ? 3 : 2) * 16 * ((R + 15) / 16 * 8 + 4) * sizeof(uint32_t); }
+template <bool F32, bool NARROW> constexpr int lr_cols() { return NARROW && !F32 ? 1024 : 512; }        // columns of a CTA
+template <bool F32, bool NARROW> constexpr int lr_pitch() { return lr_cols<F32, NARROW>() * (F32 ? 4 : 2) + 16; }       // bytes of a row of the base
+template <bool F32, bool NARROW> static size_t lr_smem(int R) { return 16 * (size_t)lr_pitch<F32, NARROW>() + (size_t)(F32 ? 3 : 2) * 16 * ((R + 15) / 16 * 8 + 4) * sizeof(uint32_t); }
 
 // A lane's LC columns of bf16 (LC = 8 or 4) as they lie, and of the rows
 template <int LC> struct LrVec { uint32_t w[LC / 2]; };
@@ -973,13 +973,14 @@ template <bool F32, int LC> __device__ __forceinline__ void lr_few(const LoraPar
         }
     }
 }
-template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora_up(const __grid_constant__ LoraParams p)
+template <bool F32, bool NARROW, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora_up(const __grid_constant__ LoraParams p)
 {
-    constexpr int TT = F32 ? 3 : 2, EB = F32 ? 4 : 2, UP = lr_cols<F32, AHEAD>(), NB = UP / 256, PITCH = lr_pitch<F32, AHEAD>(), PIECES = UP * EB / 16;
+    constexpr int TT = F32 ? 3 : 2, EB = F32 ? 4 : 2, UP = lr_cols<F32, NARROW>(), NB = UP / 256, PITCH = lr_pitch<F32, NARROW>(), PIECES = UP * EB / 16;
     extern __shared__ __align__(16) uint8_t lr_s[];
     uint32_t *ts = reinterpret_cast<uint32_t *>(lr_s + 16 * PITCH);       // [term][16][ldt] pairs of bf16
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, ldt = (p.R + 15) / 16 * 8 + 4;
     pdl_trigger();
+    if (!AHEAD) pdl_wait();
     const int j0 = (int)blockIdx.x / 16 * 16;
     int m, a;
     lr_row(p, j0 + (lane & 15), m, a, false);
@@ -989,8 +990,8 @@ template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora
     const int blocks = (p.N + UP - 1) / UP, total = __popc(work) * blocks, shares = 16 * gridDim.y, me = blockIdx.x % 16 * gridDim.y + blockIdx.y;
     const int u1 = (int)((long long)total * (me + 1) / shares);
     int u = (int)((long long)total * me / shares);
-    if (u == u1) { pdl_wait(); return; }
-    for (bool wait = true; u < u1; wait = false) {
+    if (u == u1) { if (AHEAD) pdl_wait(); return; }
+    for (bool wait = AHEAD; u < u1; wait = false) {
         unsigned w = work;
         for (int k = u / blocks; k; k--) w &= w - 1;
         const int place = __ffs(w) - 1, b0 = u % blocks, b1 = min(blocks, b0 + u1 - u);
@@ -999,11 +1000,11 @@ template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora
         const unsigned mine = __ballot_sync(~0u, m >= 0 && a == cur) & 0xffffu;
         if (__popc(mine) <= LR_FEW) { lr_few<F32, UP / 128>(p, reinterpret_cast<float *>(lr_s), j0, cur, mine, m, b0, b1, wait); continue; }
         if (!wait) __syncthreads();               // the place before this one is done with the shared memory
-        uint4 b[AHEAD ? NB : 1][4];
+        uint4 b[NARROW ? NB : 1][4];
         const auto ask = [&](int c0) {            // B and the base of the CTA's columns
-            if (AHEAD)
+            if (NARROW)
 #pragma unroll
-                for (int i = 0; i < NB; i++) lr_up_b<true>(p, cur, c0 + 256 * i + 64 * warp, 0, b[AHEAD ? i : 0]);
+                for (int i = 0; i < NB; i++) lr_up_b<true>(p, cur, c0 + 256 * i + 64 * warp, 0, b[NARROW ? i : 0]);
             for (int i = threadIdx.x; i < 16 * PIECES; i += 128) {
                 const int r = i / PIECES, n = c0 + i % PIECES * (16 / EB), row = __shfl_sync(~0u, m, r);     // r: the warp's
                 if ((mine >> r & 1) && n < p.N) lt_copy(lt_addr(lr_s + r * PITCH + i % PIECES * 16), reinterpret_cast<const uint8_t *>(p.base) + ((size_t)row * p.N + n) * EB, true);
@@ -1038,7 +1039,7 @@ template <bool F32, bool AHEAD> __global__ void __launch_bounds__(128, 4) k_lora
                 if (n0 >= p.N) break;
                 float c[8][4] = {};
                 if (cur >= 0) {
-                    if (AHEAD) lr_up_mul<F32>(p, c, b[AHEAD ? i : 0], ts + g * ldt, ldt, 0);
+                    if (NARROW) lr_up_mul<F32>(p, c, b[NARROW ? i : 0], ts + g * ldt, ldt, 0);
                     else lr_up<F32>(p, c, ts + g * ldt, ldt, cur, n0);
                 }
                 uint4 base[2][2][F32 ? 2 : 1];
@@ -1176,13 +1177,17 @@ template <bool F32> static int lora_launch(const LoraParams &p, LoraForm form, c
     QLMB_CUDA(cudaGetDevice(&dev));
     QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
     if (!configured_dev[dev]) {
-        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, true>(16)));
-        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, false>(256)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, true>(16)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, true>(16)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, false>(256)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, false>(256)));
         configured_dev[dev] = true;
     }
     QLMB_CUDA(pdl_launch_small(narrow ? k_lora_down<F32, 2, 4> : k_lora_down<F32, LR_RT / 8, 1>, gd, dim3(128), 0, st, p));
     QLMB_LAUNCH_CHECK("k_lora_down");
-    QLMB_CUDA(pdl_launch(true, narrow ? k_lora_up<F32, true> : k_lora_up<F32, false>, gu, dim3(128), narrow ? lr_smem<F32, true>(p.R) : lr_smem<F32, false>(p.R), st, p));
+    // behind k_lora_down, which waits before it lets this launch start (without early launches there is nothing to be ahead of)
+    void (*up)(const LoraParams) = pdl_enabled() ? (narrow ? k_lora_up<F32, true, true> : k_lora_up<F32, false, true>) : (narrow ? k_lora_up<F32, true, false> : k_lora_up<F32, false, false>);
+    QLMB_CUDA(pdl_launch(true, up, gu, dim3(128), narrow ? lr_smem<F32, true>(p.R) : lr_smem<F32, false>(p.R), st, p));
     QLMB_LAUNCH_CHECK("k_lora_up");
     return QLMB_OK;
 }

@@ -133,7 +133,7 @@ __device__ __forceinline__ int px_div(int x, int d)
 struct PxCursor { int b, sub, key, last; };
 __device__ __forceinline__ int px_ldcg(const int *p) { int v; asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory"); return v; }
 
-__global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_constant__ PxParams p)
+template <bool AHEAD> __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_constant__ PxParams p)
 {
     extern __shared__ __align__(1024) uint8_t px_s[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(px_s + PX_RINGS);                       // a ring's stages are full
@@ -154,9 +154,9 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
         fence_barrier_init();
     }
     pdl_trigger();
-    // Behind k_px_tc, which has waited before it let this kernel start and writes nothing that is read here, the wait comes last: SMs that
+    // AHEAD: behind k_px_tc, which has waited before it let this kernel start and writes nothing that is read here, the wait comes last: SMs that
     // have no CTA of k_px_tc left begin with the slots' own keys.  (Reads pass by L1: copies, and the positions.)
-    if (!p.Sp) pdl_wait();
+    if (!AHEAD) pdl_wait();
     const int KT = p.KV * p.t_own;
     // ---- the slots' block counts, added up by the first warp
     if (warp == 0) {
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
     }
     const unsigned me = blockIdx.x * PX_WARPS + warp;
     const unsigned from = me * per;                       // (the warps' number times per is little more than total: no overflow)
-    if (from >= total) { if (p.Sp) pdl_wait(); return; }
+    if (from >= total) { if (AHEAD) pdl_wait(); return; }
     int count = (int)min(per, total - from);              // blocks of this warp
     // ---- the first of them
     const auto open = [&](PxCursor &c, int blk) {         // block blk of item (b, sub)
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_mma(const __grid_consta
     if (*abort_flag)                                      // aborting: the copies under way must land before the CTA gives its shared memory back
         for (int i = 0; i < 2; i++)
             for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(bar + i), i < stage ? phase ^ 1u : phase); k++) {}
-    if (p.Sp) pdl_wait();
+    if (AHEAD) pdl_wait();
 }
 
 // ------------------------------------------------------------------ the shared keys of many rows
@@ -851,7 +851,8 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     QLMB_CUDA(cudaGetDevice(&dev));
     QLMB_REQUIRE(dev >= 0 && dev < 64, "device index %d", dev);
     if (!configured_dev[dev]) {
-        QLMB_CUDA(cudaFuncSetAttribute(k_px_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)px_smem(PX_MAXB)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_px_mma<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)px_smem(PX_MAXB)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_px_mma<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)px_smem(PX_MAXB)));
         QLMB_CUDA(cudaFuncSetAttribute(k_px_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM));
         configured_dev[dev] = true;
     }
@@ -867,7 +868,7 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
         QLMB_CUDA(pdl_launch(true, k_px_tc, dim3((unsigned)(t.tiles * t.pieces * KV)), dim3(PT_T), PT_SMEM, st, t));
         QLMB_LAUNCH_CHECK("k_px_tc");
     }
-    QLMB_CUDA(pdl_launch_small(k_px_mma, dim3((unsigned)(pl.warps / PX_WARPS)), dim3(32 * PX_WARPS), px_smem(B), st, p));
+    QLMB_CUDA(pdl_launch_small(pl.Sp ? k_px_mma<true> : k_px_mma<false>, dim3((unsigned)(pl.warps / PX_WARPS)), dim3(32 * PX_WARPS), px_smem(B), st, p));
     QLMB_LAUNCH_CHECK("k_px_mma");
     // Eight warps a row where rows are few: one of a long prefix has a hundred segments.  Whole calls with one warp a row and with eight:
     // 384 rows 16.6 and 11.0 us, 768 rows 33.4 and 31.8, 5120 rows 96 and 114.
