@@ -38,9 +38,12 @@ int *device_error_word(void)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     if (!g_errword[dev]) {
+        // The first call may come while a stream is being captured, where an allocation is refused unless the thread says that it knows.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
         int *p = nullptr;
-        if (cudaMalloc(&p, 16 * sizeof(int)) != cudaSuccess) return nullptr;
-        if (cudaMemset(p, 0, 16 * sizeof(int)) != cudaSuccess) return nullptr;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+        const bool made = cudaMalloc(&p, 16 * sizeof(int)) == cudaSuccess && cudaMemset(p, 0, 16 * sizeof(int)) == cudaSuccess;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess || !made) return nullptr;
         g_errword[dev] = p;
     }
     return g_errword[dev];

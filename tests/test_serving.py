@@ -848,3 +848,27 @@ def test_the_large_forms_on_two_streams(cuda):
     for k in range(2):
         for a, b in zip(got[k] if k == 0 else got[k][::-1], want):
             assert all(torch.equal(p, r) for p, r in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_the_first_call_of_a_process_may_be_captured(cuda):
+    """Nothing was set up before: the device error word and the kernels' attributes are made while the stream is captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys; sys.path.insert(0, "tests")
+import torch
+from cudalm_c_b200 import block
+x = torch.randn(2, 3, 300, device="cuda"); d = torch.zeros(2, 2, device="cuda", dtype=torch.int32)
+u, t = torch.rand(2, 3, device="cuda"), torch.ones(2, device="cuda"); torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = block.dec_verify(x, d, u, t)
+g.replay(); torch.cuda.synchronize()
+want = block.dec_verify(x, d, u, t); torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, want)); print("equal")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
