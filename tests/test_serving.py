@@ -45,9 +45,9 @@ def test_refusals_of_the_entry_points():
         (lambda: attn(nbytes=ctypes.c_size_t(16)), b"workspace of 16 bytes"),
         (lambda: verify(out=None), b"NULL"), (lambda: verify(draft=None), b"NULL"), (lambda: verify(dt=2), b"type"), (lambda: verify(n=-1), b"n -1"),
         (lambda: verify(n=64), b"n 64"), (lambda: verify(V=0), b"V 0"), (lambda: verify(ld=15), b"rows of 15"), (lambda: verify(ldq=15), b"and 15"),
-        (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None, K=8192), b"workspace"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
+        (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None, M=100, K=8192), b"workspace"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
         (lambda: lora(K=60), b"multiples of 8"), (lambda: lora(N=63), b"multiples of 8"), (lambda: lora(R=12), b"rank 12"), (lambda: lora(R=264), b"rank 264"),
-        (lambda: lora(R=0), b"rank 0"), (lambda: lora(Y=ctypes.c_void_p(8192), X=ctypes.c_void_p(8192)), b"Y is X"), (lambda: lora(Y=ctypes.c_void_p(8192), X=odd), b"aligned"), (lambda: lora(K=8192, nbytes=ctypes.c_size_t(4)), b"workspace of 4 bytes"),
+        (lambda: lora(R=0), b"rank 0"), (lambda: lora(Y=ctypes.c_void_p(8192), X=ctypes.c_void_p(8192)), b"Y is X"), (lambda: lora(Y=ctypes.c_void_p(8192), X=odd), b"aligned"), (lambda: lora(M=100, K=8192, nbytes=ctypes.c_size_t(4)), b"workspace of 4 bytes"),
     ]
     for i, (call, needle) in enumerate(cases):
         assert call() == 1, i
@@ -62,7 +62,7 @@ def test_refusals_of_the_entry_points():
     assert L.qlmb_dec_attn_prefix_bytes(2, 3, 100, 50, 4, 2) > 0
     for bad in ((0, 64, 64, 8), (4, 60, 64, 8), (4, 64, 64, 4), (4, 64, 64, 300)):
         assert L.qlmb_lora_bytes(*bad) == 0, bad
-    assert L.qlmb_lora_bytes(5, 64, 128, 16) == 16 and L.qlmb_lora_bytes(5, 4096, 128, 16) >= 5 * 16 * 4
+    assert L.qlmb_lora_bytes(5, 64, 128, 16) == 16 and L.qlmb_lora_bytes(105, 4096, 128, 16) >= 105 * 16 * 4
 
 
 def test_refusals_of_the_mirrors():
@@ -616,7 +616,7 @@ LORA = [
     (1, 8, 8, 8, 1), (1, 768, 768, 8, 4), (3, 72, 136, 16, 2), (16, 64, 64, 64, 1), (17, 256, 512, 24, 5), (64, 768, 1536, 16, 64), (64, 1000, 200, 72, 7), (130, 512, 768, 256, 3),
     (333, 384, 264, 32, 10), (1000, 768, 768, 8, 40), (2, 4096, 16384, 16, 2), (70, 40, 1032, 40, 3),
     (2049, 72, 136, 8, 3), (2500, 768, 264, 64, 9), (2300, 256, 520, 136, 5), (4097, 512, 768, 16, 200), (257, 1024, 128, 64, 3),
-    (2049, 72, 136, 24, 3), (8200, 40, 136, 8, 3), (2100, 1032, 72, 16, 5), (600, 72, 136, 16, 3), (2304, 768, 520, 256, 4), (700, 64, 64, 32, 2), (5000, 136, 72, 48, 20), (512, 1024, 1544, 112, 1), (2180, 4104, 8, 16, 2),
+    (2049, 72, 136, 24, 3), (32, 4096, 776, 16, 9), (31, 1016, 1032, 64, 31), (5, 8192, 520, 8, 2), (8200, 40, 136, 8, 3), (2100, 1032, 72, 16, 5), (600, 72, 136, 16, 3), (2304, 768, 520, 256, 4), (700, 64, 64, 32, 2), (5000, 136, 72, 48, 20), (512, 1024, 1544, 112, 1), (2180, 4104, 8, 16, 2),
 ]
 
 
