@@ -55,6 +55,6 @@ def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
         nbytes = _prefix_ws[(dev, shape)] = lib().qlmb_dec_attn_prefix_bytes(*shape)
     O = torch.empty_like(Q)
     lse = torch.empty_strided((rows, H), (H, 1), dtype=torch.float32, device=Q.device)         # (torch.empty: 0.9 us more)
-    ws = Q.new_empty(nbytes + 1 >> 1) if nbytes else None
+    ws = Q.new_empty(nbytes + 1 >> 1) if nbytes > 16 else None
     calls.dec_attn_prefix(O, lse, Q, Kp, Vp, Kc, Vc, pos, win, *shape, 64, ws, nbytes, stream_ptr())
     return O, lse

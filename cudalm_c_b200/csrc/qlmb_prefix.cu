@@ -69,11 +69,11 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 // items' borders, and leaves of each item that it meets a segment: output in fp32, normalised, and the logarithm (base 2) of its
 // sum.  Segment number = item + warp, which no two share.  k_px_join adds the segments of a row up.
 //
-// Many blocks of shared keys go through k_px_tc instead, in pieces (128 rows a tile, tcgen05), and only the slots' own through
+// Few slots and short prefixes take one launch of k_px_small instead.  Many blocks of shared keys go through k_px_tc, in pieces (128 rows a tile, tcgen05), and only the slots' own through
 // k_px_mma: see px_plan.
 //
-// Measured (12 heads, 12 kv heads unless stated; graph of calls, all launches): 1 slot after 512 keys 9.2 us, 8 slots of 4 tokens after
-// 2048 10.9 us (both the length of two small launches), 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
+// Measured (12 heads, 12 kv heads unless stated; graph of calls, all launches): 1 slot after 512 keys 5.6 us, 8 slots of 4 tokens after
+// 2048 10.9 us, 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
 // 16 heads of 4 kv heads after 32768 91 us (96 where k_px_mma waits for k_px_tc's end).  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of
 // the special-function units; without them it takes 60 us, without any softmax 41 us, which is what its MMAs of 64 columns need.
 constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
@@ -128,6 +128,111 @@ __device__ __forceinline__ int px_div(int x, int d)
     int r = __float2int_rz(__fdividef((float)x, (float)d));
     const int left = x - r * d;
     return left < 0 ? r - 1 : left >= d ? r + 1 : r;
+}
+// 32 keys from kb on (the item's end at k1) and 16 rows: scores, the rows' running maxima (base 2) and sums, O.  A thread has rows g and g + 8,
+// which see keys lo .. hi; every row of the tile sees alo .. ahi.
+__device__ __forceinline__ void px_block(uint32_t sk, uint32_t sv, const uint32_t (&qa)[4][4], int kb, int k1, const int (&lo)[2], const int (&hi)[2], int alo, int ahi,
+                                         float scale_log2, float (&m)[2], float (&l)[2], float (&oc)[8][4])
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    float s[4][4] = {};
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {                              // eight keys, dimensions 32 h .. 32 h + 31
+            uint32_t w[4];
+            px_ldm(sk + (8 * t + (lane & 7)) * 128 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4), w);
+            px_mma(s[t], qa[2 * h], w[0], w[1]);
+            px_mma(s[t], qa[2 * h + 1], w[2], w[3]);
+        }
+    const bool edge = kb < alo || kb + 31 > ahi || kb + 32 > k1;   // some row does not see some key
+    if (__builtin_expect(edge, 0)) {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int key = kb + 8 * t + 2 * q + (c & 1);
+                if (key < lo[c >> 1] || key > hi[c >> 1] || key >= k1) s[t][c] = -INFINITY;
+            }
+    }
+    float mn[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        float mx = fmaxf(fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1])),
+                         fmaxf(fmaxf(s[2][2 * e], s[2][2 * e + 1]), fmaxf(s[3][2 * e], s[3][2 * e + 1])));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+        mn[e] = fmaxf(m[e], mx * scale_log2);
+    }
+    if (__any_sync(~0u, mn[0] > m[0] || mn[1] > m[1])) {            // a new maximum in some row
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float corr = ex2(m[e] - (mn[e] == -INFINITY ? 0.0f : mn[e]));
+            m[e] = mn[e];
+            l[e] *= corr;
+#pragma unroll
+            for (int j = 0; j < 8; j++) { oc[j][2 * e] *= corr; oc[j][2 * e + 1] *= corr; }
+        }
+    }
+    uint32_t pa[2][4];                                             // weights in bf16, as every attention of the library has them
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const float mu = m[e] == -INFINITY ? 0.0f : m[e];          // nothing seen yet: every weight 0
+        float sum[2] = {};
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const float p0 = ex2(fmaf(s[t][2 * e], scale_log2, -mu)), p1 = ex2(fmaf(s[t][2 * e + 1], scale_log2, -mu));
+            sum[t & 1] += p0 + p1;
+            const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
+            pa[t >> 1][2 * (t & 1) + e] = *reinterpret_cast<const uint32_t *>(&h2);
+        }
+        l[e] += sum[0] + sum[1];
+    }
+    uint32_t vw[2][4][4];                                          // [16 keys][16 dimensions]: two pairs of operands
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) px_ldmt(sv + (16 * t + (lane & 15)) * 128 + (((2 * j + (lane >> 4)) ^ (lane & 7)) << 4), vw[t][j]);
+    bool odd = false;                                              // an infinity or a NaN that some row must not see
+    if (__builtin_expect(edge, 0)) {                               // keys behind the item's last are nobody's (a register holds keys 2 q and 2 q + 1 of eight)
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int key = kb + 16 * t + 8 * (k & 1) + 2 * q;
+                const uint32_t in = (key < k1 ? 0xffffu : 0u) | (key + 1 < k1 ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int j = 0; j < 4; j++) { vw[t][j][k] &= in; odd |= px_nonfinite(vw[t][j][k]); }
+            }
+    }
+    if (__builtin_expect(!edge || !__any_sync(~0u, odd), 1)) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) { px_mma(oc[2 * j], pa[t], vw[t][j][0], vw[t][j][1]); px_mma(oc[2 * j + 1], pa[t], vw[t][j][2], vw[t][j][3]); }
+    } else {
+        // 0 * inf is not 0: row by row, with the keys the row does not see taken as zeros
+#pragma unroll 1
+        for (int r = 0; r < 16; r++) {
+            const int rlo = __shfl_sync(~0u, r < 8 ? lo[0] : lo[1], (r & 7) * 4), rhi = __shfl_sync(~0u, r < 8 ? hi[0] : hi[1], (r & 7) * 4);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                uint32_t see[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int key = kb + 16 * t + 8 * h + 2 * q;
+                    see[h] = (key >= rlo && key <= rhi && key < k1 ? 0xffffu : 0u) | (key + 1 >= rlo && key + 1 <= rhi && key + 1 < k1 ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float c[4] = {};
+                    px_mma(c, pa[t], vw[t][j >> 1][2 * (j & 1)] & see[0], vw[t][j >> 1][2 * (j & 1) + 1] & see[1]);
+                    if (r == g) { oc[j][0] += c[0]; oc[j][1] += c[1]; }
+                    if (r == g + 8) { oc[j][2] += c[2]; oc[j][3] += c[3]; }
+                }
+            }
+        }
+    }
 }
 // a place in the row of all blocks: item `sub` of slot b (b = B: of the shared keys), the block's first key, the item's last
 struct PxCursor { int b, sub, key, last; };
@@ -310,104 +415,7 @@ template <bool AHEAD> __global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_m
             __syncwarp();                                 // the queries are read
         }
         load();                                           // into the place of the block before this one
-        float s[4][4] = {};
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {                              // eight keys, dimensions 32 h .. 32 h + 31
-                uint32_t w[4];
-                px_ldm(sk + (8 * t + (lane & 7)) * 128 + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4), w);
-                px_mma(s[t], qa[2 * h], w[0], w[1]);
-                px_mma(s[t], qa[2 * h + 1], w[2], w[3]);
-            }
-        const bool edge = kb < alo || kb + 31 > ahi || kb + 32 > k1;   // some row does not see some key
-        if (__builtin_expect(edge, 0)) {
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int key = kb + 8 * t + 2 * q + (c & 1);
-                    if (key < lo[c >> 1] || key > hi[c >> 1] || key >= k1) s[t][c] = -INFINITY;
-                }
-        }
-        float mn[2];
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            float mx = fmaxf(fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1])),
-                             fmaxf(fmaxf(s[2][2 * e], s[2][2 * e + 1]), fmaxf(s[3][2 * e], s[3][2 * e + 1])));
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-            mn[e] = fmaxf(m[e], mx * p.scale_log2);
-        }
-        if (__any_sync(~0u, mn[0] > m[0] || mn[1] > m[1])) {            // a new maximum in some row
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const float corr = ex2(m[e] - (mn[e] == -INFINITY ? 0.0f : mn[e]));
-                m[e] = mn[e];
-                l[e] *= corr;
-#pragma unroll
-                for (int j = 0; j < 8; j++) { oc[j][2 * e] *= corr; oc[j][2 * e + 1] *= corr; }
-            }
-        }
-        uint32_t pa[2][4];                                             // weights in bf16, as every attention of the library has them
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const float mu = m[e] == -INFINITY ? 0.0f : m[e];          // nothing seen yet: every weight 0
-            float sum[2] = {};
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const float p0 = ex2(fmaf(s[t][2 * e], p.scale_log2, -mu)), p1 = ex2(fmaf(s[t][2 * e + 1], p.scale_log2, -mu));
-                sum[t & 1] += p0 + p1;
-                const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
-                pa[t >> 1][2 * (t & 1) + e] = *reinterpret_cast<const uint32_t *>(&h2);
-            }
-            l[e] += sum[0] + sum[1];
-        }
-        uint32_t vw[2][4][4];                                          // [16 keys][16 dimensions]: two pairs of operands
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) px_ldmt(sv + (16 * t + (lane & 15)) * 128 + (((2 * j + (lane >> 4)) ^ (lane & 7)) << 4), vw[t][j]);
-        bool odd = false;                                              // an infinity or a NaN that some row must not see
-        if (__builtin_expect(edge, 0)) {                               // keys behind the item's last are nobody's (a register holds keys 2 q and 2 q + 1 of eight)
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int key = kb + 16 * t + 8 * (k & 1) + 2 * q;
-                    const uint32_t in = (key < k1 ? 0xffffu : 0u) | (key + 1 < k1 ? 0xffff0000u : 0u);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) { vw[t][j][k] &= in; odd |= px_nonfinite(vw[t][j][k]); }
-                }
-        }
-        if (__builtin_expect(!edge || !__any_sync(~0u, odd), 1)) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) { px_mma(oc[2 * j], pa[t], vw[t][j][0], vw[t][j][1]); px_mma(oc[2 * j + 1], pa[t], vw[t][j][2], vw[t][j][3]); }
-        } else {
-            // 0 * inf is not 0: row by row, with the keys the row does not see taken as zeros
-#pragma unroll 1
-            for (int r = 0; r < 16; r++) {
-                const int rlo = __shfl_sync(~0u, r < 8 ? lo[0] : lo[1], (r & 7) * 4), rhi = __shfl_sync(~0u, r < 8 ? hi[0] : hi[1], (r & 7) * 4);
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    uint32_t see[2];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int key = kb + 16 * t + 8 * h + 2 * q;
-                        see[h] = (key >= rlo && key <= rhi && key < k1 ? 0xffffu : 0u) | (key + 1 >= rlo && key + 1 <= rhi && key + 1 < k1 ? 0xffff0000u : 0u);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        float c[4] = {};
-                        px_mma(c, pa[t], vw[t][j >> 1][2 * (j & 1)] & see[0], vw[t][j >> 1][2 * (j & 1) + 1] & see[1]);
-                        if (r == g) { oc[j][0] += c[0]; oc[j][1] += c[1]; }
-                        if (r == g + 8) { oc[j][2] += c[2]; oc[j][3] += c[3]; }
-                    }
-                }
-            }
-        }
+        px_block(sk, sv, qa, kb, k1, lo, hi, alo, ahi, p.scale_log2, m, l, oc);
         __syncwarp();                                                  // the block is read: the next copies may take its place
         const PxCursor was = cc;
         begin = count == 1 || step(cc);
@@ -743,8 +751,143 @@ template <int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 32 * NW) k_p
     if (p.lse && lane == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mref + log2f(sum)) * 0.6931471805599453f;
 }
 
+// ------------------------------------------------------------------ few slots, short prefixes
+// One launch: a CTA per (slot, kv head, 16 rows) goes through the shared keys and the slot's own, twelve warps an equal run of blocks each,
+// and joins the warps' maxima, sums and outputs in shared memory.  Shared keys are read once a slot, from L2.
+constexpr int PS_SMEM = PX_Q + 16 * 128 + 256, PS_ROW = PX_HD + 4;      // rings, the tile's queries, barriers; a row of the join: O, maximum, sum
+__global__ void __launch_bounds__(32 * PX_WARPS, 1) k_px_small(const __grid_constant__ PxParams p)
+{
+    extern __shared__ __align__(1024) uint8_t px_s[];
+    uint64_t *bars = reinterpret_cast<uint64_t *>(px_s + PX_Q + 16 * 128);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 2 * PX_WARPS);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    if (smem_u32(px_s) & 1023u) {             // the swizzled blocks need a 1 KiB-aligned base
+        if (tid == 0 && p.errword && atomicCAS(p.errword, 0, 201) == 0) { p.errword[1] = 132; p.errword[2] = (int)blockIdx.x; }
+        pdl_wait();
+        return;
+    }
+    if (tid == 0) {
+        prefetch_map(&p.kc_map); prefetch_map(&p.vc_map);
+        if (p.P > 0) { prefetch_map(&p.kp_map); prefetch_map(&p.vp_map); }
+        for (int i = 0; i < 2 * PX_WARPS; i++) mbar_init(smem_u32(&bars[i]), 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    __syncthreads();
+    pdl_trigger();
+    pdl_wait();
+    const int KT = p.KV * p.t_own, b = (int)blockIdx.x / KT, sub = (int)blockIdx.x - b * KT, kvh = px_div(sub, p.t_own), row0 = (sub - kvh * p.t_own) * 16;
+    const int t0 = p.pos[b], rows = min(16, p.n * p.G - row0);
+    if (!px_slot_ok(t0, p.n, p.P, p.Tm)) {
+        if (sub == 0 && tid == 0) report_bad_index(p.errword, 306, b, t0);
+        return;
+    }
+    const auto place = [&](int r, int &t) {               // row r: its place in O / 64, and its position
+        const int i = px_div(row0 + r, p.G);
+        t = t0 + i;
+        return (size_t)(b * p.n + i) * p.H + kvh * p.G + row0 + r - i * p.G;
+    };
+    const int lo_pre = p.win > 0 ? max(0, t0 - p.win + 1) & ~31 : 0, n_pre = lo_pre < p.P ? (p.P - 1 - lo_pre) / 32 + 1 : 0;
+    const int first = px_first(p, t0), blocks = n_pre + px_blocks(p, t0), w0 = blocks * warp / PX_WARPS, w1 = blocks * (warp + 1) / PX_WARPS;
+    const uint32_t ring = smem_u32(px_s) + warp * (2 * PX_STAGE), sq = smem_u32(px_s) + PX_Q;
+    uint64_t *bar = bars + 2 * warp;
+    int next = w0;
+    const auto load = [&]() {
+        if (next < w1) {
+            if (elect_one()) {
+                const bool mine = next >= n_pre;
+                const uint32_t full = smem_u32(bar + ((next - w0) & 1)), d = ring + ((next - w0) & 1) * PX_STAGE;
+                const int x = kvh * PX_HD, y = mine ? b * p.Tm + first + 32 * (next - n_pre) : lo_pre + 32 * next;
+                mbar_expect_tx(full, 2 * PX_BLK);
+                tma_load_2d(d, mine ? &p.kc_map : &p.kp_map, full, x, y);
+                tma_load_2d(d + PX_BLK, mine ? &p.vc_map : &p.vp_map, full, x, y);
+            }
+            __syncwarp();
+            next++;
+        }
+    };
+    load();
+    if (tid < 128) {                          // 16 bytes each
+        const int r = tid >> 3, c = tid & 7;
+        int t;
+        px_copy(sq + r * 128 + ((c ^ (r & 7)) << 4), p.Q + place(min(r, rows - 1), t) * PX_HD + 8 * c, r < rows);
+    }
+    px_commit();
+    px_wait<0>();
+    __syncthreads();
+    uint32_t qa[4][4];
+#pragma unroll
+    for (int s = 0; s < 4; s++) px_ldm(sq + (lane & 15) * 128 + (((2 * s + (lane >> 4)) ^ (lane & 7)) << 4), qa[s]);
+    float oc[8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    int lo[2], hi[2], alo = 0, ahi = 0, bad = 0;
+    for (int j = w0; j < w1; j++) {
+        const bool mine = j >= n_pre;
+        if (j == w0 || j == n_pre) {          // the keys that the thread's rows see of these, and those that every row sees
+            alo = -1; ahi = 0x7fffffff;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                int t;
+                const int r = g + 8 * e;
+                lo[e] = 0x7fffffff; hi[e] = -1;
+                if (r >= rows) continue;
+                place(r, t);
+                hi[e] = mine ? t - p.P : p.P - 1;
+                lo[e] = p.win > 0 ? max(0, t - p.win + 1 - (mine ? p.P : 0)) : 0;
+                if (lo[e] > hi[e]) { lo[e] = 0x7fffffff; hi[e] = -1; }
+                alo = max(alo, lo[e]); ahi = min(ahi, hi[e]);
+            }
+#pragma unroll
+            for (int o = 16; o >= 4; o >>= 1) { alo = max(alo, __shfl_xor_sync(~0u, alo, o)); ahi = min(ahi, __shfl_xor_sync(~0u, ahi, o)); }
+        }
+        const int stage = (j - w0) & 1;
+        load();                               // (its place was read in the round before)
+        if ((bad = at_all_wait(smem_u32(bar + stage), (uint32_t)((j - w0) >> 1) & 1u, abort_flag, 133))) break;
+        const uint32_t sk = ring + stage * PX_STAGE;
+        px_block(sk, sk + PX_BLK, qa, mine ? first + 32 * (j - n_pre) : lo_pre + 32 * j, mine ? t0 + p.n - p.P : p.P, lo, hi, alo, ahi, p.scale_log2, m, l, oc);
+        __syncwarp();                         // the block is read
+    }
+    at_give_up(bad, abort_flag, p.errword);
+    if (*abort_flag)                          // aborting: the copies under way must land before the CTA gives its shared memory back
+        for (int i = max(w0, next - 2); i < next; i++)
+            for (uint32_t k = 0; k < AT_WAIT_LIMIT && !at_test(smem_u32(bar + ((i - w0) & 1)), (uint32_t)((i - w0) >> 1) & 1u); k++) {}
+    __syncthreads();                          // the rings are free
+    if (*abort_flag) return;
+    float *xs = reinterpret_cast<float *>(px_s);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        l[e] += __shfl_xor_sync(~0u, l[e], 1);
+        l[e] += __shfl_xor_sync(~0u, l[e], 2);
+        float *d = xs + (warp * 16 + g + 8 * e) * PS_ROW;
+#pragma unroll
+        for (int j = 0; j < 8; j++) *reinterpret_cast<float2 *>(d + 8 * j + 2 * q) = make_float2(oc[j][2 * e], oc[j][2 * e + 1]);
+        if (q == 0) { d[PX_HD] = m[e]; d[PX_HD + 1] = l[e]; }
+    }
+    __syncthreads();
+    if (tid >= 256) return;
+    const int r = tid >> 4, c = 4 * (tid & 15);           // four columns of a row
+    if (r >= rows) return;
+    float mx = -INFINITY, sum = 0.0f, x[4] = {};
+#pragma unroll
+    for (int k = 0; k < PX_WARPS; k++) mx = fmaxf(mx, xs[(k * 16 + r) * PS_ROW + PX_HD]);
+    const float mref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int k = 0; k < PX_WARPS; k++) {
+        const float *d = xs + (k * 16 + r) * PS_ROW;
+        if (d[PX_HD + 1] == 0.0f) continue;   // nothing seen, or all of it -inf
+        const float w = ex2(d[PX_HD] - mref);
+        const float4 v = *reinterpret_cast<const float4 *>(d + c);
+        sum += w * d[PX_HD + 1]; x[0] += w * v.x; x[1] += w * v.y; x[2] += w * v.z; x[3] += w * v.w;
+    }
+    int t;
+    const size_t at = place(r, t);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0] * inv, x[1] * inv), d2 = __floats2bfloat162_rn(x[2] * inv, x[3] * inv);
+    *reinterpret_cast<uint2 *>(p.O + at * PX_HD + c) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&d2));
+    if (p.lse && c == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mref + log2f(sum)) * 0.6931471805599453f;
+}
+
 // What a call needs: tiles, items, warps, pieces of k_px_tc (Sp of `per` steps of keys), bytes of the workspace's parts.
-struct PxPlan { int t_own, t_pre, warps, Sp, per; size_t seg_o, seg_l, part_o, part_l, table, bytes; };
+struct PxPlan { bool small; int t_own, t_pre, warps, Sp, per; size_t seg_o, seg_l, part_o, part_l, table, bytes; };
 static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
 {
     PxPlan pl = {};
@@ -756,6 +899,17 @@ static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
     // 12288 (64, 12) 47.8 and 50.7, 15360 (320, 4) 25.5 and 29.1, 16384 (128, 4) 24.4 and 27.0.  So the border moves with what the slots' caches
     // can hold (10560 blocks, 480 rows, 2 kv heads, caches of 36 rows: 27.5 and 22.6).  k_px_tc has no window.
     pl.t_own = (n * (H / KV) + 15) / 16;
+    // k_px_small up to a CTA an SM and 2048 shared keys, or two and 512.  Us, it and k_px_mma with its join, slots with 64 / 1000 keys of their
+    // own, 12 kv heads: 1 slot after 512 keys 5.8 and 9.4 / 7.5 and 9.0, after 2048 9.6 and 9.6 / 11.7 and 9.5 (and 4 less of the host, a launch
+    // and the workspace), after 4096 14.8 and 10.9; 12 slots after 1024 7.2 and 9.9 / 10.5 and 12.4; 16 slots of 8 tokens, 4 kv heads, after 2048
+    // 10.9 and 20.2; 20 slots (240 CTAs) after 128 8.2 and 9.9 / 14.7 and 16.3, after 512 10.9 and 9.9 / 16.0 and 16.5, after 1024 13.0 and 10.2;
+    // 36 slots (432) after 128 12.7 and 10.3.
+    const long long items = (long long)B * KV * pl.t_own;
+    if ((items <= sm_count() && P <= 2048) || (items <= 2 * sm_count() && P <= 512)) {
+        pl.small = true;
+        pl.bytes = 16;
+        return pl;
+    }
     const long long most_own = (long long)B * KV * pl.t_own * (Tm / 32 + 1);         // if the slots' caches are full
     const bool tc = P > 0 && win <= 0 && KV * ((rows + 15) / 16) * ((P + 31) / 32) > 8704 + (most_own < 4096 ? most_own : 4096);
     pl.t_pre = P > 0 && !tc ? (int)((rows + 15) / 16) : 0;
@@ -814,7 +968,7 @@ extern "C" size_t qlmb_dec_attn_prefix_bytes(int B, int n, int P, int Tm, int H,
 extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const void *Kp, const void *Vp, const void *Kc, const void *Vc, const int *pos,
                                     int win, int B, int n, int P, int Tm, int H, int KV, int hd, void *ws, size_t ws_bytes, void *stream)
 {
-    QLMB_REQUIRE(O && Q && Kc && Vc && pos && ws && (P == 0 || (Kp && Vp)), "qlmb_dec_attn_prefix: NULL argument");
+    QLMB_REQUIRE(O && Q && Kc && Vc && pos && (P == 0 || (Kp && Vp)), "qlmb_dec_attn_prefix: NULL argument");
     QLMB_REQUIRE(hd == PX_HD, "qlmb_dec_attn_prefix: head dimension %d (only 64 is built)", hd);
     if (B <= 0) return QLMB_OK;
     QLMB_REQUIRE(px_shape_ok(B, n, P, Tm, H, KV), "qlmb_dec_attn_prefix: bad shape B %d (up to %d) n %d P %d Tm %d H %d KV %d", B, PX_MAXB, n, P, Tm, H, KV);
@@ -822,7 +976,7 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
                  "qlmb_dec_attn_prefix: rows, caches and workspace must be 16-byte aligned");
     if (win >= P + Tm) win = 0;                                        // hides nothing
     const PxPlan pl = px_plan(B, n, P, Tm, H, KV, win);
-    QLMB_REQUIRE(ws_bytes >= pl.bytes, "qlmb_dec_attn_prefix: a workspace of %zu bytes, %zu are needed", ws_bytes, pl.bytes);
+    QLMB_REQUIRE(pl.small || (ws && ws_bytes >= pl.bytes), "qlmb_dec_attn_prefix: a workspace of %zu bytes, %zu are needed", ws_bytes, pl.bytes);
     PxParams p;
     memset(&p, 0, sizeof p);
     const size_t rows = (size_t)B * n * H;
@@ -853,8 +1007,14 @@ extern "C" int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const vo
     if (!configured_dev[dev]) {
         QLMB_CUDA(cudaFuncSetAttribute(k_px_mma<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)px_smem(PX_MAXB)));
         QLMB_CUDA(cudaFuncSetAttribute(k_px_mma<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)px_smem(PX_MAXB)));
+        QLMB_CUDA(cudaFuncSetAttribute(k_px_small, cudaFuncAttributeMaxDynamicSharedMemorySize, PS_SMEM));
         QLMB_CUDA(cudaFuncSetAttribute(k_px_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM));
         configured_dev[dev] = true;
+    }
+    if (pl.small) {
+        QLMB_CUDA(pdl_launch_small(k_px_small, dim3((unsigned)(B * KV * pl.t_own)), dim3(32 * PX_WARPS), PS_SMEM, st, p));
+        QLMB_LAUNCH_CHECK("k_px_small");
+        return QLMB_OK;
     }
     if (pl.Sp) {
         PxTcParams t;

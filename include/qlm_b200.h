@@ -677,8 +677,8 @@ int qlmb_dec_rope_kv(void *Qo, void *Kc, void *Vc, const void *q, const void *k,
  * caller has appended.  pos[b] = P - 1 is allowed: the slot's first token then sees shared rows only.  O [B*n][H*hd]; lse (may be
  * NULL) [B*n][H] = log of the sum of exp(scores); a token that sees nothing gives zeros and -inf.  What lies in rows that a token does not
  * see has no influence on it, be it infinite or NaN.  P = 0 is allowed (Kp, Vp may then be NULL).  B <= 1024, n <= 64; any Tm and P
- * with P + Tm < 2^30 and B * Tm < 2^31.  ws: qlmb_dec_attn_prefix_bytes(...) bytes (0: the shape is not supported), 16-byte aligned, written and read by
- * the call only; calls that may overlap need one each.  Site 306. */
+ * with P + Tm < 2^30 and B * Tm < 2^31.  ws: qlmb_dec_attn_prefix_bytes(...) bytes (0: the shape is not supported; up to 16: none is needed,
+ * ws may be NULL), 16-byte aligned, written and read by the call only; calls that may overlap need one each.  Site 306. */
 size_t qlmb_dec_attn_prefix_bytes(int B, int n, int P, int Tm, int H, int KV);
 int qlmb_dec_attn_prefix(void *O, float *lse, const void *Q, const void *Kp, const void *Vp, const void *Kc, const void *Vc, const int *pos,
                          int win, int B, int n, int P, int Tm, int H, int KV, int hd, void *ws, size_t ws_bytes, void *stream);

@@ -39,10 +39,10 @@ def test_refusals_of_the_entry_points():
     cases = [
         (lambda: rope(Qo=None), b"NULL"), (lambda: rope(hd=128), b"head dimension"), (lambda: rope(n=0), b"bad shape"), (lambda: rope(Tm=0), b"bad shape"),
         (lambda: rope(Tr=0), b"bad shape"), (lambda: rope(Qo=odd), b"aligned"), (lambda: rope(cos=ctypes.c_void_p(4104)), b"aligned"),
-        (lambda: attn(O=None), b"NULL"), (lambda: attn(Kp=None), b"NULL"), (lambda: attn(ws=None), b"NULL"), (lambda: attn(hd=32), b"head dimension"),
+        (lambda: attn(O=None), b"NULL"), (lambda: attn(Kp=None), b"NULL"), (lambda: attn(P=5000, ws=None), b"workspace"), (lambda: attn(hd=32), b"head dimension"),
         (lambda: attn(n=0), b"bad shape"), (lambda: attn(n=65), b"bad shape"), (lambda: attn(P=-1), b"bad shape"), (lambda: attn(H=3, KV=2), b"bad shape"),
         (lambda: attn(P=1 << 30), b"bad shape"), (lambda: attn(O=odd), b"aligned"), (lambda: attn(ws=odd), b"aligned"),
-        (lambda: attn(nbytes=ctypes.c_size_t(16)), b"workspace of 16 bytes"),
+        (lambda: attn(P=5000, nbytes=ctypes.c_size_t(16)), b"workspace of 16 bytes"),
         (lambda: verify(out=None), b"NULL"), (lambda: verify(draft=None), b"NULL"), (lambda: verify(dt=2), b"type"), (lambda: verify(n=-1), b"n -1"),
         (lambda: verify(n=64), b"n 64"), (lambda: verify(V=0), b"V 0"), (lambda: verify(ld=15), b"rows of 15"), (lambda: verify(ldq=15), b"and 15"),
         (lambda: lora(Y=None), b"NULL"), (lambda: lora(ws=None, M=100, K=8192), b"workspace"), (lambda: lora(dt=7), b"type"), (lambda: lora(n=0), b"0 adapters"),
@@ -59,7 +59,7 @@ def test_refusals_of_the_entry_points():
     # workspaces: 0 where the shape is not supported
     for bad in ((0, 1, 8, 8, 2, 2), (1, 65, 8, 8, 2, 2), (1, 1, -1, 8, 2, 2), (1, 1, 8, 8, 3, 2), (1, 1, 1 << 30, 8, 2, 2), (1025, 2, 8, 8, 2, 2), (1024, 1, 8, 1 << 22, 2, 2)):
         assert L.qlmb_dec_attn_prefix_bytes(*bad) == 0, bad
-    assert L.qlmb_dec_attn_prefix_bytes(2, 3, 100, 50, 4, 2) > 0
+    assert L.qlmb_dec_attn_prefix_bytes(2, 3, 100, 50, 4, 2) == 16 and L.qlmb_dec_attn_prefix_bytes(2, 3, 5000, 50, 4, 2) > 2 * 3 * 4 * 64 * 4
     for bad in ((0, 64, 64, 8), (4, 60, 64, 8), (4, 64, 64, 4), (4, 64, 64, 300)):
         assert L.qlmb_lora_bytes(*bad) == 0, bad
     assert L.qlmb_lora_bytes(5, 64, 128, 16) == 16 and L.qlmb_lora_bytes(105, 4096, 128, 16) >= 105 * 16 * 4
@@ -209,7 +209,7 @@ SHAPES = [
     (2, 16, 32, 2, 60, 100, 0), (4, 1, 2, 2, 4097, 20, 0), (1, 1, 2, 2, 3, 5000, 0), (16, 8, 8, 8, 0, 300, 0), (70, 3, 4, 4, 200, 30, 0), (1, 5, 1, 1, 20000, 9, 0),
     # shared keys of many rows (or very many of one) have a kernel of their own, joins of many rows and windows theirs
     (16, 5, 16, 4, 5003, 40, 0), (13, 5, 8, 8, 9857, 20, 0), (1, 1, 12, 12, 33003, 20, 0), (3, 64, 8, 2, 16448, 80, 0), (12, 5, 16, 2, 4800, 36, 0), (64, 5, 16, 4, 1217, 50, 0), (16, 5, 16, 4, 5003, 40, 4000),
-    (300, 2, 4, 2, 40, 9, 0), (1024, 1, 2, 2, 40, 6, 0), (1024, 1, 1, 1, 13000, 3, 0),
+    (300, 2, 4, 2, 40, 9, 0), (160, 3, 8, 2, 129, 40, 0), (400, 1, 2, 2, 0, 300, 0), (150, 2, 4, 4, 100, 50, 20), (37, 1, 4, 4, 2048, 33, 0), (37, 1, 4, 4, 2049, 33, 0), (5, 9, 8, 1, 700, 700, 100), (1024, 1, 2, 2, 40, 6, 0), (1024, 1, 1, 1, 13000, 3, 0),
     (3, 2, 4, 2, 100, 50, 1), (3, 4, 4, 2, 100, 50, 20), (6, 3, 2, 2, 400, 300, 128), (20, 5, 8, 2, 300, 64, 100), (2, 1, 2, 1, 64, 64, 2 ** 31 - 1), (9, 7, 3, 3, 5, 70, 33),
 ]
 
@@ -238,7 +238,7 @@ def test_attention(cuda, B, n, H, KV, P, Tm, win):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,n,H,KV,P,Tm,win", [(2, 4, 4, 2, 40, 30, 0), (9, 3, 16, 1, 200, 40, 0), (3, 4, 4, 2, 90, 60, 16), (40, 4, 4, 2, 300, 60, 64)])
+@pytest.mark.parametrize("B,n,H,KV,P,Tm,win", [(2, 4, 4, 2, 40, 30, 0), (9, 3, 16, 1, 200, 40, 0), (3, 4, 4, 2, 90, 60, 16), (40, 4, 4, 2, 300, 60, 64), (160, 4, 4, 2, 300, 60, 64), (160, 3, 16, 1, 200, 40, 0)])
 @pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
 def test_attention_keeps_infinities_to_those_who_see_them(cuda, B, n, H, KV, P, Tm, win, what):
     """The last new token's value (and with a window a row that only the first token still sees) is no number: the tokens that
