@@ -827,6 +827,7 @@ template <bool F32, int NT, int UK> __global__ void __launch_bounds__(256) k_lor
 }
 
 // ---- few rows, large adapters: two launches, CTAs of places again; first the inner numbers in slices of K, then blocks of columns.
+// (64 inner columns: two steps at a time of fp32 rows, 64.9 to 46.6 us at K 4040; of bf16 rows, 22.2 to 32.4 at K 4096, one.)
 template <bool F32, int NT, int UK> __global__ void __launch_bounds__(128) k_lora_down(const __grid_constant__ LoraParams p)
 {
     __shared__ float red[4][16][8 * NT + 2];
@@ -1078,8 +1079,12 @@ static LoraForm lora_form(int M, int K, int N, int R, int *S, int *kslice)
     *kslice = K; *S = 0;
     if (M > 8192 || (M > 2048 && R > 16)) return LORA_TILE;
     if (M <= 256 && R <= 64 && (long long)K * R <= (M <= 32 && N <= 4096 ? 65536 : 32768) && (N <= 2048 || (long long)M * N <= 32768)) return LORA_ONE;
+    // Slices of K: as many CTAs as the device holds, if every row has a place; four times as many of at least 1024, since rows mostly share
+    // their adapter with neighbours.  (R 64: fp32, K 4040, 895 / 1 64.9 and 34.3, with the loads below; bf16, K 4096, R 32, 1024 / 64 52.7 and
+    // 37.8; slices of 384 where there was one of 768, 2048 / 8: 13.1 and 14.3.)
     long long s = (4LL * sm_count() + M - 1) / M;
-    const long long most = (K + 511) / 512;              // four warps with four steps of 32 each
+    const long long most = (K + 511) / 512, more = (16LL * sm_count() + M - 1) / M;       // most: four warps with four steps of 32 each
+    if (s < more) s = more < K / 1024 ? more : s > K / 1024 ? s : K / 1024;
     if (s > most) s = most;
     if (s < 1) s = 1;
     *kslice = (int)(((K + s - 1) / s + 127) / 128 * 128);
@@ -1186,7 +1191,7 @@ template <bool F32> static int lora_launch(const LoraParams &p, LoraForm form, c
         QLMB_CUDA(cudaFuncSetAttribute(k_lora_up<F32, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lr_smem<F32, false>(256)));
         configured_dev[dev] = true;
     }
-    QLMB_CUDA(pdl_launch_small(narrow ? k_lora_down<F32, 2, 4> : k_lora_down<F32, LR_RT / 8, 1>, gd, dim3(128), 0, st, p));
+    QLMB_CUDA(pdl_launch_small(narrow ? k_lora_down<F32, 2, 4> : k_lora_down<F32, LR_RT / 8, F32 ? 2 : 1>, gd, dim3(128), 0, st, p));
     QLMB_LAUNCH_CHECK("k_lora_down");
     // behind k_lora_down, which waits before it lets this launch start (without early launches there is nothing to be ahead of)
     void (*up)(const LoraParams) = pdl_enabled() ? (narrow ? k_lora_up<F32, true, true> : k_lora_up<F32, false, true>) : (narrow ? k_lora_up<F32, true, false> : k_lora_up<F32, false, false>);
