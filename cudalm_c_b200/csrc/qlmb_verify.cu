@@ -23,6 +23,7 @@ namespace qlmb {
 
 constexpr int VF_C = 8;                       // CTAs of a slot: one cluster
 constexpr int VF_ROWS = 64;                   // rows of logits of a slot, at most
+constexpr int VF_GROUP = 2;                   // rows of a round, at most
 
 struct VerifyParams {
     int *out, *count;
@@ -80,7 +81,8 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
     constexpr int VF_T = 32 * VF_W, RPL = VF_C * VF_W / 32;      // threads; runs of a row a lane looks at when they are joined
     cg::cluster_group cl = cg::this_cluster();
     __shared__ VfPart warp_part[VF_ROWS][VF_W], row_part[VF_ROWS];
-    __shared__ double wtot[VF_W], wleft[VF_W];            // of the row that ends the slot: the runs' weights without the refused draft
+    __shared__ double run_w[VF_GROUP][VF_C * VF_W];       // of the rows of a round: what the runs weigh, by the row's maximum
+    __shared__ double wtot[VF_W], wleft[VF_W];            // of the row that ends the slot: the runs' weights behind a refused draft
     __shared__ int sx[VF_ROWS];               // the drafts, their logits, u q of each
     __shared__ float sl[VF_ROWS];
     __shared__ double suq[VF_ROWS];
@@ -97,7 +99,7 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
         }
         return;
     }
-    const float temp = p.temp[b];
+    const float temp = p.temp[b], un = p.u[(size_t)b * (n + 1) + n];
     const bool greedy = !(temp > 0.0f);
     const double it = greedy ? 1.4426950408889634 : 1.4426950408889634 / fmin((double)temp, 1e30);      // an infinite one: every finite logit has the weight 1
     const float cT = (float)fmin(it, 1e38);
@@ -122,7 +124,7 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
     };
     float4 x[4], y[4];
     fetch(0, 0, x);
-    int r = 0, kind = -1;
+    int r = 0, kind = -1, at = 0;             // at: the row's place in its round
     for (int i0 = 0; i0 <= nd; i0 += p.group) {
         const int i1 = min(i0 + p.group, nd + 1);
         // ---- this warp's run of the rows i0 .. i1 - 1; the next step is requested ahead, the next group's first one too
@@ -199,7 +201,9 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
             double zt = 0.0, z1 = 0.0;
 #pragma unroll
             for (int k = 0; k < RPL; k++) {
-                zt += a[k].st * vf_scale(a[k].m, t.m, it);
+                const double x = a[k].st * vf_scale(a[k].m, t.m, it);
+                zt += x;
+                run_w[i - i0][RPL * ln + k] = vf_ex2((a[k].m - t.m) * cT) > 0.0f ? x : 0.0;      // 0: every weight of the run is 0 below
                 z1 += (double)(a[k].s1 * vf_ex2((fmaxf(a[k].m, -FLT_MAX) - fmaxf(t.m, -FLT_MAX)) * 1.4426950408889634f));
             }
             t.st = vf_warp_sum(zt);
@@ -221,25 +225,14 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
         const int first = __reduce_min_sync(~0u, r), who = __ffs(__ballot_sync(~0u, r == first)) - 1;
         kind = __shfl_sync(~0u, kind, who);
         r = first;
+        at = r - i0;
         if (kind >= 0) break;
     }
-    if (c == 0) {                             // what was taken, and the places behind the end
-        for (int i = tid; i <= n; i += VF_T) {
-            if (i == r && kind < 2) continue;
-            out[i] = i < r ? sx[i] : -1;
-            lp[i] = i < r ? (float)((double)sl[i] - (double)row_part[i].m) - logf(row_part[i].s1) : 0.0f;
-        }
-        if (tid == 0) {
-            p.count[b] = kind < 2 ? r + 1 : r;
-            if (kind == 2) report_bad_index(p.errword, 309, b, r);
-            if (kind == 3) report_bad_index(p.errword, 308, b, sx[r]);
-        }
-    }
-    if (kind >= 2) { cl.sync(); return; }     // nobody reads this CTA's shared memory any more
     const size_t base = row0 + (size_t)r * p.ld;
-    const VfPart row = row_part[r];
+    const VfPart row = row_part[min(r, VF_ROWS - 1)];
     int pick = -1;
-    if (greedy) {
+    if (kind >= 2) {
+    } else if (greedy) {
         if (c == 0 && tid == 0) pick = row.arg;
     } else {
         const bool rest = kind == 1;
@@ -250,34 +243,36 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
             if (rest) { if (qr) e = fmax(fma(-(double)qr[v], row.st, e), 0.0); else if (v == xr) e = 0.0; }
             return e;
         };
-        double a = 0.0;
-        if (rest) {
+        // every warp of the slot finds the run whose end passes the target; the last with a weight where rounding leaves none
+        double xs[RPL], mysum = 0.0, all = 0.0;
+        if (qr) {                                         // what q leaves of each run
+            double a = 0.0;
 #pragma unroll 8
             for (int v = w0 + ln; v < w1; v += 32) a += weight(v, true);
             a = vf_warp_sum(a);
             if (ln == 0) wleft[w] = a;
             cl.sync();
-        }
-        // every warp of the slot finds the run whose end passes the target; the last with a weight where rounding leaves none
-        double xs[RPL], mysum = 0.0, all = 0.0;
-        if (rest) {
 #pragma unroll
             for (int k = 0; k < RPL; k++) { xs[k] = *cl.map_shared_rank(&wleft[(RPL * ln + k) % VF_W], (RPL * ln + k) / VF_W); mysum += xs[k]; }
+            all = vf_warp_sum(mysum);
+        } else if (rest) {                                // the refused draft's run without it: every warp adds it up for itself
+            const int rx = xr / run, x1 = min((rx + 1) * run, p.V);
+            double a = 0.0;
+#pragma unroll 8
+            for (int v = rx * run + ln; v < x1; v += 32) a += weight(v, true);
+            a = vf_warp_sum(a);
+#pragma unroll
+            for (int k = 0; k < RPL; k++) { xs[k] = RPL * ln + k == rx ? a : run_w[at][RPL * ln + k]; mysum += xs[k]; }
             all = vf_warp_sum(mysum);
         }
         const bool left = all > 0.0;
         if (!left) {                                      // a draw behind the drafts, or nothing is left: by e
             mysum = 0.0;
 #pragma unroll
-            for (int k = 0; k < RPL; k++) {
-                const VfPart *o = cl.map_shared_rank(&warp_part[r][(RPL * ln + k) % VF_W], (RPL * ln + k) / VF_W);
-                const float om = o->m;
-                xs[k] = vf_ex2((om - row.m) * cT) > 0.0f ? o->st * vf_scale(om, row.m, it) : 0.0;   // a run whose every weight is 0 below
-                mysum += xs[k];
-            }
+            for (int k = 0; k < RPL; k++) { xs[k] = run_w[at][RPL * ln + k]; mysum += xs[k]; }
             all = vf_warp_sum(mysum);
         }
-        const double target = (double)p.u[(size_t)b * (n + 1) + n] * all;
+        const double target = (double)un * all;
         double cum = mysum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(~0u, cum, o); if (ln >= o) cum += y; }
@@ -297,10 +292,16 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
             // the CTA reads the run again: a lane has `each` neighbouring tokens
             const int r0 = min(mine * run, p.V), r1 = min(r0 + run, p.V), each = (r1 - r0 + VF_T - 1) / VF_T;
             const int l0 = min(r0 + tid * each, r1), l1 = min(l0 + each, r1);
+            const bool held = each <= 4;                  // the weights stay in registers
+            double e4[4];
             mysum = 0.0;
             int last = -1;
+            if (held) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) { e4[k] = l0 + k < l1 ? weight(l0 + k, left) : 0.0; mysum += e4[k]; if (e4[k] > 0.0) last = l0 + k; }
+            } else
 #pragma unroll 4
-            for (int v = l0; v < l1; v++) { const double e = weight(v, left); mysum += e; if (e > 0.0) last = v; }
+                for (int v = l0; v < l1; v++) { const double e = weight(v, left); mysum += e; if (e > 0.0) last = v; }
             cum = mysum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(~0u, cum, o); if (ln >= o) cum += y; }
@@ -318,11 +319,20 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
                 if (past ? ln == __ffs(past) - 1 : ln == 31 - __clz(some)) {
                     from += cum - mysum;
                     pick = last;
-                    for (int v = l0; v <= last; v++) {
-                        const double e = weight(v, left);
-                        from += e;
-                        if (e > 0.0 && from > target) { pick = v; break; }
-                    }
+                    if (held) {
+#pragma unroll
+                        for (int k = 3; k >= 0; k--) {    // (the lowest that passes; the sums in the order of the loop below)
+                            double x = from;
+#pragma unroll
+                            for (int j = 0; j <= k; j++) x += e4[j];
+                            if (e4[k] > 0.0 && x > target) pick = l0 + k;
+                        }
+                    } else
+                        for (int v = l0; v <= last; v++) {
+                            const double e = weight(v, left);
+                            from += e;
+                            if (e > 0.0 && from > target) { pick = v; break; }
+                        }
                 }
             }
         }
@@ -331,7 +341,19 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
         out[r] = pick;
         lp[r] = (float)((double)vf_ld<BF>(p.logits, base + pick) - (double)row.m) - logf(row.s1);
     }
-    cl.sync();
+    if (c == 0) {                             // what was taken, and the places behind the end
+        for (int i = tid; i <= n; i += VF_T) {
+            if (i == r && kind < 2) continue;
+            out[i] = i < r ? sx[i] : -1;
+            lp[i] = i < r ? (float)((double)sl[i] - (double)row_part[i].m) - logf(row_part[i].s1) : 0.0f;
+        }
+        if (tid == 0) {
+            p.count[b] = kind < 2 ? r + 1 : r;
+            if (kind == 2) report_bad_index(p.errword, 309, b, r);
+            if (kind == 3) report_bad_index(p.errword, 308, b, sx[r]);
+        }
+    }
+    cl.sync();                                // nobody reads this CTA's shared memory any more
 }
 
 }  // namespace qlmb
