@@ -368,12 +368,14 @@ extern "C" int qlmb_dec_verify(int *out, int *count, float *lp, const void *logi
     QLMB_REQUIRE(ld >= V && (!q || ldq >= V), "qlmb_dec_verify: rows of %lld and %lld elements, %d tokens", ld, ldq, V);
     if (B <= 0) return QLMB_OK;
     QLMB_REQUIRE(B < (1 << 24), "qlmb_dec_verify: %d slots", B);
-    // A round (a group of rows, the cluster's meeting, the test) costs about 3 us beside the reading, and rows behind the end are read for
+    // A round (a group of rows, the cluster's meeting, the test) costs about 2.5 us beside the reading, and rows behind the end are read for
     // nothing.  Vocabularies of up to 32768: four warps a CTA, so that the 64 clusters of a full server run at once, and two rows a
-    // round (64 slots of 16384, five rows: 19.4 us; one row a round 21.5, eight warps 24.2, all five rows 20.2).  Above: eight warps
-    // and one row (32 slots of 130001, eight rows: 33.7 us; four warps 44.5, two rows 36.8, sixteen warps 34.0).
+    // round (64 slots of 16384, five rows: 15.5 us; one row a round 17.8, all five rows 16.0, eight warps 23.0; 64 of 32768 23.3, eight warps
+    // 24.7).  Above: eight warps, and two rows where drafts come with probabilities, since those are mostly taken (8 slots of 130048, five
+    // rows 35.4, one row 38.3; 16 of 65536 21.0 and 23.9; four warps 59.2 and 24.2), one where they do not (32 slots of 130001, eight
+    // rows: 26.9 us; two rows 28.9, four warps 33.4).
     const bool wide = V > 32768, bf = lg_dtype == QLMB_BF16, vec = ld % 4 == 0 && ((uintptr_t)logits & (bf ? 7 : 15)) == 0;
-    VerifyParams p = {out, count, lp, logits, q, u, temp, draft, nd, B, n, V, wide ? 1 : 2, ld, ldq, device_error_word()};
+    VerifyParams p = {out, count, lp, logits, q, u, temp, draft, nd, B, n, V, wide && !q ? 1 : 2, ld, ldq, device_error_word()};
     void (*kern)(const VerifyParams);
     if (wide) kern = bf ? (vec ? k_dec_verify<true, true, 8> : k_dec_verify<true, false, 8>) : (vec ? k_dec_verify<false, true, 8> : k_dec_verify<false, false, 8>);
     else kern = bf ? (vec ? k_dec_verify<true, true, 4> : k_dec_verify<true, false, 4>) : (vec ? k_dec_verify<false, true, 4> : k_dec_verify<false, false, 4>);
