@@ -177,7 +177,8 @@ template <bool F32> __device__ __forceinline__ void lr_up_base(const LoraParams 
                     base[e][h][k] = reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(p.base) + ((size_t)mrow[e] * p.N + col) * (F32 ? 4 : 2))[k];
         }
 }
-template <bool F32> __device__ __forceinline__ void lr_up_store(const LoraParams &p, const float (&c)[8][4], const uint4 (&base)[2][2][F32 ? 2 : 1], int cur, int n0, const int (&mrow)[2], const bool (&keep)[2])
+template <bool F32> __device__ __forceinline__ void lr_up_store(const LoraParams &p, const float (&c)[8][4], const uint4 (&base)[2][2][F32 ? 2 : 1], int cur, int n0,
+                                                                    const int (&mrow)[2], const bool (&keep)[2])
 {
     const int q = threadIdx.x & 3;
 #pragma unroll
@@ -431,7 +432,8 @@ template <bool F32, bool SMALL> __global__ void __launch_bounds__(256, 2) k_lora
                 for (int i = lane; i < 16 * XP / 2; i += 32) {
                     const int r = rg + i / (XP / 2), cc = nh * EB / 16 + i % (XP / 2), row = srow[r], n = n0 + cc * (16 / EB);
                     if (row >= 0 && n < c1)
-                        *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p.Y) + ((size_t)row * p.N + n) * EB) = *reinterpret_cast<const uint4 *>(sx + r * (XP * 16) + ((cc ^ (r & 7)) << 4));
+                        *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p.Y) + ((size_t)row * p.N + n) * EB) =
+                            *reinterpret_cast<const uint4 *>(sx + r * (XP * 16) + ((cc ^ (r & 7)) << 4));
                 }
                 rc = 0; n0 += 64;
             }
@@ -445,7 +447,8 @@ template <bool F32, bool SMALL> __global__ void __launch_bounds__(256, 2) k_lora
             const int row = __shfl_sync(~0u, r < 32 ? m[0] : m[1], r & 31), ad = __shfl_sync(~0u, r < 32 ? a[0] : a[1], r & 31);
             if (row < 0 || ad >= 0) continue;
             for (int n = c0 + lane * (16 / EB); n < c1; n += 32 * (16 / EB))
-                *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p.Y) + ((size_t)row * p.N + n) * EB) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p.base) + ((size_t)row * p.N + n) * EB);
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p.Y) + ((size_t)row * p.N + n) * EB) =
+                    *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p.base) + ((size_t)row * p.N + n) * EB);
         }
 }
 
@@ -754,7 +757,10 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
                 } else {
                     uint4 out[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) { const int rr = 32 * quarter + 4 * i + (lane >> 3); out[i] = *reinterpret_cast<const uint4 *>(tile + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)); }
+                    for (int i = 0; i < 8; i++) {
+                        const int rr = 32 * quarter + 4 * i + (lane >> 3);
+                        out[i] = *reinterpret_cast<const uint4 *>(tile + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                    }
                     fence_proxy_async();                  // the next copy comes after these reads and writes (the fence waits for stores to Y, too)
                     bf16 *y = reinterpret_cast<bf16 *>(p.Y) + (size_t)(128 * w.t + 32 * quarter + (lane >> 3)) * p.N + 64 * b + 8 * (lane & 7);
                     if (64 * b + 8 * (lane & 7) < p.N)
@@ -1049,7 +1055,8 @@ template <bool F32, bool NARROW, bool AHEAD> __global__ void __launch_bounds__(1
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int k = 0; k < (F32 ? 2 : 1); k++) base[e][h][k] = *reinterpret_cast<const uint4 *>(lr_s + (g + 8 * e) * PITCH + (256 * i + 64 * warp + 16 * q + 8 * h) * EB + 16 * k);
+                        for (int k = 0; k < (F32 ? 2 : 1); k++)
+                            base[e][h][k] = *reinterpret_cast<const uint4 *>(lr_s + (g + 8 * e) * PITCH + (256 * i + 64 * warp + 16 * q + 8 * h) * EB + 16 * k);
                 lr_up_store<F32>(p, c, base, cur, n0, rows, keep);
             }
             c0 += UP;
@@ -1135,10 +1142,12 @@ static int lora_tc_launch(const LoraParams &p, cudaStream_t st)
     c.l = p;
     c.stages = lc_stages(p.R);
     const unsigned long long M = p.M, K = p.K, N = p.N, AR = (unsigned long long)p.adapters * p.R;
-    const struct { CUtensorMap *m; const void *base; unsigned long long inner, rows; unsigned box; } maps[5] = {{&c.x_map, p.X, K, M, 128}, {&c.a_map, p.A, K, AR, (unsigned)p.R}, {&c.base_map, p.base, N, M, 128}, {&c.b_map, p.Bm, N, AR, (unsigned)p.R},
-                                                                                                                      {&c.y_map, p.Y, N, M, 32}};
+    const unsigned rank = (unsigned)p.R;
+    const struct { CUtensorMap *m; const void *base; unsigned long long inner, rows; unsigned box; } maps[5] = {
+        {&c.x_map, p.X, K, M, 128}, {&c.a_map, p.A, K, AR, rank}, {&c.base_map, p.base, N, M, 128}, {&c.b_map, p.Bm, N, AR, rank}, {&c.y_map, p.Y, N, M, 32}};
     for (int i = 0; i < 5; i++) {
-        const int rc = make_map(maps[i].m, maps[i].base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, maps[i].inner, maps[i].rows, maps[i].inner * 2, 64, maps[i].box, CU_TENSOR_MAP_SWIZZLE_128B);
+        const int rc = make_map(maps[i].m, maps[i].base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, maps[i].inner, maps[i].rows, maps[i].inner * 2, 64, maps[i].box,
+                                CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc) return rc;
     }
     const long long most = (long long)((p.M + 127) / 128) * ((p.N + 63) / 64);
@@ -1194,7 +1203,8 @@ template <bool F32> static int lora_launch(const LoraParams &p, LoraForm form, c
     QLMB_CUDA(pdl_launch_small(narrow ? k_lora_down<F32, 2, 4> : k_lora_down<F32, LR_RT / 8, F32 ? 2 : 1>, gd, dim3(128), 0, st, p));
     QLMB_LAUNCH_CHECK("k_lora_down");
     // behind k_lora_down, which waits before it lets this launch start (without early launches there is nothing to be ahead of)
-    void (*up)(const LoraParams) = pdl_enabled() ? (narrow ? k_lora_up<F32, true, true> : k_lora_up<F32, false, true>) : (narrow ? k_lora_up<F32, true, false> : k_lora_up<F32, false, false>);
+    void (*up)(const LoraParams) = pdl_enabled() ? (narrow ? k_lora_up<F32, true, true> : k_lora_up<F32, false, true>)
+                                                 : (narrow ? k_lora_up<F32, true, false> : k_lora_up<F32, false, false>);
     QLMB_CUDA(pdl_launch(true, up, gu, dim3(128), narrow ? lr_smem<F32, true>(p.R) : lr_smem<F32, false>(p.R), st, p));
     QLMB_LAUNCH_CHECK("k_lora_up");
     return QLMB_OK;
@@ -1207,7 +1217,8 @@ extern "C" int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype
     if (M <= 0) return QLMB_OK;
     QLMB_REQUIRE(lora_shape_ok(M, K, N, R) && adapters > 0, "qlmb_lora_add: M %d, K %d and N %d (multiples of 8), rank %d (a multiple of 8 up to 256), %d adapters", M, K, N, R, adapters);
     QLMB_REQUIRE(Y != X, "qlmb_lora_add: Y is X (it may be the base)");
-    QLMB_REQUIRE((((uintptr_t)Y | (uintptr_t)X | (uintptr_t)base | (uintptr_t)A | (uintptr_t)Bm | (uintptr_t)ws) & 15) == 0, "qlmb_lora_add: rows, adapters and workspace must be 16-byte aligned");
+    QLMB_REQUIRE((((uintptr_t)Y | (uintptr_t)X | (uintptr_t)base | (uintptr_t)A | (uintptr_t)Bm | (uintptr_t)ws) & 15) == 0,
+                 "qlmb_lora_add: rows, adapters and workspace must be 16-byte aligned");
     const size_t need = qlmb_lora_bytes(M, K, N, R);
     QLMB_REQUIRE(need <= 16 || (ws && ws_bytes >= need), "qlmb_lora_add: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
     LoraParams p = {Y, X, base, (const bf16 *)A, (const bf16 *)Bm, scale, adapter, order, (float *)ws, M, K, N, R, adapters, 0, 0, device_error_word()};

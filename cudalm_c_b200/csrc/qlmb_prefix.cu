@@ -69,13 +69,13 @@ __global__ void __launch_bounds__(256) k_dec_rope_kv(bf16 *Qo, bf16 *Kc, bf16 *V
 // items' borders, and leaves of each item that it meets a segment: output in fp32, normalised, and the logarithm (base 2) of its
 // sum.  Segment number = item + warp, which no two share.  k_px_join adds the segments of a row up.
 //
-// Few slots and short prefixes take one launch of k_px_small instead.  Many blocks of shared keys go through k_px_tc, in pieces (128 rows a tile, tcgen05), and only the slots' own through
-// k_px_mma: see px_plan.
+// Few slots and short prefixes take one launch of k_px_small instead.  Many blocks of shared keys go through k_px_tc, in pieces (128
+// rows a tile, tcgen05), and only the slots' own through k_px_mma: see px_plan.
 //
 // Measured (12 heads, 12 kv heads unless stated; graph of calls, all launches): 1 slot after 512 keys 5.6 us, 8 slots of 4 tokens after
-// 2048 10.9 us, 64 slots after 8192 31.6 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and
-// 16 heads of 4 kv heads after 32768 91 us (96 where k_px_mma waits for k_px_tc's end).  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of
-// the special-function units; without them it takes 60 us, without any softmax 41 us, which is what its MMAs of 64 columns need.
+// 2048 10.9 us, 64 slots after 8192 31.8 us (101 MB, 3.2 TB/s), 64 slots of 5 tokens and 16 heads of 4 kv heads after 32768 91 us (96
+// where k_px_mma waits for k_px_tc's end).  In the last k_px_tc has 75 us, 43 GFLOP at 573 TF/s: 168 M exponentials are 37 us of the
+// special-function units; without them it takes 60 us, without any softmax 41 us, which is what its MMAs of 64 columns need.
 constexpr int PX_WARPS = 12;                              // of a CTA, one CTA an SM: their rings fill its shared memory, and its registers
 constexpr int PX_MAXB = 1024;                             // slots: every CTA keeps their positions and block counts
 struct PxParams {

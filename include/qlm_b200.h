@@ -699,9 +699,10 @@ int qlmb_dec_verify(int *out, int *count, float *lp, const void *logits, int lg_
  * Y[m,:] = base[m,:] + scale[a] * (X[m,:] A[a]^T) Bm[a] with a = adapter[m], Y[m,:] = base[m,:] where a is -1.  X [M][K], base and Y
  * [M][N] of `dtype` (Y may be base, not X); A [adapters][R][K] and Bm [adapters][R][N] bf16; scale [adapters]; adapter [M] (device).
  * order (may be NULL): the rows 0 .. M-1 in the order of their adapters; without it rows in any order give the same result, but
- * 16 neighbouring rows (of many: 64 or 128) cost as many passes as they have adapters.  K, N and R multiples of 8, R <= 256 (adapters of a lower rank:
- * zero rows).  Pointers to rows, adapters and ws 16-byte aligned; ws: qlmb_lora_bytes(...) bytes (0: not supported; up to 16: none
- * is needed, ws may be NULL), written and read by the call only.  An adapter or an entry of order out of range is reported (site 307); the row then takes its base, resp. is left out. */
+ * 16 neighbouring rows (of many: 64 or 128) cost as many passes as they have adapters.  K, N and R multiples of 8, R <= 256
+ * (adapters of a lower rank: zero rows).  Pointers to rows, adapters and ws 16-byte aligned; ws: qlmb_lora_bytes(...) bytes (0: not
+ * supported; up to 16: none is needed, ws may be NULL), written and read by the call only.  An adapter or an entry of order out of
+ * range is reported (site 307); the row then takes its base, resp. is left out. */
 size_t qlmb_lora_bytes(int M, int K, int N, int R);
 int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype, const void *A, const void *Bm, const float *scale, int adapters,
                   const int *adapter, const int *order, int M, int K, int N, int R, void *ws, size_t ws_bytes, void *stream);
