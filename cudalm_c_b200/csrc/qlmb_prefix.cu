@@ -899,13 +899,19 @@ static PxPlan px_plan(int B, int n, int P, int Tm, int H, int KV, int win)
     // 12288 (64, 12) 47.8 and 50.7, 15360 (320, 4) 25.5 and 29.1, 16384 (128, 4) 24.4 and 27.0.  So the border moves with what the slots' caches
     // can hold (10560 blocks, 480 rows, 2 kv heads, caches of 36 rows: 27.5 and 22.6).  k_px_tc has no window.
     pl.t_own = (n * (H / KV) + 15) / 16;
-    // k_px_small up to a CTA an SM and 2048 shared keys, or two and 512.  Us, it and k_px_mma with its join, slots with 64 / 1000 keys of their
-    // own, 12 kv heads: 1 slot after 512 keys 5.8 and 9.4 / 7.5 and 9.0, after 2048 9.6 and 9.6 / 11.7 and 9.5 (and 4 less of the host, a launch
-    // and the workspace), after 4096 14.8 and 10.9; 12 slots after 1024 7.2 and 9.9 / 10.5 and 12.4; 16 slots of 8 tokens, 4 kv heads, after 2048
-    // 10.9 and 20.2; 20 slots (240 CTAs) after 128 8.2 and 9.9 / 14.7 and 16.3, after 512 10.9 and 9.9 / 16.0 and 16.5, after 1024 13.0 and 10.2;
-    // 36 slots (432) after 128 12.7 and 10.3.
-    const long long items = (long long)B * KV * pl.t_own;
-    if ((items <= sm_count() && P <= 2048) || (items <= 2 * sm_count() && P <= 512)) {
+    // k_px_small up to a CTA an SM and 2048 shared keys, or two and 512, unless it has a CTA for less than half of the SMs and a warp of it would
+    // go through 8 blocks of keys more than one of k_px_mma, which deals them out evenly (if the caches are full: the host does not see how
+    // full they are).  Us, it and k_px_mma with its join, slots with 64 / 1000 keys of their own, 12 kv heads: 1 slot after 512 keys 5.6 and
+    // 8.4 / 7.6 and 9.0, after 2048 9.5 and 9.0 / 11.7 and 9.5 (and 4 less of the host, a launch and the workspace), after 4096 14.8 and 10.9; 12
+    // slots after 1024 7.2 and 9.9 / 10.5 and 12.4; 16 slots of 8 tokens, 4 kv heads, after 2048 10.9 and 20.2; 20 slots (240 CTAs) after 128 8.2
+    // and 9.9 / 14.7 and 16.3, after 512 10.9 and 9.9 / 16.0 and 16.5, after 1024 13.0 and 10.2; 36 slots (432) after 128 12.7 and 10.3.
+    //   Longer caches, by the blocks a warp has more: 1 slot, no shared keys, 2000 of its own (5) 9.6 and 9.4, 4000 (10) 14.3 and 10.1, 16000
+    // (38) 46.1 and 14.5; 4 slots (48 CTAs) 4000 (7) 14.8 and 12.3, 8000 (14) 25.8 and 17.2, 16000 (28) 47.7 and 40.5; a window of 1024 in 16000
+    // (2) 6.2 and 8.2, of 4096 (10) 14.5 and 9.7.  From half of the SMs on k_px_small asks for as much as HBM gives: 6 slots (72 CTAs) 8000 26.8
+    // and 31.3, 32000 93 and 135; 16 slots, 4 kv heads (64) 4000 14.8 and 12.9, 8000 26.2 and 27.8, 32000 90 and 83; 24 slots (288) 16000 180 and 254.
+    const long long items = (long long)B * KV * pl.t_own, sms = sm_count(), most = win > 0 && (long long)win + n < (long long)P + Tm ? (long long)win + n : (long long)P + Tm;
+    const long long dealt = (items * (Tm < most ? Tm : most) + KV * ((rows + 15) / 16) * (P < most ? P : most)) / sms;       // keys of an SM
+    if (((items <= sms && P <= 2048) || (items <= 2 * sms && P <= 512)) && (2 * items >= sms || most - dealt <= 8 * 32 * PX_WARPS)) {
         pl.small = true;
         pl.bytes = 16;
         return pl;
@@ -961,7 +967,9 @@ extern "C" int qlmb_dec_rope_kv(void *Qo, void *Kc, void *Vc, const void *q, con
 extern "C" size_t qlmb_dec_attn_prefix_bytes(int B, int n, int P, int Tm, int H, int KV)
 {
     if (!px_shape_ok(B, n, P, Tm, H, KV)) return 0;
-    const size_t a = px_plan(B, n, P, Tm, H, KV, 0).bytes, b = px_plan(B, n, P, Tm, H, KV, 1).bytes;
+    // For any window: where k_px_small takes a call without one it takes every one, else the widest is not its, and the rest of a plan asks only
+    // whether there is a window.
+    const size_t a = px_plan(B, n, P, Tm, H, KV, 0).bytes, b = px_plan(B, n, P, Tm, H, KV, P + Tm - 1).bytes;
     return a > b ? a : b;
 }
 

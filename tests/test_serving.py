@@ -872,3 +872,47 @@ assert all(torch.equal(a, b) for a, b in zip(out, want)); print("equal")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------ long caches of few slots
+def test_long_caches_are_dealt_out_to_the_whole_device():
+    """One launch of a CTA per (slot, kv head, 16 rows) only where its warps have few blocks of keys more than dealt out evenly: few slots
+    with long caches have a workspace.  The workspace is enough for every window."""
+    L = _lib()
+    size = L.qlmb_dec_attn_prefix_bytes
+    # B, n, P, Tm, H, KV
+    for few in ((1, 1, 512, 1024, 12, 12), (8, 4, 2048, 1024, 12, 12), (1, 1, 0, 1, 1, 1), (12, 1, 0, 4000, 12, 12)):
+        assert size(*few) == 16, few
+    for long in ((1, 1, 512, 32768, 12, 12), (1, 1, 0, 8000, 1, 1), (4, 1, 512, 16000, 12, 12), (1, 5, 0, 65536, 16, 4)):
+        assert size(*long) > 1000, long
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,n,H,KV,P,Tm", [(1, 1, 12, 12, 512, 5000), (2, 3, 8, 2, 40, 9000), (1, 5, 4, 4, 0, 4100)])
+@pytest.mark.parametrize("win", [0, 1, 100, 2500, 4000, -1])
+def test_attention_in_long_caches_of_few_slots(cuda, B, n, H, KV, P, Tm, win):
+    """On both sides of the border between one launch and three, which a window moves (-1: the widest that hides something)."""
+    from cudalm_c_b200 import attn
+    q, kp, vp, kc, vc = make_attn(B, n, H, KV, P, Tm, 61, cuda)
+    pos = positions(B, n, P, Tm, 62, cuda)
+    win = P + Tm - 1 if win < 0 else win
+    o, lse = attn.dec_attn_prefix(q, kp, vp, kc, vc, pos, H, win=win)
+    ok()
+    check_attn(o, lse, attn64(q, kp, vp, kc, vc, pos, H, win))
+
+
+@pytest.mark.gpu
+def test_attention_dealt_out_in_a_cache_past_32_bits(cuda):
+    """As test_attention_in_a_cache_past_32_bits, with a window too wide for one launch: the same rows in a short cache give the same."""
+    from cudalm_c_b200 import attn
+    B, n, H, KV, P, Tm, win, keep = 3, 2, 12, 12, 50, 1000000, 5000, 5200
+    if torch.cuda.get_device_properties(0).total_memory < 40e9:
+        pytest.skip("needs 10 GB")
+    kc = torch.empty(B, Tm, KV * HD, dtype=torch.bfloat16, device=cuda)
+    vc = torch.empty_like(kc)
+    q, kp, vp, k1, v1 = make_attn(B, n, H, KV, P, keep, 63, cuda)
+    kc[:, Tm - keep:], vc[:, Tm - keep:] = k1, v1
+    pos = torch.tensor([P + Tm - n, P + Tm - 40, P + Tm - n - 130], dtype=torch.int32, device=cuda)
+    o, lse = attn.dec_attn_prefix(q, kp, vp, kc, vc, pos, H, win=win)
+    ok()
+    check_attn(o, lse, attn64(q, kp[:0], vp[:0], k1, v1, pos - P - Tm + keep, H, win))
