@@ -4,6 +4,8 @@
 #include "qlmb_tc.cuh"
 #include <string.h>
 #include <stdlib.h>
+#include <atomic>
+#include <mutex>
 
 namespace qlmb {
 
@@ -23,7 +25,8 @@ int cuda_fail(cudaError_t e, const char *what)
     return QLMB_E_CUDA;
 }
 
-static int *g_errword[64];
+static std::atomic<int *> g_errword[64];
+static std::mutex g_errword_made;
 static int g_sms[64];
 
 bool pdl_enabled(void)
@@ -33,20 +36,34 @@ bool pdl_enabled(void)
     return on != 0;
 }
 
+// 16 words of the current device that are 0 before anyone can see them.  The first call may come while a stream is being captured, where an
+// allocation is refused unless the thread says that it knows, and where nothing may go to the legacy stream if that stream waits for it.
+static int *make_error_word(void)
+{
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+    int *p = nullptr;
+    cudaStream_t st = nullptr;
+    bool made = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess;
+    if (made) {
+        made = cudaMalloc(&p, 16 * sizeof(int)) == cudaSuccess && cudaMemsetAsync(p, 0, 16 * sizeof(int), st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+        if (p && !made) { cudaFree(p); p = nullptr; }
+        cudaStreamDestroy(st);
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return made ? p : nullptr;
+}
 int *device_error_word(void)
 {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-    if (!g_errword[dev]) {
-        // The first call may come while a stream is being captured, where an allocation is refused unless the thread says that it knows.
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        int *p = nullptr;
-        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
-        const bool made = cudaMalloc(&p, 16 * sizeof(int)) == cudaSuccess && cudaMemset(p, 0, 16 * sizeof(int)) == cudaSuccess;
-        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess || !made) return nullptr;
-        g_errword[dev] = p;
+    int *p = g_errword[dev].load(std::memory_order_acquire);
+    if (!p) {
+        std::lock_guard<std::mutex> one(g_errword_made);               // of two first calls at once one makes it
+        p = g_errword[dev].load(std::memory_order_acquire);
+        if (!p) g_errword[dev].store(p = make_error_word(), std::memory_order_release);
     }
-    return g_errword[dev];
+    return p;
 }
 
 int sm_count(void)

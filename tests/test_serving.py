@@ -916,3 +916,38 @@ def test_attention_dealt_out_in_a_cache_past_32_bits(cuda):
     o, lse = attn.dec_attn_prefix(q, kp, vp, kc, vc, pos, H, win=win)
     ok()
     check_attn(o, lse, attn64(q, kp[:0], vp[:0], k1, v1, pos - P - Tm + keep, H, win))
+
+
+# ------------------------------------------------------------------ the device error word
+_BLOCKING = """
+import sys; sys.path.insert(0, "tests")
+import ctypes, torch
+from cudalm_c_b200 import block, lib
+x = torch.randn(2, 3, 300, device="cuda"); d = torch.zeros(2, 2, device="cuda", dtype=torch.int32)
+u, t = torch.rand(2, 3, device="cuda"), torch.zeros(2, device="cuda")
+x[1, 0, 7] = float("nan"); torch.cuda.synchronize()
+rt, st = ctypes.CDLL("libcudart.so.12"), ctypes.c_void_p()
+assert rt.cudaStreamCreate(ctypes.byref(st)) == 0                # waits for the legacy stream, unlike torch's own
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(st.value)):
+    out = block.dec_verify(x, d, u, t)
+g.replay(); torch.cuda.synchronize()
+assert lib().qlmb_check_device(None) == 4 and b"site 309" in lib().qlmb_last_error(), lib().qlmb_last_error()
+assert lib().qlmb_check_device(None) == 0
+print("reported")
+"""
+
+
+def _fresh_process(code):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    return subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=200)
+
+
+@pytest.mark.gpu
+def test_the_error_word_may_be_made_while_a_blocking_stream_is_captured(cuda):
+    """The first call of a process, on a stream of plain cudaStreamCreate that is being captured: the word exists and is reported into."""
+    r = _fresh_process(_BLOCKING)
+    assert r.returncode == 0 and "reported" in r.stdout, r.stderr[-2000:]
