@@ -38,12 +38,15 @@ __device__ __forceinline__ void lr_mma(float c[4], const uint32_t a[4], uint32_t
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x, y as pairs of bf16: the nearest to them, then the nearest to what that leaves, and so on.  Two terms hold 16 bits, three all 24.
-template <int TERMS> __device__ __forceinline__ void lr_split(float x, float y, uint32_t t[TERMS])
+// x, y as pairs of bf16: the nearest to them, then the nearest to what that leaves, and so on.  Two terms hold 16 bits, three all 24.  LIMIT: above
+// bf16's largest number (an infinity too) every term but the last is that number; without it what is left is inf - inf, a NaN.
+template <int TERMS, bool LIMIT> __device__ __forceinline__ void lr_split(float x, float y, uint32_t t[TERMS])
 {
+    const __nv_bfloat162 top = __halves2bfloat162(__ushort_as_bfloat16(0x7f7f), __ushort_as_bfloat16(0x7f7f));
 #pragma unroll
     for (int k = 0; k < TERMS; k++) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        if (LIMIT && k + 1 < TERMS) h = __hmin2(__hmax2(h, __hneg2(top)), top);
         t[k] = *reinterpret_cast<const uint32_t *>(&h);
         x -= __uint_as_float(t[k] << 16); y -= __uint_as_float(t[k] & 0xffff0000u);
     }
@@ -70,8 +73,8 @@ __device__ __forceinline__ void lr_row(const LoraParams &p, int j, int &m, int &
 
 // c += X A^T for 16 rows (m0: row g, m1: row g + 8 of the thread, -1 for none) and NT tiles of 8 inner columns, over steps of 32 of K:
 // kb, kb + stride, ... below k1.  UK steps are loaded before the first is multiplied.
-template <bool F32, int NT, int UK>
-__device__ __forceinline__ void lr_down(const LoraParams &p, float (&c)[NT][4], const bf16 *A, int ncol, int m0, int m1, int kb, int k1, int stride)
+template <bool F32, int NT, int UK, bool LIMIT>
+__device__ __forceinline__ void lr_down_pass(const LoraParams &p, float (&c)[NT][4], const bf16 *A, int ncol, int m0, int m1, int kb, int k1, int stride)
 {
     constexpr int XT = F32 ? 3 : 1;
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
@@ -109,7 +112,7 @@ __device__ __forceinline__ void lr_down(const LoraParams &p, float (&c)[NT][4], 
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
                         uint32_t t[XT];
-                        lr_split<XT>(__uint_as_float(f[2 * w]), __uint_as_float(f[2 * w + 1]), t);
+                        lr_split<XT, LIMIT>(__uint_as_float(f[2 * w]), __uint_as_float(f[2 * w + 1]), t);
 #pragma unroll
                         for (int i = 0; i < XT; i++) xs[i][e][w] = t[i];
                     }
@@ -125,6 +128,25 @@ __device__ __forceinline__ void lr_down(const LoraParams &p, float (&c)[NT][4], 
                 }
         }
     }
+}
+
+// The same from c = 0.  fp32 rows whose sums are no numbers are taken once more with limited terms (limits at all times: 7 % of 8192 fp32 rows).
+template <bool F32, int NT, int UK>
+__device__ __forceinline__ void lr_down(const LoraParams &p, float (&c)[NT][4], const bf16 *A, int ncol, int m0, int m1, int kb, int k1, int stride)
+{
+    lr_down_pass<F32, NT, UK, false>(p, c, A, ncol, m0, m1, kb, k1, stride);
+    if (!F32) return;
+    bool odd = false;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) odd |= c[t][k] != c[t][k];
+    if (__builtin_expect(!__any_sync(~0u, odd), 1)) return;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) c[t][k] = 0.0f;
+    lr_down_pass<F32, NT, 1, true>(p, c, A, ncol, m0, m1, kb, k1, stride);
 }
 
 // Columns n0 .. n0 + 63 of 16 rows: base + T B.  A thread asks for B's rows r0 + 2 q, + 1, + 8, + 9, columns n0 + 8 g .. n0 + 8 g + 7.
@@ -236,6 +258,7 @@ __device__ __forceinline__ void lt_ldmt(uint32_t a, uint32_t v[4])
 // SMALL (R <= 64): a warp keeps the terms of its 16 rows in registers while it goes through the columns.
 // blockIdx.z: a tile's adapters are dealt out to LT_Z CTAs, so that the tiles at the border of two prompts take no longer than the others.
 constexpr int LT_Z = 4;
+template <bool B> struct LtFlag { static constexpr bool value = B; };
 template <bool F32, bool SMALL> __global__ void __launch_bounds__(256, 2) k_lora_tile(const __grid_constant__ LoraParams p)
 {
     constexpr int XT = F32 ? 3 : 1, TT = F32 ? 3 : 2, XB = lt_x<F32>(), STAGE = XB + LT_W, XP = F32 ? 16 : 8, EB = F32 ? 4 : 2;   // XP: pieces of a row of 64
@@ -272,7 +295,7 @@ template <bool F32, bool SMALL> __global__ void __launch_bounds__(256, 2) k_lora
 #pragma unroll
         for (int i = 0; i < NX; i++) xrow[i] = srow[xr + 256 / XP * i];
         // ---- inner numbers: 64 of K at a time, block of 64 inner columns by block
-        int lrc = 0, lk = 0, ls = 0;                      // the next step to be requested, and its stage
+        int lrc, lk, ls;                                  // the next step to be requested, and its stage
         const auto load1 = [&]() {
             if (lrc < p.R) {
                 const int k = lk + xc * (16 / EB), kw = lk + wc * 8;
@@ -294,63 +317,68 @@ template <bool F32, bool SMALL> __global__ void __launch_bounds__(256, 2) k_lora
             ls = (ls + 1) % LT_NS;
             lt_commit();
         };
-        for (int st = 0; st < LT_NS - 1; st++) load1();
         float c[4][4] = {};
-        for (int st = 0, rc = 0, k0 = 0; rc < p.R; st = (st + 1) % LT_NS) {
-            lt_wait<LT_NS - 2>();
-            __syncthreads();                              // the step has landed for everyone, and everyone is done with the one before
-            load1();
-            const uint8_t *sx = lt_s + st * STAGE, *sw = sx + XB;
+        const auto inner = [&](auto limit) {              // true where a sum is no number
+            lrc = lk = ls = 0;
+            for (int st = 0; st < LT_NS - 1; st++) load1();
+            bool odd = false;
+            for (int st = 0, rc = 0, k0 = 0; rc < p.R; st = (st + 1) % LT_NS) {
+                lt_wait<LT_NS - 2>();
+                __syncthreads();                              // the step has landed for everyone, and everyone is done with the one before
+                load1();
+                const uint8_t *sx = lt_s + st * STAGE, *sw = sx + XB;
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                uint32_t x[XT][4], w[2][4];
-                if (F32) {
+                for (int s = 0; s < 4; s++) {
+                    uint32_t x[XT][4], w[2][4];
+                    if (F32) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                        for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const int r = rg + g + 8 * e, k = 16 * s + 8 * h + 2 * q;
-                            const float2 f = *reinterpret_cast<const float2 *>(sx + r * 256 + (((k >> 2) ^ (r & 7)) << 4) + (k & 3) * 4);
-                            uint32_t t[XT];
-                            lr_split<XT>(f.x, f.y, t);
+                            for (int e = 0; e < 2; e++) {
+                                const int r = rg + g + 8 * e, k = 16 * s + 8 * h + 2 * q;
+                                const float2 f = *reinterpret_cast<const float2 *>(sx + r * 256 + (((k >> 2) ^ (r & 7)) << 4) + (k & 3) * 4);
+                                uint32_t t[XT];
+                                lr_split<XT, decltype(limit)::value>(f.x, f.y, t);
 #pragma unroll
-                            for (int i = 0; i < XT; i++) x[i][2 * h + e] = t[i];
-                        }
-                } else {
-                    const int r = rg + (lane & 15), cc = 2 * s + (lane >> 4);
-                    lt_ldm(lt_addr(sx + r * 128 + ((cc ^ (r & 7)) << 4)), x[0]);
+                                for (int i = 0; i < XT; i++) x[i][2 * h + e] = t[i];
+                            }
+                    } else {
+                        const int r = rg + (lane & 15), cc = 2 * s + (lane >> 4);
+                        lt_ldm(lt_addr(sx + r * 128 + ((cc ^ (r & 7)) << 4)), x[0]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {             // two tiles of 8 inner columns: rows of A, their 16 elements of K in two pieces
+                        const int r = nh + 16 * t + (lane & 7) + 8 * (lane >> 4), cc = 2 * s + ((lane >> 3) & 1);
+                        lt_ldm(lt_addr(sw + r * 128 + ((cc ^ (r & 7)) << 4)), w[t]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int i = XT - 1; i >= 0; i--) lr_mma(c[t], x[i], w[t >> 1][2 * (t & 1)], w[t >> 1][2 * (t & 1) + 1]);
                 }
+                k0 += 64;
+                if (k0 >= p.K) {                              // the block's sums are whole
 #pragma unroll
-                for (int t = 0; t < 2; t++) {             // two tiles of 8 inner columns: rows of A, their 16 elements of K in two pieces
-                    const int r = nh + 16 * t + (lane & 7) + 8 * (lane >> 4), cc = 2 * s + ((lane >> 3) & 1);
-                    lt_ldm(lt_addr(sw + r * 128 + ((cc ^ (r & 7)) << 4)), w[t]);
+                    for (int t = 0; t < 4; t++) {
+                        const int col = rc + nh + 8 * t;
+                        if (col < p.R)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                uint32_t v[TT];
+                                lr_split<TT, true>(c[t][2 * e] * scale, c[t][2 * e + 1] * scale, v);
+#pragma unroll
+                                for (int i = 0; i < TT; i++) ts[(i * LT_M + rg + g + 8 * e) * ldt + col / 2 + q] = v[i];
+                            }
+#pragma unroll
+                        for (int k = 0; k < 4; k++) { odd |= c[t][k] != c[t][k]; c[t][k] = 0.0f; }
+                    }
+                    k0 = 0; rc += 64;
                 }
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int i = XT - 1; i >= 0; i--) lr_mma(c[t], x[i], w[t >> 1][2 * (t & 1)], w[t >> 1][2 * (t & 1) + 1]);
             }
-            k0 += 64;
-            if (k0 >= p.K) {                              // the block's sums are whole
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int col = rc + nh + 8 * t;
-                    if (col < p.R)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            uint32_t v[TT];
-                            lr_split<TT>(c[t][2 * e] * scale, c[t][2 * e + 1] * scale, v);
-#pragma unroll
-                            for (int i = 0; i < TT; i++) ts[(i * LT_M + rg + g + 8 * e) * ldt + col / 2 + q] = v[i];
-                        }
-#pragma unroll
-                    for (int k = 0; k < 4; k++) c[t][k] = 0.0f;
-                }
-                k0 = 0; rc += 64;
-            }
-        }
-        lt_wait<0>();
-        __syncthreads();
+            lt_wait<0>();
+            return __syncthreads_or(odd);
+        };
+        if (inner(LtFlag<false>()) && F32) inner(LtFlag<true>());        // (as in lr_down)
         // ---- Y: 64 inner indices at a time, block of 64 columns by block; the base comes with a block's last step
         int ln = c0;
         lrc = 0; ls = 0;
@@ -702,7 +730,7 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
                         uint32_t t[2];
-                        lr_split<2>(__uint_as_float(v[2 * k]) * scale, __uint_as_float(v[2 * k + 1]) * scale, t);
+                        lr_split<2, true>(__uint_as_float(v[2 * k]) * scale, __uint_as_float(v[2 * k + 1]) * scale, t);
                         hi[k] = t[0]; lo[k] = t[1];
                     }
                     tmem_st16(tT + lanes + c / 2, hi);
@@ -816,7 +844,7 @@ template <bool F32, int NT, int UK> __global__ void __launch_bounds__(256) k_lor
 #pragma unroll
             for (int k = 0; k < 8; k++) { const float2 v = *reinterpret_cast<const float2 *>(&red[k][r][col]); x += v.x; y += v.y; }
             uint32_t t[TT];
-            lr_split<TT>(x * scale, y * scale, t);
+            lr_split<TT, true>(x * scale, y * scale, t);
 #pragma unroll
             for (int k = 0; k < TT; k++) ts[(k * 16 + r) * ldt + col / 2] = t[k];
         }
@@ -1032,7 +1060,7 @@ template <bool F32, bool NARROW, bool AHEAD> __global__ void __launch_bounds__(1
 #pragma unroll 8
                 for (int s = 0; s < p.S; s++) { const float2 v = *reinterpret_cast<const float2 *>(src + (size_t)s * p.M * p.R); x += v.x; y += v.y; }
                 uint32_t t[TT];
-                lr_split<TT>(x * scale, y * scale, t);
+                lr_split<TT, true>(x * scale, y * scale, t);
 #pragma unroll
                 for (int k = 0; k < TT; k++) ts[(k * 16 + r) * ldt + col / 2] = t[k];
             }

@@ -951,3 +951,62 @@ def test_the_error_word_may_be_made_while_a_blocking_stream_is_captured(cuda):
     """The first call of a process, on a stream of plain cudaStreamCreate that is being captured: the word exists and is reported into."""
     r = _fresh_process(_BLOCKING)
     assert r.returncode == 0 and "reported" in r.stdout, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------ adapters: values that are not finite, in every form
+FORMS = [
+    # M, K, N, R, adapters, order: one launch; two launches with one or two rows of an adapter, with more, of a larger rank; tiles of 64 rows; of 128
+    (20, 72, 136, 8, 3, False), (24, 72, 136, 64, 3, False), (40, 1032, 4104, 16, 37, False), (40, 1032, 4104, 16, 4, False), (40, 1032, 2056, 72, 37, False), (40, 1032, 2056, 72, 4, True),
+    (300, 256, 136, 16, 5, False), (2100, 72, 136, 24, 5, False), (2100, 136, 72, 48, 5, True), (2060, 72, 136, 136, 5, True), (600, 72, 136, 32, 5, False), (2100, 264, 72, 128, 5, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,R,n,ordered", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lora_takes_infinities_for_what_they_are(cuda, M, K, N, R, n, ordered, dtype):
+    """Adapters of positive numbers: a row with an infinity is that infinity throughout, one with the type's largest number, which the
+    adapter makes small, is finite."""
+    from cudalm_c_b200 import linear
+    X, base, A, Bm, scale = make_lora(M, K, N, R, n, dtype, 71, cuda)
+    X, A, Bm = X.abs() + 0.125, A.abs() + 0.125, Bm.abs() + 0.125
+    adapter = (torch.arange(M, device=cuda, dtype=torch.int32) * 7) % n
+    top = torch.finfo(dtype).max
+    A[:, :, 5] = 2.0 ** -100
+    up, down, large = 3, M - 1, M // 2
+    X[up, 9], X[down, K - 1] = math.inf, -math.inf
+    X[large] = 0
+    X[large, 5] = top
+    order = linear.lora_order(adapter) if ordered else None
+    y = linear.lora_add(X, base, A, Bm, scale, adapter, order=order)
+    ok()
+    assert bool((y[up] == math.inf).all()) and bool((y[down] == -math.inf).all())
+    odd = torch.zeros(M, dtype=torch.bool, device=cuda)
+    odd[up] = odd[down] = True
+    check_lora(torch.where(odd[:, None], base, y), X, base, A, Bm, scale, torch.where(odd, torch.full_like(adapter, -1), adapter))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,R,n,ordered", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("place", ["new", "in place"])
+def test_lora_keeps_infinities_apart_in_every_form(cuda, M, K, N, R, n, ordered, dtype, place):
+    """An adapter with a NaN and an infinity and a row of infinities reach nobody else's rows, nor do rows without an adapter."""
+    from cudalm_c_b200 import linear
+    X, base, A, Bm, scale = make_lora(M, K, N, R, n, dtype, 72, cuda)
+    adapter = (torch.arange(M, device=cuda, dtype=torch.int32) * 5) % (n + 1) - 1
+    A[2, 3], Bm[2, 5], X[1] = math.nan, math.inf, math.inf
+    if M > 100:
+        adapter[64:96] = 1                                 # tiles with several adapters, and a whole piece of one
+        X[70] = math.nan
+    order = linear.lora_order(adapter) if ordered else None
+    out = base.clone() if place == "in place" else None
+    b = out if out is not None else base
+    y = linear.lora_add(X, b, A, Bm, scale, adapter, order=order, out=out)
+    ok()
+    odd = adapter == 2
+    odd[1] = adapter[1] >= 0
+    if M > 100:
+        odd[70] = True
+    assert bool(torch.isfinite(y[~odd].float()).all()) and not bool(torch.isfinite(y[odd].float()).any())
+    check_lora(torch.where(odd[:, None], base, y), X, base, A, Bm, scale, torch.where(odd, torch.full_like(adapter, -1), adapter))
