@@ -1010,3 +1010,28 @@ def test_lora_keeps_infinities_apart_in_every_form(cuda, M, K, N, R, n, ordered,
         odd[70] = True
     assert bool(torch.isfinite(y[~odd].float()).all()) and not bool(torch.isfinite(y[odd].float()).any())
     check_lora(torch.where(odd[:, None], base, y), X, base, A, Bm, scale, torch.where(odd, torch.full_like(adapter, -1), adapter))
+
+
+# ------------------------------------------------------------------ verification: sums of large vocabularies, masks at any temperature
+@pytest.mark.gpu
+@pytest.mark.parametrize("low,T", [(-2.8125, 1.0), (-1.5, 1.0), (-1.40625, 0.5)])
+def test_verify_sums_a_large_vocabulary(cuda, low, T):
+    """128 tokens of every 2^16 ahead of the others, which are equal: a lane of a warp has one or more of the former and some 2000 of the
+    latter.  A draft is taken and refused as its u lies 2^-19 on
+    either side of its probability: weights are off by 2^-21.7 (the exponent's two roundings, 2^x to 2 ulp), a step's 16 terms in fp32 by
+    (2 + .. + 16) / 16 2^-24 = 2^-20.9."""
+    from cudalm_c_b200 import block
+    V = 1 << 22
+    lg = torch.full((2, 2, V), low, device=cuda)
+    lg.view(2, 2, -1, 1 << 16)[:, :, :, :128] = 0
+    ahead = 128 * (V >> 16)
+    p0 = 1.0 / (ahead + (V - ahead) * math.exp(low / T))
+    u = torch.tensor([[p0 * (1 - 2.0 ** -19), 0.5], [p0 * (1 + 2.0 ** -19), 0.5]], dtype=torch.float64, device=cuda).float()
+    x = torch.zeros(2, 1, dtype=torch.int32, device=cuda)
+    out, count, lp = block.dec_verify(lg, x, u, torch.full((2,), T, device=cuda))
+    ok()
+    assert count.tolist() == [2, 1] and int(out[0, 0]) == 0 and int(out[1, 0]) > 0
+    z1 = math.log(ahead + (V - ahead) * math.exp(low))     # log-probabilities at temperature 1
+    want = torch.tensor([-z1, float(lg[1, 0, int(out[1, 0])]) - z1], dtype=torch.float64)
+    have = torch.stack((lp[0, 0], lp[1, 0])).cpu().double()
+    assert bool(((have - want).abs() <= 2.0 ** -20 * (1 + want.abs())).all()), (have, want)
