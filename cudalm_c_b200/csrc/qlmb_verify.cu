@@ -112,8 +112,9 @@ template <bool BF, bool VEC, int VF_W> __global__ void __cluster_dims__(VF_C, 1,
     }
     const float temp = p.temp[b], un = p.u[(size_t)b * (n + 1) + n];
     const bool greedy = !(temp > 0.0f);
-    const double it = greedy ? 1.4426950408889634 : 1.4426950408889634 / fmin((double)temp, 1e30);      // an infinite one: every finite logit has the weight 1
-    const VfScale cT = vf_scale2(fmin(it, 1e38));
+    // (an infinite temperature: every logit but -inf has the weight 1, a mask of fp32's lowest number too)
+    const double it = greedy ? 1.4426950408889634 : fmin(fmax(1.4426950408889634 / (double)temp, 1.5e-45), 1e38);
+    const VfScale cT = vf_scale2(it);
     constexpr float c1 = 1.4426950408889634f;             // (log-probabilities are fp32 numbers)
     const bool unit = greedy || temp == 1.0f;             // the two sums are one
     // runs of whole groups of four

@@ -1035,3 +1035,21 @@ def test_verify_sums_a_large_vocabulary(cuda, low, T):
     want = torch.tensor([-z1, float(lg[1, 0, int(out[1, 0])]) - z1], dtype=torch.float64)
     have = torch.stack((lp[0, 0], lp[1, 0])).cpu().double()
     assert bool(((have - want).abs() <= 2.0 ** -20 * (1 + want.abs())).all()), (have, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 40001])
+def test_verify_masks_of_the_lowest_number(cuda, V):
+    """Logits of fp32's lowest number have no weight at ordinary temperatures, large ones too, and that of any other number at an infinite one."""
+    from cudalm_c_b200 import block
+    B = 6
+    lg, x, u, temp, _ = make_verify(B, 0, V, V, torch.float32, False, 81, cuda)
+    lg[:, 0, :V - 7] = torch.finfo(torch.float32).min
+    temp[:] = torch.tensor([1.0, 1e-30, 1e30, 1e36, math.inf, math.inf], device=cuda)
+    out, count, lp = block.dec_verify(lg, x, u, temp)
+    ok()
+    want = verify64(lg[:4], x[:4], u[:4], temp[:4], None, None, V)
+    check_verify((out[:4], count[:4], lp[:4]), want)
+    # all weights 1 (to 2^-20, the masked ones): the token is the one in which u V falls
+    for b in (4, 5):
+        assert abs(int(out[b, 0]) - float(u[b, 0]) * V) <= 1 + V * 2.0 ** -19
