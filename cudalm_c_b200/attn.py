@@ -1,5 +1,7 @@
 """Host-side mirror of the reference's attention operators (e_attn, cudalm.cu:3705-3730, and the
 attention part of gpu_backward, cudalm.cu:5918-5960) over the C ABI."""
+from functools import lru_cache
+
 import torch
 
 from ._lib import calls, check, device_index, lib, need, ptr, stream_ptr
@@ -26,7 +28,10 @@ def attn_bwd(Q, K, V, O, dA, lse, B, T, H, KV, win=0, rope=None):
     return dQ, dK, dV, drow
 
 
-_prefix_ws = {}                                          # bytes of dec_attn_prefix's scratch by device and shape
+@lru_cache(maxsize=1024)                                 # a ctypes call, 2 us; a server's shapes change from step to step
+def _prefix_bytes(dev, *shape):
+    """Bytes of dec_attn_prefix's scratch on a device, for (B, n, P, Tm, H, KV)."""
+    return lib().qlmb_dec_attn_prefix_bytes(*shape)
 
 
 def _dec_attn_prefix_args(Q, Kp, Vp, Kc, Vc, pos, H):
@@ -50,9 +55,7 @@ def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
         _dec_attn_prefix_args(Q, Kp, Vp, Kc, Vc, pos, H)
     rows, _, B, Tm, KD, P = got
     shape = (B, rows // B, P, Tm, H, KD // 64)
-    nbytes = _prefix_ws.get((dev, shape))
-    if nbytes is None:
-        nbytes = _prefix_ws[(dev, shape)] = lib().qlmb_dec_attn_prefix_bytes(*shape)
+    nbytes = _prefix_bytes(dev, *shape)
     O = torch.empty_like(Q)
     lse = torch.empty_strided((rows, H), (H, 1), dtype=torch.float32, device=Q.device)         # (torch.empty: 0.9 us more)
     ws = Q.new_empty(nbytes + 1 >> 1) if nbytes > 16 else None

@@ -4,6 +4,8 @@
 `layout` says how the 4-bit codes are stored relative to Y = X W:
 KN = codes of W[K,N] (the reference's own [in,out] storage, applied with g_ab),
 NK = codes of W[N,K] (applied with g_abt)."""
+from functools import lru_cache
+
 import torch
 
 from ._lib import BF16, F32, KN, NK, Qkv, calls, check, device_index, lib, need, ptr, stream_ptr  # noqa: F401
@@ -79,7 +81,10 @@ def lora_order(adapter):
     return torch.argsort(adapter, stable=True).to(torch.int32)
 
 
-_lora_ws = {}                                            # bytes of lora_add's scratch by device and shape
+@lru_cache(maxsize=1024)                                 # a ctypes call, 2 us; a server's shapes change from step to step
+def _lora_bytes(dev, *shape):
+    """Bytes of lora_add's scratch on a device, for (M, K, N, R)."""
+    return lib().qlmb_lora_bytes(*shape)
 
 
 def _lora_add_args(X, base, A, Bm, scale, adapter, order, out):
@@ -110,9 +115,7 @@ def lora_add(X, base, A, Bm, scale, adapter, order=None, out=None):
     if M == 0:
         return out
     shape = (M, K, N, R)
-    nbytes = _lora_ws.get((dev, shape))
-    if nbytes is None:
-        nbytes = _lora_ws[(dev, shape)] = lib().qlmb_lora_bytes(*shape)
+    nbytes = _lora_bytes(dev, *shape)
     ws = Bm.new_empty(nbytes + 1 >> 1) if nbytes > 16 else None
     calls.lora_add(out, X, base, F32 if dt is torch.float32 else BF16, A, Bm, scale, n, adapter, order, M, K, N, R, ws, nbytes, stream_ptr())
     return out

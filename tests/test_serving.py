@@ -1053,3 +1053,12 @@ def test_verify_masks_of_the_lowest_number(cuda, V):
     # all weights 1 (to 2^-20, the masked ones): the token is the one in which u V falls
     for b in (4, 5):
         assert abs(int(out[b, 0]) - float(u[b, 0]) * V) <= 1 + V * 2.0 ** -19
+
+
+def test_the_mirrors_keep_few_sizes():
+    """Batches and prompts change from step to step: what the mirrors keep by shape has an end."""
+    from cudalm_c_b200 import attn, linear
+    for i in range(1, 3000):
+        assert attn._prefix_bytes(0, 1, 1, i, 64, 1, 1) > 0 and linear._lora_bytes(0, i, 64, 64, 8) > 0
+    assert attn._prefix_bytes(0, 1, 65, 8, 8, 2, 2) == 0 and linear._lora_bytes(0, 4, 60, 64, 8) == 0
+    assert attn._prefix_bytes.cache_info().currsize <= 1024 and linear._lora_bytes.cache_info().currsize <= 1024
