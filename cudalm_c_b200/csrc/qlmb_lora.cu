@@ -1249,6 +1249,9 @@ extern "C" int qlmb_lora_add(void *Y, const void *X, const void *base, int dtype
                  "qlmb_lora_add: rows, adapters and workspace must be 16-byte aligned");
     const size_t need = qlmb_lora_bytes(M, K, N, R);
     QLMB_REQUIRE(need <= 16 || (ws && ws_bytes >= need), "qlmb_lora_add: a workspace of %zu bytes, %zu are needed", ws_bytes, need);
+    // Rows are read while others are written.
+    const uintptr_t es = dtype == QLMB_F32 ? 4 : 2, y = (uintptr_t)Y, ny = (uintptr_t)M * N * es, x = (uintptr_t)X, b = (uintptr_t)base;
+    QLMB_REQUIRE((y + ny <= x || x + (uintptr_t)M * K * es <= y) && (Y == base || y + ny <= b || b + ny <= y), "qlmb_lora_add: Y overlaps X, or the base without being it");
     LoraParams p = {Y, X, base, (const bf16 *)A, (const bf16 *)Bm, scale, adapter, order, (float *)ws, M, K, N, R, adapters, 0, 0, device_error_word()};
     LoraForm form = lora_form(M, K, N, R, &p.S, &p.kslice);
     if (dtype == QLMB_BF16 && !order && lora_tc_ok(M, K, N, R, adapters)) form = LORA_TC;

@@ -697,7 +697,7 @@ int qlmb_dec_verify(int *out, int *count, float *lp, const void *logits, int lg_
                     const int *draft, const int *nd, const float *u, const float *temp, int B, int n, int V, void *stream);
 /* Low-rank adapters of many requests beside a projection their rows share (qlmb_linear_fwd, qlmb_gemv_decode):
  * Y[m,:] = base[m,:] + scale[a] * (X[m,:] A[a]^T) Bm[a] with a = adapter[m], Y[m,:] = base[m,:] where a is -1.  X [M][K], base and Y
- * [M][N] of `dtype` (Y may be base, not X); A [adapters][R][K] and Bm [adapters][R][N] bf16; scale [adapters]; adapter [M] (device).
+ * [M][N] of `dtype` (Y may be base; else it overlaps neither); A [adapters][R][K] and Bm [adapters][R][N] bf16; scale [adapters]; adapter [M] (device).
  * order (may be NULL): the rows 0 .. M-1 in the order of their adapters; without it rows in any order give the same result, but
  * 16 neighbouring rows (of many: 64 or 128) cost as many passes as they have adapters.  K, N and R multiples of 8, R <= 256
  * (adapters of a lower rank: zero rows).  Pointers to rows, adapters and ws 16-byte aligned; ws: qlmb_lora_bytes(...) bytes (0: not

@@ -1062,3 +1062,16 @@ def test_the_mirrors_keep_few_sizes():
         assert attn._prefix_bytes(0, 1, 1, i, 64, 1, 1) > 0 and linear._lora_bytes(0, i, 64, 64, 8) > 0
     assert attn._prefix_bytes(0, 1, 65, 8, 8, 2, 2) == 0 and linear._lora_bytes(0, 4, 60, 64, 8) == 0
     assert attn._prefix_bytes.cache_info().currsize <= 1024 and linear._lora_bytes.cache_info().currsize <= 1024
+
+
+def test_lora_refuses_a_result_over_its_rows():
+    """Rows are read while others are written: Y may be the base as a whole, nothing else."""
+    L, ws = _lib(), ctypes.c_void_p(1 << 30)
+
+    def lora(Y, X, base, dtype=1, M=4, K=64, N=128):
+        return L.qlmb_lora_add(ctypes.c_void_p(Y), ctypes.c_void_p(X), ctypes.c_void_p(base), dtype, ws, ws, ws, 2, ws, None, M, K, N, 8, ws, ctypes.c_size_t(1 << 30), None)
+
+    big, far = 1 << 20, 1 << 24
+    # Y of 4 x 128 and X of 4 x 64 bf16: 1024 and 512 bytes
+    for y, x, base, dtype in ((big, big + 1008, far, 1), (big, big - 496, far, 1), (big, big + 2032, far, 0), (big, far, big + 1008, 1), (big, far, big - 16, 1), (big, big + 256, big, 1)):
+        assert lora(y, x, base, dtype) == 1 and b"overlaps" in L.qlmb_last_error(), (y, x, base, dtype, L.qlmb_last_error())
