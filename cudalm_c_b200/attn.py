@@ -51,9 +51,11 @@ def dec_attn_prefix(Q, Kp, Vp, Kc, Vc, pos, H, win=0):
     the scores' log-sum-exp [B*n, H] fp32."""
     dev = device_index()
     got = calls.sizes(dev, torch.bfloat16, Q, "rw", Kc, "btk", Vc, "btk", Kp, "pk", Vp, "pk", torch.int32, pos, "b")
-    if got is None or not (got[1] == H * 64 and got[4] % 64 == 0 and got[2] > 0 and got[0] > 0 and got[0] % got[2] == 0):
+    if got is None or not (got[1] == H * 64 and got[4] % 64 == 0 and (got[0] % got[2] == 0 < got[0] if got[2] else got[0] == 0)):
         _dec_attn_prefix_args(Q, Kp, Vp, Kc, Vc, pos, H)
     rows, _, B, Tm, KD, P = got
+    if B == 0:
+        return torch.empty_like(Q), Q.new_empty((0, H), dtype=torch.float32)
     shape = (B, rows // B, P, Tm, H, KD // 64)
     nbytes = _prefix_bytes(dev, *shape)
     O = torch.empty_like(Q)

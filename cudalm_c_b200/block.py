@@ -154,9 +154,11 @@ def dec_rope_kv(q, k, v, Kc, Vc, cosb, sinb, pos, H, P=0, out=None):
     if out is None and isinstance(q, torch.Tensor):
         out = torch.empty_like(q)
     got = calls.sizes(dev, torch.bfloat16, q, "rw", out, "rw", Kc, "btk", Vc, "btk", k, "rk", v, "rk", torch.float32, cosb, "x5", sinb, "x5", torch.int32, pos, "b")
-    if got is None or not (got[1] == H * 64 and got[4] % 64 == 0 and got[2] > 0 and got[0] > 0 and got[0] % got[2] == 0):
+    if got is None or not (got[1] == H * 64 and got[4] % 64 == 0 and (got[0] % got[2] == 0 < got[0] if got[2] else got[0] == 0)):
         _dec_rope_kv_args(q, k, v, Kc, Vc, cosb, sinb, pos, H, out)
     rows, _, B, Tm, KD, Tr = got
+    if B == 0:
+        return out
     calls.dec_rope_kv(out, Kc, Vc, q, k, v, cosb, sinb, pos, B, rows // B, P, Tm, H, KD // 64, 64, Tr, stream_ptr())
     return out
 
@@ -181,13 +183,15 @@ def dec_verify(logits, draft, u, temp, q=None, nd=None, V=None):
     dev = device_index()
     dt = torch.bfloat16 if getattr(logits, "dtype", None) is torch.bfloat16 else torch.float32
     got = calls.sizes(dev, dt, logits, "bml", torch.float32, u, "bm", temp, "b", torch.int32, draft, "bn", nd, "?b", torch.float32, q, "?bnq")
-    if got is None or not (got[0] > 0 and got[3] == got[1] - 1):
+    if got is None or got[3] != got[1] - 1:
         _dec_verify_args(logits, draft, u, temp, q, nd, V)
     B, n1, ld, n = got[:4]
     ldq = got[4] if q is not None else 0
     out = torch.empty_like(u, dtype=torch.int32)
     count = draft.new_empty(B)
     lp = torch.empty_like(u)
+    if B == 0:
+        return out, count, lp
     calls.dec_verify(out, count, lp, logits, F32 if dt is torch.float32 else BF16, ld, q if n else None, ldq, draft if n else None, nd, u, temp,
                      B, n, ld if V is None else V, stream_ptr())
     return out, count, lp

@@ -1075,3 +1075,24 @@ def test_lora_refuses_a_result_over_its_rows():
     # Y of 4 x 128 and X of 4 x 64 bf16: 1024 and 512 bytes
     for y, x, base, dtype in ((big, big + 1008, far, 1), (big, big - 496, far, 1), (big, big + 2032, far, 0), (big, far, big + 1008, 1), (big, far, big - 16, 1), (big, big + 256, big, 1)):
         assert lora(y, x, base, dtype) == 1 and b"overlaps" in L.qlmb_last_error(), (y, x, base, dtype, L.qlmb_last_error())
+
+
+@pytest.mark.gpu
+def test_an_empty_batch(cuda):
+    """A step without slots gives empty results, as lora_add does; rows without slots and slots without rows are refused."""
+    from cudalm_c_b200 import attn, block, linear
+    bf = torch.bfloat16
+    q, k, kp, kc = (torch.zeros(s, dtype=bf, device=cuda) for s in ((0, 256), (0, 128), (9, 128), (0, 8, 128)))
+    pos, tab = torch.zeros(0, dtype=torch.int32, device=cuda), torch.zeros(16, 32, device=cuda)
+    assert block.dec_rope_kv(q, k, k, kc, kc, tab, tab, pos, 4, P=9).shape == (0, 256)
+    o, lse = attn.dec_attn_prefix(q, kp, kp, kc, kc, pos, 4)
+    assert o.shape == (0, 256) and o.dtype == bf and lse.shape == (0, 4) and lse.dtype == torch.float32
+    out, count, lp = block.dec_verify(torch.zeros(0, 3, 50, device=cuda), torch.zeros(0, 2, dtype=torch.int32, device=cuda), torch.zeros(0, 3, device=cuda), torch.zeros(0, device=cuda))
+    assert out.shape == lp.shape == (0, 3) and count.shape == (0,) and out.dtype == count.dtype == torch.int32
+    A = torch.zeros(2, 8, 256, dtype=bf, device=cuda)
+    assert linear.lora_add(q, q, A, A, torch.zeros(2, device=cuda), pos).shape == (0, 256)
+    ok()
+    rows, one = torch.zeros(2, 256, dtype=bf, device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    for args in ((rows, kp, kp, kc, kc, pos, 4), (q, kp, kp, torch.zeros(1, 8, 128, dtype=bf, device=cuda), torch.zeros(1, 8, 128, dtype=bf, device=cuda), one, 4)):
+        with pytest.raises(ValueError, match="dec_attn_prefix"):
+            attn.dec_attn_prefix(*args)
