@@ -1096,3 +1096,39 @@ def test_an_empty_batch(cuda):
     for args in ((rows, kp, kp, kc, kc, pos, 4), (q, kp, kp, torch.zeros(1, 8, 128, dtype=bf, device=cuda), torch.zeros(1, 8, 128, dtype=bf, device=cuda), one, 4)):
         with pytest.raises(ValueError, match="dec_attn_prefix"):
             attn.dec_attn_prefix(*args)
+
+
+_COLD = """
+import sys; sys.path.insert(0, "tests")
+import torch
+from cudalm_c_b200 import attn, linear
+import test_serving as t
+dev = torch.device("cuda:0")
+calls = []
+for B, n, H, KV, P, Tm in ((2, 2, 4, 2, 100, 40), (40, 4, 4, 2, 300, 60), (16, 5, 16, 4, 5003, 40)):
+    at = t.make_attn(B, n, H, KV, P, Tm, 91, dev)
+    pos = t.positions(B, n, P, Tm, 92, dev)
+    calls.append((lambda at=at, pos=pos, H=H: attn.dec_attn_prefix(*at, pos, H), lambda o, lse, at=at, pos=pos, H=H: t.check_attn(o, lse, t.attn64(*at, pos, H, 0))))
+bf, f32 = torch.bfloat16, torch.float32
+for M, K, N, R, n, dt in ((20, 72, 136, 8, 3, bf), (40, 1032, 4104, 16, 37, bf), (40, 1032, 2056, 72, 4, f32), (2100, 72, 136, 24, 5, f32), (2100, 136, 72, 72, 5, bf),
+                          (2100, 264, 72, 128, 5, bf)):
+    lo = t.make_lora(M, K, N, R, n, dt, 93, dev)
+    ad = (torch.arange(M, device=dev, dtype=torch.int32) * 3) % n
+    calls.append((lambda lo=lo, ad=ad: (linear.lora_add(*lo, ad),), lambda y, lo=lo, ad=ad: t.check_lora(y, *lo, ad)))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = [f() for f, _ in calls]
+g.replay(); t.ok()
+for (f, check), out in zip(calls, got):
+    assert all(torch.equal(a, b) for a, b in zip(out, f()))
+    check(*out)
+t.ok(); print("equal")
+"""
+
+
+@pytest.mark.gpu
+def test_every_form_may_be_captured_before_it_ever_ran(cuda):
+    """The first calls of a process under capture, for every kernel with an attribute or tensor maps of its own."""
+    r = _fresh_process(_COLD)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
