@@ -664,12 +664,12 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
         const uint64_t x00 = make_desc(smem_u32(lc_s), 16, 1024), a00 = make_desc(smem_u32(lc_s) + 128 * 128, 16, 1024), b00 = make_desc(smem_u32(lc_s) + 128 * 128, 8192, 1024);
         int nb = 0, np = 0;                   // blocks, pairs with an adapter
         while (!bad && next()) {
-            if (w.cur < 0) { advance(b1 - b0); continue; }
-            for (int k = 0; k < 4 && !bad; k++) {         // D takes the place of the last pair's sums
+            const bool adapted = w.cur >= 0;
+            for (int k = 0; k < 4 && !bad && adapted; k++) {             // D takes the place of the last pair's sums
                 const int uses = (nb - k + 3) / 4;
                 if (uses > 0) bad = at_all_wait(smem_u32(&d2_empty[k]), (uint32_t)(uses - 1) & 1u, abort_flag, 162);
             }
-            for (int i = 0; i < steps && !bad; i++) {
+            for (int i = 0; i < steps && !bad && adapted; i++) {
                 if ((bad = at_all_wait(smem_u32(&full[s]), phase, abort_flag, 163))) break;
                 tc_fence_after();
                 const uint64_t o = (uint64_t)(s * (STAGE / 16));
@@ -683,8 +683,10 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
                 __syncwarp();
                 advance(1);
             }
-            if (bad || (bad = at_all_wait(smem_u32(t_full), (uint32_t)np & 1u, abort_flag, 164))) break;
-            np++;
+            if (bad || (adapted && (bad = at_all_wait(smem_u32(t_full), (uint32_t)np & 1u, abort_flag, 164)))) break;
+            if (adapted) np++;
+            // Blocks without an adapter, too, go through here: a wait tells a stage's turn from the one two before it only if the warp saw
+            // the one in between.
             for (int b = b0; b < b1; b++, nb++) {
                 const int buf = nb & 3;
                 if ((bad = at_all_wait(smem_u32(&full[s]), phase, abort_flag, 165))) break;
@@ -692,11 +694,13 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
                 tc_fence_after();
                 const uint64_t o = (uint64_t)(s * (STAGE / 16));
                 if (elect_one()) {
-                    for (int k = 0; k < p.R / 16; k++) {
-                        tc_mma_bf16_ta(tD + 64 * buf, tT + k * 8, b00 + o + 128 * k, IDESC_Y, k > 0);
-                        tc_mma_bf16_ta(tD + 64 * buf, tT + 128 + k * 8, b00 + o + 128 * k, IDESC_Y, 1);
-                    }
-                    tc_commit(smem_u32(&d2_full[buf]));
+                    if (adapted) {
+                        for (int k = 0; k < p.R / 16; k++) {
+                            tc_mma_bf16_ta(tD + 64 * buf, tT + k * 8, b00 + o + 128 * k, IDESC_Y, k > 0);
+                            tc_mma_bf16_ta(tD + 64 * buf, tT + 128 + k * 8, b00 + o + 128 * k, IDESC_Y, 1);
+                        }
+                        tc_commit(smem_u32(&d2_full[buf]));
+                    } else mbar_arrive(smem_u32(&d2_full[buf]));
                 }
                 __syncwarp();
                 advance(1);
@@ -712,7 +716,7 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
         // a warp reaches the 32 lanes of tensor memory that its place in the warpgroup gives it
         const int quarter = warp & 3, group = (warp - 2) >> 2, r = 32 * quarter + lane;
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
-        int nb = 0, np = 0, turn = 0;         // turn: blocks of all pairs
+        int nb = 0, np = 0;
         while (!bad && next()) {
             const bool adapted = w.cur >= 0;
             const int own = quarter == 0 ? w.a[0] : quarter == 1 ? w.a[1] : quarter == 2 ? w.a[2] : w.a[3];
@@ -742,12 +746,12 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
                 if (lane == 0) mbar_arrive(smem_u32(t_full));
                 advance(steps);
             }
-            for (int b = b0; b < b1; b++, turn++) {
-                const int buf = nb & 3, at = nb;
-                if (adapted) nb++;
-                if ((turn & 1) != group) { advance(1); continue; }
-                if ((bad = at_all_wait(smem_u32(&full[s]), phase, abort_flag, 168))) break;
-                if (adapted && (bad = at_all_wait(smem_u32(&d2_full[buf]), (uint32_t)(at / 4) & 1u, abort_flag, 169))) break;
+            for (int b = b0; b < b1; b++, nb++) {
+                const int buf = nb & 3;
+                if ((nb & 1) != group) { advance(1); continue; }
+                // (the sum first: then the stage has its turn, which the group alone, seeing every second one, could not tell from an earlier one)
+                if ((bad = at_all_wait(smem_u32(&d2_full[buf]), (uint32_t)(nb / 4) & 1u, abort_flag, 168))) break;
+                if ((bad = at_all_wait(smem_u32(&full[s]), phase, abort_flag, 169))) break;
                 uint8_t *tile = lc_s + s * STAGE;
                 if (adapted && keep) {
                     tc_fence_after();
@@ -773,7 +777,7 @@ __global__ void __launch_bounds__(LC_T, 1) k_lora_tc(const __grid_constant__ LcP
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (adapted && lane == 0) mbar_arrive(smem_u32(&d2_empty[buf]));
+                if (lane == 0) mbar_arrive(smem_u32(&d2_empty[buf]));
                 if (whole) {
                     fence_proxy_async();
                     __syncwarp();

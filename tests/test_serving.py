@@ -1132,3 +1132,31 @@ def test_every_form_may_be_captured_before_it_ever_ran(cuda):
     """The first calls of a process under capture, for every kernel with an attribute or tensor maps of its own."""
     r = _fresh_process(_COLD)
     assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------ adapters: rows without one in the tiles of 128
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,R,n", [(4200, 136, 1544, 16, 3), (4200, 2056, 1544, 16, 3), (6000, 72, 2056, 32, 2), (5000, 64, 1032, 256, 4), (4100, 200, 4104, 176, 1), (3000, 1032, 520, 64, 9), (20000, 72, 72, 16, 2)])
+@pytest.mark.parametrize("mode", ["mixed", "runs", "first", "every other tile"])
+def test_lora_tiles_with_rows_without_an_adapter(cuda, M, K, N, R, n, mode):
+    """Pairs of a tile and no adapter, with more blocks of columns than the ring has stages, in front of and between pairs with one."""
+    from cudalm_c_b200 import linear
+    X, base, A, Bm, scale = make_lora(M, K, N, R, n, torch.bfloat16, M + N, cuda)
+    rs = np.random.RandomState(M + R)
+    a = rs.randint(-1, n, size=M)
+    if mode == "runs":
+        a = np.sort(a)
+    elif mode == "first":
+        a = np.where(np.arange(M) % 128 < 5, -1, a)
+    elif mode == "every other tile":
+        a = np.where(np.arange(M) // 128 % 2 == 0, -1, np.arange(M) // 256 % n)
+    adapter = torch.from_numpy(a.astype(np.int32)).to(cuda)
+    b0 = base.clone()
+    for _ in range(3):
+        y = linear.lora_add(X, base, A, Bm, scale, adapter)
+        ok()
+        check_lora(y, X, base, A, Bm, scale, adapter)
+    assert torch.equal(base, b0)
+    y2 = linear.lora_add(X, base, A, Bm, scale, adapter, out=base)
+    ok()
+    assert torch.equal(y2, y)
