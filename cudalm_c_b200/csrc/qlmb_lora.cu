@@ -1140,8 +1140,14 @@ static LoraForm lora_form(int M, int K, int N, int R, int *S, int *kslice)
 //   where rows come in no order with many adapters, or a small rank: K 768, N 1536, R 64: 512 / 8 14.6 and 21.6, 1024 / 16 28.9 and 39.4,
 //   1024 / 32 47.9 and 44.7; K 768, N 768, R 16: 512 / 16 22.9 and 9.6, 512 / 64 67 and 9.3 (above 2048 the tiles of 64 are no better: K 768,
 //   N 1536, R 64: 4096 / 64 255 and 581).
+// Above them, up to 8192 rows of R 16, LORA_TWO's are so where K is large and N is not, whatever the rows' order: K 2048, N 2048: 2056 / 9 25.5 and
+// 19.0, in no order 43.6 and 32.1, 4096 / 9 28.4 and 28.0; K 4096, N 1024: 4096 / 9 41.5 and 31.8; N 4096: 2056 / 9 44.5 and 25.3, 3300 / 9 47.2
+// and 50.9; K 2048, N 6144: 3300 / 9 35.4 and 41.8; N 16384: K 4096, 2560 / 9 68 and 81; K 1536, N 1536: 2056 / 3 13.9 and 17.4.  Elsewhere it goes
+// by the order, which the host does not see: K 768, N 768: 4096 / 9 11.8 and 19.8, 4096 / 64 19.0 and 20.0, 4096 / 200 31.6 and 20.7; in no order 34.9
+// and 31.1, 164 and 40, 278 and 41 (8192 / 64 308 and 75).  Rows in no order come with `order`, and then take no TC.
 static bool lora_tc_ok(int M, int K, int N, int R, int adapters)
 {
+    if (R == 16 && K >= 2048 && M <= 8192 && (long long)M * N <= 3000LL * K) return false;
     return R % 16 == 0 && (M > 2048 || (M >= 512 && K <= 1024 && R >= 32 && adapters <= 16)) && (M + 127) / 128 <= LC_TILES && (long long)M * ((N + 63) / 64) < (1LL << 31) &&
            (long long)adapters * R < (1LL << 31);
 }

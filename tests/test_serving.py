@@ -1160,3 +1160,11 @@ def test_lora_tiles_with_rows_without_an_adapter(cuda, M, K, N, R, n, mode):
     y2 = linear.lora_add(X, base, A, Bm, scale, adapter, out=base)
     ok()
     assert torch.equal(y2, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,R,n", [(2180, 4104, 8, 32, 2), (4200, 2056, 1544, 16, 3), (4100, 2048, 1496, 16, 9), (3000, 2048, 2056, 16, 70), (8200, 2048, 72, 16, 5), (2049, 2040, 264, 16, 40)])
+@pytest.mark.parametrize("mode", ["runs", "mixed"])
+def test_lora_of_many_rows_and_a_large_k(cuda, M, K, N, R, n, mode):
+    """Both sides of the border between tiles of 128 rows and two launches."""
+    test_lora(cuda, M, K, N, R, n, torch.bfloat16, mode)
