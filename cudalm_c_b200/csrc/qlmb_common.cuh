@@ -50,7 +50,11 @@ struct ProfScope {
 // anything that a kernel may write: activations, but the weights too (codes, scales, gains, the router matrix, the
 // embedding), for the kernel in front may be an optimizer's.  That a writer does not trigger is not enough: its successor
 // then starts when its blocks are done, but sees its stores only behind the wait.  Only where `weights_quiet` answers
-// QUIET, no writer of weights being able to run or to be unseen, are they loaded ahead of it.  (Prefetches into L2 ahead of
+// QUIET, no writer of weights being able to run or to be unseen, are they loaded ahead of it.  The other exception are kernels that only ever
+// follow a kernel of the same call which waits before it triggers (k_px_mma<true> behind k_px_tc, k_lora_up<.., true> behind k_lora_down):
+// every launch in front of that one has then ended, and its stores are visible, when they start, so that they may, ahead of their wait, read
+// whatever the kernel in front does not write, by loads that pass by L1, and write what it neither reads nor writes.  Their wait comes
+// before they read its results, and on every way out: what follows them relies on it.  (Prefetches into L2 ahead of
 // the wait, which would be allowed, cost more than they gain: a streaming GEMV of 4096 x 16384 14.3 -> 15 us.)
 // The caller decides per launch (`early`): with one to four rows per step the early blocks of the decode chain cost the
 // running kernel more than they gain (decode step 0.53 -> 0.56 ms at one slot, 0.85 -> 0.81 ms at eight, CUDA events).

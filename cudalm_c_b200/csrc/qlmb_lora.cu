@@ -1109,7 +1109,7 @@ template <bool F32, bool NARROW, bool AHEAD> __global__ void __launch_bounds__(1
 //                             9.7; K 2048, N 2048, R 16: 64 / 64 7.2 and 8.1; K 768, N 4096, R 16: 8 / 8 4.5 and 5.5, 64 / 64 10.4 and
 //                             7.4; K 768, N 16384, R 16: 1 row 5.7 and 5.5, 64 / 64 30.8 and 15.1
 //                             K 768, N 1536, R 64 (K R 49152): 64 rows 14.2 and 10.3
-//   ONE up to 32 rows, N of 4096 and K R of 65536: K 1024, N 1024, R 64: 1 row 7.5 and 9.2, 32 7.9 and 9.6; K 4096, R 16: N 768 1 row 5.5 and 5.5, 32 5.8
+//   ONE up to 32 rows, N of 2048 (4096 where M N is at most 32768) and K R of 65536: K 1024, N 1024, R 64: 1 row 7.5 and 9.2, 32 7.9 and 9.6; K 4096, R 16: N 768 1 row 5.5 and 5.5, 32 5.8
 //                             and 6.7, N 4096 4 rows 6.2 and 5.6 (fp32 rows 2.4 more than LORA_TWO), and 4 us less of the host; K R 131072:
 //                             K 4096, N 2048, R 32: 4 rows 13.0 and 6.9; K 2048, N 16384, R 24: 1 row 10.9 and 6.9
 enum LoraForm { LORA_ONE, LORA_TWO, LORA_TILE, LORA_TC };

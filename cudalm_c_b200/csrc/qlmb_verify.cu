@@ -11,6 +11,10 @@
 // A slot is a cluster of eight CTAs, a row of logits is cut into runs, one a warp.  A lane keeps maximum, lowest index of it and
 // the two sums (T, and 1 for the log-probability) of what it reads, rescaled as the maximum moves; lanes are joined at the end of a
 // run, warps and CTAs through (distributed) shared memory.  The run that holds the draw is read once more.
+//
+// Measured over twelve sets of drafts (median, least and most; the rows that the longest slot reads): 1 slot of 16384 fp32 logits, four drafts
+// 11.8 us (8.3 to 12.0; 1 to 5 rows), 64 of them, a third greedy, 14.4 (14.0 to 15.6; 4 or 5), bf16 17.1 (16.4 to 18.1), 32 of 130001, seven drafts
+// 27.4 (19 to 49; 1 to 8), 8 of 65536 18.8 (18.8 to 19.2; 4 or 5).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
@@ -385,11 +389,12 @@ extern "C" int qlmb_dec_verify(int *out, int *count, float *lp, const void *logi
     if (B <= 0) return QLMB_OK;
     QLMB_REQUIRE(B < (1 << 24), "qlmb_dec_verify: %d slots", B);
     // A round (a group of rows, the cluster's meeting, the test) costs about 2.5 us beside the reading, and rows behind the end are read for
-    // nothing.  Vocabularies of up to 32768: four warps a CTA, so that the 64 clusters of a full server run at once, and two rows a
-    // round (64 slots of 16384, five rows: 15.5 us; one row a round 17.8, all five rows 16.0, eight warps 23.0; 64 of 32768 23.3, eight warps
-    // 24.7).  Above: eight warps, and two rows where drafts come with probabilities, since those are mostly taken (8 slots of 130048, five
-    // rows 35.4, one row 38.3; 16 of 65536 21.0 and 23.9; four warps 59.2 and 24.2), one where they do not (32 slots of 130001, eight
-    // rows: 26.9 us; two rows 28.9, four warps 33.4).
+    // nothing.  Means over eight sets of drafts (a call lasts as long as its longest slot, see k_dec_verify's figures), us.  Vocabularies of up
+    // to 32768: four warps a CTA, so that the 64 clusters of a full server run at once, and two rows a round (64 slots of 16384, up to five
+    // rows: 16.0; one row a round 18.3, all five 16.5, eight warps 23.5; 64 of 32768 21.7, eight warps 24.0).  Above: eight warps, and two
+    // rows where drafts come with probabilities, since those are mostly taken (8 slots of 130048, up to five rows 29.6, one row 31.8, four
+    // warps 42.6; 16 of 65536 21.5, 24.3 and 25.2), one where they do not (32 slots of 130001, up to eight rows: 26.8; two rows 29.4, four
+    // warps 31.8).
     const bool wide = V > 32768, bf = lg_dtype == QLMB_BF16, vec = ld % 4 == 0 && ((uintptr_t)logits & (bf ? 7 : 15)) == 0;
     VerifyParams p = {out, count, lp, logits, q, u, temp, draft, nd, B, n, V, wide && !q ? 1 : 2, ld, ldq, device_error_word()};
     void (*kern)(const VerifyParams);

@@ -77,7 +77,8 @@ def gemv_decode(X, codes, scales, layout, N, out=None):
 
 
 def lora_order(adapter):
-    """The rows in the order of their adapters (int32), for lora_add: made once for as long as a batch stays the same."""
+    """The rows in the order of their adapters (int32), for lora_add: made once for as long as a batch stays the same.  For rows in no
+    order, as slots are; rows that stand in runs, as prompts do, are faster without it."""
     return torch.argsort(adapter, stable=True).to(torch.int32)
 
 
